@@ -390,6 +390,155 @@ int mfc_sdpa_static_dev(int32_t num_attn_heads, int32_t num_kv_heads, int32_t kv
                         const void *k_cache, const void *v_cache, float *out, void *stream);
 int mfc_sdpa_static_status(void *stream);
 
+/* ------------------------------------------------------------------------
+ * Serving a batch from cached rows.  None of these calls has a counterpart in
+ * the reference (it serves one sequence); they work on rows that the caller
+ * holds, or that a context holds (mfc_kv_cache_view), and keep no state of
+ * their own.  All pointers inside the structs are device pointers on the
+ * context's device; the struct itself is host memory and is read before the
+ * call returns.  Asynchronous on mfc_stream(ctx), usable in a stream capture;
+ * nothing is allocated.  Calls of one context use its scratch and are ordered
+ * by its stream: graphs captured from one context must not be replayed side by
+ * side.  head_dim is 256.  Strides are in elements.  Return 0 on success, -1
+ * on a refused argument (nothing was launched).  Lengths read from device
+ * memory are checked by the kernels: a sequence whose length lies outside
+ * [0, capacity] is treated as empty and reported by mfc_synchronize.
+ * ---------------------------------------------------------------------- */
+
+/* Where a full-attention layer's rows of one sequence live: *k and *v point at
+ * row 0 of kv head 0; the next head starts *head_stride elements later, the
+ * same layer's next sequence *seq_stride elements later, the next row 256
+ * elements later; *len rows are in use (of the context's kv_dtype).  Rows up to
+ * the layer's length may be read until the sequence is cleared, truncated or
+ * reloaded. */
+int mfc_kv_cache_view(mfc_ctx *ctx, int32_t layer, int32_t seq_id, void **k, void **v,
+                      int64_t *seq_stride, int64_t *head_stride, int32_t *len);
+
+/* Attention of a batch whose sequences share a long prefix.  Query token t of
+ * sequence b attends to all prefix_len prefix rows and to the sequence's own
+ * rows j < own_lens[b] - (n_tokens - 1 - t): the n_tokens newest rows are the
+ * step's own tokens, causal among themselves (n_tokens > 1: drafted tokens that
+ * are being verified).  The prefix rows are stored once and read once for all
+ * sequences.
+ *   q, gate: bf16, element (b, t, h, d) at b*seq + t*token + h*head + d; q is
+ *     post-RoPE; gate NULL = no sigmoid gate.
+ *   prefix_k/_v: bf16 [kv head][prefix_len][256] by the two strides.
+ *   own_k/_v: bf16 [seq][kv head][own_cap][256] by the three strides; rows at
+ *     and beyond own_lens[b] are never used, whatever they hold.  Every row
+ *     below own_lens[b] enters the products of all n_tokens queries, with weight
+ *     zero where a query does not see it: V must be finite there.
+ *   own_lens: int32 [n_seqs] in device memory, the new rows included.
+ *   out: bf16 [n_seqs][n_tokens][heads][256];  lse: fp32 [n_seqs][n_tokens][heads],
+ *     ln sum exp of the scaled scores, or NULL.
+ * A query that sees no row at all gets out = 0 and lse = -inf.  Strides are
+ * multiples of 8, pointers 16-byte aligned.  1 <= n_tokens <= 16, n_seqs <= 4096,
+ * at most 16 query heads per kv head. */
+typedef struct mfc_shared_prefix_attn {
+    int32_t n_seqs, n_tokens, num_attn_heads, num_kv_heads;
+    float softmax_scale;
+    const void *q;
+    int64_t q_seq_stride, q_token_stride, q_head_stride;
+    const void *gate;
+    int64_t gate_seq_stride, gate_token_stride, gate_head_stride;
+    const void *prefix_k, *prefix_v;
+    int64_t prefix_head_stride, prefix_row_stride;
+    int32_t prefix_len;
+    const void *own_k, *own_v;
+    int64_t own_seq_stride, own_head_stride, own_row_stride;
+    int32_t own_cap;
+    const int32_t *own_lens;
+    void *out;
+    float *lse;
+} mfc_shared_prefix_attn;
+int mfc_shared_prefix_attn_dev(mfc_ctx *ctx, const mfc_shared_prefix_attn *args);
+
+/* The attention weight that cached rows received in a step, added to a running
+ * sum per row (what an eviction policy ranks rows by):
+ *   weights[b][hk][j] = decay * weights[b][hk][j]
+ *       + sum over tokens t and the query heads h of kv head hk of
+ *         exp(scale * q[b][t][h] . k[b][hk][j] - lse[b][t][h])
+ * for j < lens[b], the sum taken over the tokens that see row j (as above:
+ * j < lens[b] - (n_tokens - 1 - t)); other rows of `weights` are left as they
+ * were.  lse is what mfc_shared_prefix_attn_dev returned, so weights taken with a
+ * shared prefix are shares of the whole softmax.  q, k bf16, lse and weights
+ * fp32.  Strides of q and k are multiples of 8, their pointers 16-byte aligned. */
+typedef struct mfc_attn_weights {
+    int32_t n_seqs, n_tokens, num_attn_heads, num_kv_heads;
+    float softmax_scale, decay;
+    const void *q;
+    int64_t q_seq_stride, q_token_stride, q_head_stride;
+    const void *k;
+    int64_t k_seq_stride, k_head_stride, k_row_stride;
+    int32_t cap;
+    const int32_t *lens;
+    const float *lse;
+    float *weights;
+    int64_t weights_seq_stride, weights_head_stride;
+} mfc_attn_weights;
+int mfc_attn_weights_accumulate_dev(mfc_ctx *ctx, const mfc_attn_weights *args);
+
+/* Eviction: every (sequence, kv head) with lens[b] > budget rows keeps the
+ * `budget` rows of the largest weight, in place.  Rows whose position is below
+ * n_sink or at least next_pos[b] - n_recent are protected and rank before all
+ * others; a NaN weight ranks last; ties go to the lowest row.  The result's row r < min(lens[b], budget) is the old row r if it was kept, else
+ * the next kept row from beyond the budget: the j-th evicted row below the
+ * budget receives the j-th kept row at or above it (attention does not depend on
+ * the order of rows whose keys are already rotated; `positions` says which
+ * position a row holds).  K and V rows outside the evicted places are not
+ * written.
+ *   k, v: [seq][kv head][cap][256] of kv_dtype by the three strides;
+ *   weights, positions (int32): element (b, hk, row) at b*map_seq + hk*map_head + row;
+ *   weights_out, positions_out: same strides, may be weights and positions
+ *     themselves; rows [0, min(lens[b], budget)) are written;
+ *   lens, next_pos: int32 [n_seqs]; lens_out[b] = min(lens[b], budget), not lens.
+ * cap <= MFC_EVICT_MAX_ROWS, pointers 16-byte aligned, K and V strides multiples
+ * of 16 bytes. */
+#define MFC_EVICT_MAX_ROWS 262144
+typedef struct mfc_kv_evict {
+    int32_t n_seqs, num_kv_heads, kv_dtype, cap;
+    void *k, *v;
+    int64_t seq_stride, head_stride, row_stride;
+    int32_t budget, n_sink, n_recent;
+    const int32_t *lens, *next_pos;
+    const float *weights;
+    const int32_t *positions;
+    int64_t map_seq_stride, map_head_stride;
+    float *weights_out;
+    int32_t *positions_out;
+    int32_t *lens_out;
+} mfc_kv_evict;
+int mfc_kv_evict_dev(mfc_ctx *ctx, const mfc_kv_evict *args);
+
+/* Verification of drafted tokens from given uniforms in [0, 1): draft i of
+ * sequence b is accepted while u_accept[b][i] * q_i(x_i) < p_i(x_i) (evaluated
+ * exactly), p = target_probs[b][i], q = draft_probs[b][i]; n_accepted[b] counts
+ * the drafts before the first refusal.  The token after them is drawn from
+ * max(p - q, 0) at the refused place, or from p behind the last draft when none
+ * was refused: the lowest v whose cumulative weight exceeds u_sample[b] times the
+ * total, sums in 64 bits.  If that residual is zero everywhere the token is drawn
+ * from p; if p is zero too it is -1.  Entries that are negative or NaN count as
+ * zero.  draft_probs NULL: the drafts were not sampled (q is 1 at x_i).  A drafted
+ * token outside [0, vocab) is refused.
+ *   target_probs: fp32 [n_seqs][max_drafts + 1][vocab], draft_probs: fp32
+ *     [n_seqs][max_drafts][vocab] by their strides;
+ *   draft_tokens int32, u_accept fp32: [n_seqs][max_drafts];  u_sample [n_seqs];
+ *   draft_lens: int32 [n_seqs], drafts in use, or NULL = max_drafts; a negative
+ *     length marks an idle place (n_accepted 0, tokens -1);
+ *   tokens: int32 [n_seqs][max_drafts + 1]: the accepted drafts, the drawn token,
+ *     then -1.
+ * 0 <= max_drafts <= 32. */
+typedef struct mfc_verify_drafts {
+    int32_t n_seqs, max_drafts, vocab;
+    const float *target_probs;
+    int64_t target_seq_stride, target_row_stride;
+    const float *draft_probs;
+    int64_t draft_seq_stride, draft_row_stride;
+    const int32_t *draft_tokens, *draft_lens;
+    const float *u_accept, *u_sample;
+    int32_t *n_accepted, *tokens;
+} mfc_verify_drafts;
+int mfc_verify_drafts_dev(mfc_ctx *ctx, const mfc_verify_drafts *args);
+
 /* ---- The step either side of the path: 4-bit affine-quantised projections ----
  * Replaces dequant_matvec_4bit_cpu (crates/moeflux/src/riir/cpu_matvec.rs:83-171) and the
  * GPU dispatch encode_matvec (riir/gpu_matvec.rs:84-129; kernels dequant_matvec_4bit_v3 /

@@ -46,6 +46,117 @@ class Config(C.Structure):
     ]
 
 
+class SharedPrefixAttn(C.Structure):
+    """``mfc_shared_prefix_attn``"""
+
+    _fields_ = [
+        ("n_seqs", C.c_int32),
+        ("n_tokens", C.c_int32),
+        ("num_attn_heads", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("softmax_scale", C.c_float),
+        ("q", C.c_void_p),
+        ("q_seq_stride", C.c_int64),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("gate", C.c_void_p),
+        ("gate_seq_stride", C.c_int64),
+        ("gate_token_stride", C.c_int64),
+        ("gate_head_stride", C.c_int64),
+        ("prefix_k", C.c_void_p),
+        ("prefix_v", C.c_void_p),
+        ("prefix_head_stride", C.c_int64),
+        ("prefix_row_stride", C.c_int64),
+        ("prefix_len", C.c_int32),
+        ("own_k", C.c_void_p),
+        ("own_v", C.c_void_p),
+        ("own_seq_stride", C.c_int64),
+        ("own_head_stride", C.c_int64),
+        ("own_row_stride", C.c_int64),
+        ("own_cap", C.c_int32),
+        ("own_lens", C.c_void_p),
+        ("out", C.c_void_p),
+        ("lse", C.c_void_p),
+    ]
+
+
+class AttnWeights(C.Structure):
+    """``mfc_attn_weights``"""
+
+    _fields_ = [
+        ("n_seqs", C.c_int32),
+        ("n_tokens", C.c_int32),
+        ("num_attn_heads", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("softmax_scale", C.c_float),
+        ("decay", C.c_float),
+        ("q", C.c_void_p),
+        ("q_seq_stride", C.c_int64),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k", C.c_void_p),
+        ("k_seq_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("k_row_stride", C.c_int64),
+        ("cap", C.c_int32),
+        ("lens", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("weights_seq_stride", C.c_int64),
+        ("weights_head_stride", C.c_int64),
+    ]
+
+
+class KvEvict(C.Structure):
+    """``mfc_kv_evict``"""
+
+    _fields_ = [
+        ("n_seqs", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("kv_dtype", C.c_int32),
+        ("cap", C.c_int32),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("seq_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("row_stride", C.c_int64),
+        ("budget", C.c_int32),
+        ("n_sink", C.c_int32),
+        ("n_recent", C.c_int32),
+        ("lens", C.c_void_p),
+        ("next_pos", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("map_seq_stride", C.c_int64),
+        ("map_head_stride", C.c_int64),
+        ("weights_out", C.c_void_p),
+        ("positions_out", C.c_void_p),
+        ("lens_out", C.c_void_p),
+    ]
+
+
+class VerifyDrafts(C.Structure):
+    """``mfc_verify_drafts``"""
+
+    _fields_ = [
+        ("n_seqs", C.c_int32),
+        ("max_drafts", C.c_int32),
+        ("vocab", C.c_int32),
+        ("target_probs", C.c_void_p),
+        ("target_seq_stride", C.c_int64),
+        ("target_row_stride", C.c_int64),
+        ("draft_probs", C.c_void_p),
+        ("draft_seq_stride", C.c_int64),
+        ("draft_row_stride", C.c_int64),
+        ("draft_tokens", C.c_void_p),
+        ("draft_lens", C.c_void_p),
+        ("u_accept", C.c_void_p),
+        ("u_sample", C.c_void_p),
+        ("n_accepted", C.c_void_p),
+        ("tokens", C.c_void_p),
+    ]
+
+
 _F = C.POINTER(C.c_float)
 _I = C.POINTER(C.c_int32)
 _U16 = C.POINTER(C.c_uint16)
@@ -114,6 +225,12 @@ SIGNATURES = {
     "mfc_mla_sdpa_folded_dev": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_float, _P, _P, _P, _P, _P]),
     "mfc_mla_sdpa_folded_bf16_dev": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_float, _P, _P, _P, _P, _P]),
     "mfc_mla_sdpa_folded": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_float, _F, _F, _F, _F, _F]),
+    "mfc_kv_cache_view": (C.c_int, [_P, C.c_int32, C.c_int32, C.POINTER(_P), C.POINTER(_P), C.POINTER(C.c_int64),
+                                    C.POINTER(C.c_int64), _I]),
+    "mfc_shared_prefix_attn_dev": (C.c_int, [_P, C.POINTER(SharedPrefixAttn)]),
+    "mfc_attn_weights_accumulate_dev": (C.c_int, [_P, C.POINTER(AttnWeights)]),
+    "mfc_kv_evict_dev": (C.c_int, [_P, C.POINTER(KvEvict)]),
+    "mfc_verify_drafts_dev": (C.c_int, [_P, C.POINTER(VerifyDrafts)]),
     "mfc_set_tuning": (C.c_int, [_P, C.c_char_p, C.c_int]),
     "mfc_launch_count": (C.c_longlong, [_P]),
 }

@@ -98,6 +98,7 @@ struct mfc_ctx {
     unsigned *tickets = nullptr, *group_tickets = nullptr, *status = nullptr;
     unsigned *mv_sched = nullptr;  // two pairs (tile counter, finished CTAs) of the one-vector projection kernel, used in turn
     unsigned mv_launches = 0;
+    int *serve_plan = nullptr;     // tile plan of a shared-prefix attention call (written by its main kernel, read by its merge)
     bool mv_overlap = true;        // tuning "matvec_overlap"
     struct MvMap {
         const uint32_t *w;
@@ -864,6 +865,7 @@ mfc_ctx *mfc_open(const mfc_config *cfg) {
          DA(sc_o, (size_t)c->max_parts * 16 * HEAD_DIM, false) && DA(sc_m, (size_t)c->max_parts * 16, false) &&
          DA(sc_l, (size_t)c->max_parts * 16, false) && DA(tickets, mb * g.num_kv_heads, true) &&
          DA(group_tickets, c->max_parts, true) && DA(status, 1, true) && DA(mv_sched, 4, true) &&
+         DA(serve_plan, SHARED_ATTN_PLAN_INTS, true) &&
          DA(phase_trace, (size_t)mfc_ctx::MAX_TRACE_CTAS * PHASE_TRACE_WORDS, true) && DA(st_q, mb * qd, false) &&
          DA(st_gate, mb * qd, false) && DA(st_k, mb * kvd, false) && DA(st_v, mb * kvd, false) &&
          DA(st_out, mb * qd, false) && DA(st_qkv, mb * c->conv_dim, false) && DA(st_z, mb * vd, false) &&
@@ -900,7 +902,9 @@ mfc_ctx *mfc_open(const mfc_config *cfg) {
     if (ok && gdn_prefill_configure() != cudaSuccess) ok = fail(c, "cannot opt in to the prefill kernel's shared memory size");
     if (ok && gqa_prefill_configure() != cudaSuccess) ok = fail(c, "cannot opt in to the prefill kernel's shared memory size");
     if (ok && (gqa_decode_configure() != cudaSuccess || gqa_decode_f32_configure() != cudaSuccess ||
-               mla_decode_configure() != cudaSuccess))
+               mla_decode_configure() != cudaSuccess || verify_drafts_configure() != cudaSuccess ||
+               kv_evict_configure() != cudaSuccess || attn_weights_configure() != cudaSuccess ||
+               shared_prefix_attn_configure() != cudaSuccess))
         ok = fail(c, "cannot opt in to the kernels' shared memory size");
     if (ok) c->coop_capacity = g.kv_dtype == MFC_KV_BF16 ? gqa_decode_bf16_coop_capacity() : gqa_decode_f32_coop_capacity();
     if (!ok) {
@@ -1453,6 +1457,347 @@ int mfc_mla_sdpa_folded(mfc_ctx *c, int32_t num_heads, int32_t cache_len, float 
     cudaStreamSynchronize(c->stream);
     cudaFree(d);
     return rc;
+}
+
+// ---------------------------------------------------------------- serving a batch from cached rows
+
+namespace {
+// The context's device for the duration of a call; the caller's current device comes back afterwards.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(int dev) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        if (before != dev) cudaSetDevice(dev);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+bool misaligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
+
+// head layout shared by the attention calls
+bool check_heads(mfc_ctx *c, int n_seqs, int n_tokens, int H, int Hkv, float scale) {
+    if (n_seqs < 0 || n_seqs > SHARED_ATTN_MAX_SEQS) return fail(c, "n_seqs must be in [0, 4096]");
+    if (n_tokens < 1 || n_tokens > 16) return fail(c, "n_tokens must be in [1, 16]");
+    if (H <= 0 || Hkv <= 0 || Hkv > 1024 || H % Hkv != 0 || H / Hkv > 16)
+        return fail(c, "bad head geometry: need num_attn_heads % num_kv_heads == 0, a group of at most 16 and at most 1024 kv heads");
+    if (!(scale > 0.0f) || !(scale < INFINITY)) return fail(c, "softmax_scale must be positive and finite");
+    return true;
+}
+bool strides8(int64_t a, int64_t b, int64_t d) { return a % 8 == 0 && b % 8 == 0 && d % 8 == 0; }
+
+// Map over cached bf16 rows (dim 256, row, kv head[, sequence]), boxes of 64 dims x box_rows rows.
+bool make_rows_map(mfc_ctx *c, CUtensorMap *map, const void *base, int64_t rows, int64_t row_stride, int heads, int64_t head_stride,
+                   int seqs, int64_t seq_stride, int rank, int box_rows) {
+    static EncodeTiledFn encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
+        return e == cudaSuccess && qres == cudaDriverEntryPointSuccess ? (EncodeTiledFn)fn : nullptr;
+    }();
+    if (!encode) return fail(c, "cuTensorMapEncodeTiled is not available from the driver");
+    // the stride of an axis of one element is never used; any valid one will do
+    if (heads == 1) head_stride = row_stride;
+    if (seqs == 1) seq_stride = row_stride;
+    const int64_t most = (int64_t)1 << 39;  // the encoder's limit, in elements of two bytes
+    if (row_stride < HEAD_DIM || row_stride >= most || head_stride <= 0 || head_stride >= most || seq_stride <= 0 || seq_stride >= most)
+        return fail(c, "the strides of cached rows must be positive, at least 256 elements between rows, and below 2^39");
+    cuuint64_t dims[4] = {(cuuint64_t)HEAD_DIM, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)seqs};
+    cuuint64_t strides[3] = {(cuuint64_t)row_stride * 2, (cuuint64_t)head_stride * 2, (cuuint64_t)seq_stride * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(c, "cuTensorMapEncodeTiled failed, code " + std::to_string((int)r));
+    return true;
+}
+}  // namespace
+
+int mfc_kv_cache_view(mfc_ctx *c, int32_t layer, int32_t seq_id, void **k, void **v, int64_t *seq_stride, int64_t *head_stride,
+                      int32_t *len) {
+    if (!c) return -1;
+    if (!k || !v || !seq_stride || !head_stride || !len) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (layer < 0 || layer >= c->cfg.num_layers || c->layer_to_full[layer] < 0 || seq_id < 0 || seq_id >= c->cfg.n_seqs) {
+        fail(c, "not a full-attention layer, or seq_id out of range");
+        return -1;
+    }
+    const size_t slot = (size_t)c->layer_to_full[layer] * c->cfg.n_seqs + seq_id;
+    const size_t per_head = (size_t)c->cap_rows * HEAD_DIM, per_slot = per_head * c->cfg.num_kv_heads;
+    *k = (uint8_t *)c->k_cache + slot * per_slot * c->kv_esize;
+    *v = (uint8_t *)c->v_cache + slot * per_slot * c->kv_esize;
+    *seq_stride = (int64_t)per_slot;
+    *head_stride = (int64_t)per_head;
+    *len = local_len_of(c->kv_len[slot], c->cfg.kv_rank, c->cfg.kv_world, c->cfg.kv_block);
+    return 0;
+}
+
+int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try {
+    if (!c) return -1;
+    if (!a) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (!check_heads(c, a->n_seqs, a->n_tokens, a->num_attn_heads, a->num_kv_heads, a->softmax_scale)) return -1;
+    if (a->n_seqs == 0) return 0;
+    if (a->prefix_len < 0 || a->own_cap < 0) {
+        fail(c, "prefix_len and own_cap must not be negative");
+        return -1;
+    }
+    const bool has_prefix = a->prefix_len > 0, has_own = a->own_cap > 0;
+    if (!a->q || !a->out || !a->own_lens || (has_prefix && (!a->prefix_k || !a->prefix_v)) || (has_own && (!a->own_k || !a->own_v))) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (misaligned(a->q, 16) || misaligned(a->gate, 16) || misaligned(a->out, 16) || misaligned(a->prefix_k, 16) ||
+        misaligned(a->prefix_v, 16) || misaligned(a->own_k, 16) || misaligned(a->own_v, 16) || misaligned(a->own_lens, 4) ||
+        misaligned(a->lse, 4)) {
+        fail(c, "all arrays must be 16-byte aligned");
+        return -1;
+    }
+    if (!strides8(a->q_seq_stride, a->q_token_stride, a->q_head_stride) ||
+        (a->gate && !strides8(a->gate_seq_stride, a->gate_token_stride, a->gate_head_stride)) ||
+        (has_prefix && !strides8(a->prefix_head_stride, a->prefix_row_stride, 0)) ||
+        (has_own && !strides8(a->own_seq_stride, a->own_head_stride, a->own_row_stride))) {
+        fail(c, "strides must be multiples of 8 elements");
+        return -1;
+    }
+    SharedAttnParams p;
+    memset(&p, 0, sizeof(p));
+    p.B = a->n_seqs;
+    p.T = a->n_tokens;
+    p.H = a->num_attn_heads;
+    p.Hkv = a->num_kv_heads;
+    p.group = p.H / p.Hkv;
+    p.prefix_len = a->prefix_len;
+    p.own_cap = a->own_cap;
+    p.prefix_tiles = (a->prefix_len + SHARED_ATTN_N - 1) / SHARED_ATTN_N;
+    p.prefix_mtiles = (int)(((int64_t)p.B * p.T * p.group + SHARED_ATTN_M - 1) / SHARED_ATTN_M);
+    p.own_mtiles = (p.T * p.group + SHARED_ATTN_M - 1) / SHARED_ATTN_M;
+    p.own_rows = p.T * p.group < SHARED_ATTN_M ? p.T * p.group : SHARED_ATTN_M;
+    const int64_t own_units = (int64_t)p.B * p.Hkv * p.own_mtiles;
+    const int64_t own_tiles = own_units * ((a->own_cap + SHARED_ATTN_N - 1) / SHARED_ATTN_N);
+    const int64_t tiles = (int64_t)p.Hkv * p.prefix_mtiles * p.prefix_tiles + own_tiles;
+    if (tiles >= ((int64_t)1 << 30)) {
+        fail(c, "too many rows and queries in one call");
+        return -1;
+    }
+    p.grid = tiles < c->n_sms ? (int)tiles : c->n_sms;
+    if (p.grid < 1) p.grid = 1;
+    // one slot per (unit, CTA) pair at most: units + CTAs of each kind
+    const int64_t need = ((int64_t)p.Hkv * p.prefix_mtiles + p.grid) * SHARED_ATTN_M + (own_units + p.grid) * p.own_rows;
+    if (need > (int64_t)c->max_parts * 16) {
+        fail(c, "n_seqs * n_tokens * num_attn_heads needs " + std::to_string(need) + " partial rows, the scratch reserved at open holds " +
+                    std::to_string((int64_t)c->max_parts * 16));
+        return -1;
+    }
+    p.q = (const __nv_bfloat16 *)a->q;
+    p.q_seq = a->q_seq_stride;
+    p.q_token = a->q_token_stride;
+    p.q_head = a->q_head_stride;
+    p.gate = (const __nv_bfloat16 *)a->gate;
+    p.g_seq = a->gate_seq_stride;
+    p.g_token = a->gate_token_stride;
+    p.g_head = a->gate_head_stride;
+    p.lens = a->own_lens;
+    p.out = (__nv_bfloat16 *)a->out;
+    p.lse = a->lse;
+    p.part_o = c->sc_o;
+    p.part_m = c->sc_m;
+    p.part_l = c->sc_l;
+    p.plan = c->serve_plan;
+    p.status = c->status;
+    p.scale = a->softmax_scale;
+    CUtensorMap m[4];
+    memset(m, 0, sizeof(m));
+    if (has_prefix && (!make_rows_map(c, &m[0], a->prefix_k, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 3, 128) ||
+                       !make_rows_map(c, &m[1], a->prefix_v, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 3, 32)))
+        return -1;
+    if (has_own && (!make_rows_map(c, &m[2], a->own_k, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 4, 128) ||
+                    !make_rows_map(c, &m[3], a->own_v, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 4, 32)))
+        return -1;
+    DeviceScope dev(c->cfg.device);
+    CK(launch_shared_prefix_attn(m[0], m[1], m[2], m[3], p, c->stream));
+    c->launches += 2;
+    return 0;
+} catch (...) {
+    return -1;
+}
+
+int mfc_attn_weights_accumulate_dev(mfc_ctx *c, const mfc_attn_weights *a) try {
+    if (!c) return -1;
+    if (!a) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (!check_heads(c, a->n_seqs, a->n_tokens, a->num_attn_heads, a->num_kv_heads, a->softmax_scale)) return -1;
+    if (a->cap < 0) {
+        fail(c, "cap must not be negative");
+        return -1;
+    }
+    if (a->n_seqs == 0 || a->cap == 0) return 0;
+    if (!a->q || !a->k || !a->lens || !a->lse || !a->weights) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (misaligned(a->q, 16) || misaligned(a->k, 16) || misaligned(a->lens, 4) || misaligned(a->lse, 4) || misaligned(a->weights, 4)) {
+        fail(c, "q and k must be 16-byte aligned, the other arrays 4-byte aligned");
+        return -1;
+    }
+    if (!strides8(a->q_seq_stride, a->q_token_stride, a->q_head_stride) || !strides8(a->k_seq_stride, a->k_head_stride, a->k_row_stride)) {
+        fail(c, "the strides of q and k must be multiples of 8 elements");
+        return -1;
+    }
+    AttnWeightsParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = (const __nv_bfloat16 *)a->q;
+    p.k = (const __nv_bfloat16 *)a->k;
+    p.q_seq = a->q_seq_stride;
+    p.q_token = a->q_token_stride;
+    p.q_head = a->q_head_stride;
+    p.k_seq = a->k_seq_stride;
+    p.k_head = a->k_head_stride;
+    p.k_row = a->k_row_stride;
+    p.lens = a->lens;
+    p.lse = a->lse;
+    p.w = a->weights;
+    p.w_seq = a->weights_seq_stride;
+    p.w_head = a->weights_head_stride;
+    p.status = c->status;
+    p.B = a->n_seqs;
+    p.T = a->n_tokens;
+    p.H = a->num_attn_heads;
+    p.Hkv = a->num_kv_heads;
+    p.group = p.H / p.Hkv;
+    p.cap = a->cap;
+    p.scale = a->softmax_scale;
+    p.decay = a->decay;
+    DeviceScope dev(c->cfg.device);
+    CK(launch_attn_weights(p, c->n_sms, c->stream));
+    c->launches += 1;
+    return 0;
+} catch (...) {
+    return -1;
+}
+
+int mfc_kv_evict_dev(mfc_ctx *c, const mfc_kv_evict *a) try {
+    if (!c) return -1;
+    if (!a) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (a->n_seqs < 0 || a->n_seqs > SHARED_ATTN_MAX_SEQS || a->num_kv_heads <= 0 || a->num_kv_heads > 1024) {
+        fail(c, "n_seqs must be in [0, 4096] and num_kv_heads in [1, 1024]");
+        return -1;
+    }
+    if (a->kv_dtype != MFC_KV_F32 && a->kv_dtype != MFC_KV_BF16) {
+        fail(c, "kv_dtype must be MFC_KV_F32 or MFC_KV_BF16");
+        return -1;
+    }
+    if (a->cap <= 0 || a->cap > MFC_EVICT_MAX_ROWS || a->budget < 1 || a->n_sink < 0 || a->n_recent < 0) {
+        fail(c, "cap must be in [1, " + std::to_string(MFC_EVICT_MAX_ROWS) + "], budget positive, n_sink and n_recent not negative");
+        return -1;
+    }
+    if (a->n_seqs == 0) return 0;
+    if (!a->k || !a->v || !a->lens || !a->next_pos || !a->weights || !a->positions || !a->weights_out || !a->positions_out || !a->lens_out) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (a->k == a->v || a->lens_out == a->lens || a->lens_out == a->next_pos) {
+        fail(c, "k and v, and lens_out and the input lengths, must be different arrays");
+        return -1;
+    }
+    const int64_t es = a->kv_dtype == MFC_KV_BF16 ? 2 : 4;
+    if (misaligned(a->k, 16) || misaligned(a->v, 16) || (a->seq_stride * es) % 16 || (a->head_stride * es) % 16 || (a->row_stride * es) % 16 ||
+        misaligned(a->lens, 4) || misaligned(a->next_pos, 4) || misaligned(a->weights, 4) || misaligned(a->positions, 4) ||
+        misaligned(a->weights_out, 4) || misaligned(a->positions_out, 4) || misaligned(a->lens_out, 4)) {
+        fail(c, "k, v and their strides must be multiples of 16 bytes, the other arrays 4-byte aligned");
+        return -1;
+    }
+    if (a->row_stride < HEAD_DIM) {
+        fail(c, "rows must be at least 256 elements apart");
+        return -1;
+    }
+    EvictParams p;
+    memset(&p, 0, sizeof(p));
+    p.k = (uint8_t *)a->k;
+    p.v = (uint8_t *)a->v;
+    p.seq_stride = a->seq_stride * es;
+    p.head_stride = a->head_stride * es;
+    p.row_stride = a->row_stride * es;
+    p.row_bytes = (int)(HEAD_DIM * es);
+    p.lens = a->lens;
+    p.next_pos = a->next_pos;
+    p.w = a->weights;
+    p.pos = a->positions;
+    p.map_seq = a->map_seq_stride;
+    p.map_head = a->map_head_stride;
+    p.w_out = a->weights_out;
+    p.pos_out = a->positions_out;
+    p.lens_out = a->lens_out;
+    p.status = c->status;
+    p.B = a->n_seqs;
+    p.Hkv = a->num_kv_heads;
+    p.cap = a->cap;
+    p.budget = a->budget;
+    p.n_sink = a->n_sink;
+    p.n_recent = a->n_recent;
+    DeviceScope dev(c->cfg.device);
+    CK(launch_kv_evict(p, c->n_sms, c->stream));
+    c->launches += 1;
+    return 0;
+} catch (...) {
+    return -1;
+}
+
+int mfc_verify_drafts_dev(mfc_ctx *c, const mfc_verify_drafts *a) try {
+    if (!c) return -1;
+    if (!a) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (a->n_seqs < 0 || a->n_seqs > SHARED_ATTN_MAX_SEQS || a->max_drafts < 0 || a->max_drafts > 32 || a->vocab < 1 || a->vocab > (1 << 30)) {
+        fail(c, "n_seqs must be in [0, 4096], max_drafts in [0, 32] and vocab in [1, 2^30]");
+        return -1;
+    }
+    if (a->n_seqs == 0) return 0;
+    if (!a->target_probs || !a->u_sample || !a->n_accepted || !a->tokens || (a->max_drafts > 0 && (!a->draft_tokens || !a->u_accept))) {
+        fail(c, "NULL argument");
+        return -1;
+    }
+    if (misaligned(a->target_probs, 4) || misaligned(a->draft_probs, 4) || misaligned(a->draft_tokens, 4) || misaligned(a->draft_lens, 4) ||
+        misaligned(a->u_accept, 4) || misaligned(a->u_sample, 4) || misaligned(a->n_accepted, 4) || misaligned(a->tokens, 4)) {
+        fail(c, "all arrays must be 4-byte aligned");
+        return -1;
+    }
+    VerifyParams p;
+    memset(&p, 0, sizeof(p));
+    p.p = a->target_probs;
+    p.q = a->max_drafts > 0 ? a->draft_probs : nullptr;
+    p.p_seq = a->target_seq_stride;
+    p.p_row = a->target_row_stride;
+    p.q_seq = a->draft_seq_stride;
+    p.q_row = a->draft_row_stride;
+    p.drafts = a->draft_tokens;
+    p.draft_lens = a->draft_lens;
+    p.u_accept = a->u_accept;
+    p.u_sample = a->u_sample;
+    p.n_accepted = a->n_accepted;
+    p.tokens = a->tokens;
+    p.B = a->n_seqs;
+    p.K = a->max_drafts;
+    p.V = a->vocab;
+    DeviceScope dev(c->cfg.device);
+    CK(launch_verify_drafts(p, c->n_sms, c->stream));
+    c->launches += 1;
+    return 0;
+} catch (...) {
+    return -1;
 }
 
 int mfc_set_tuning(mfc_ctx *c, const char *key, int value) {

@@ -282,6 +282,75 @@ size_t dequant_matvec_4bit_smem(int in_dim, int n_vec);
 cudaError_t launch_dequant_matvec_4bit(MatvecBatch mb, const float *x, int in_dim, int n_vec, int n_sms,
                                        cudaStream_t stream, const MatvecMaps *maps = nullptr, int *grid_out = nullptr);
 
+// ---------------------------------------------------------------- serving a batch from cached rows
+struct VerifyParams {
+    const float *p, *q;            // target and draft probabilities; q may be nullptr
+    int64_t p_seq, p_row, q_seq, q_row;
+    const int32_t *drafts, *draft_lens;
+    const float *u_accept, *u_sample;
+    int32_t *n_accepted, *tokens;
+    int B, K, V;
+};
+cudaError_t verify_drafts_configure();
+cudaError_t launch_verify_drafts(const VerifyParams &p, int n_sms, cudaStream_t stream);
+
+struct EvictParams {
+    uint8_t *k, *v;
+    int64_t seq_stride, head_stride, row_stride;  // bytes
+    int row_bytes;                                // 512 or 1024
+    const int32_t *lens, *next_pos;
+    const float *w;
+    const int32_t *pos;
+    int64_t map_seq, map_head;
+    float *w_out;
+    int32_t *pos_out, *lens_out;
+    unsigned *status;
+    int B, Hkv, cap, budget, n_sink, n_recent;
+};
+cudaError_t kv_evict_configure();
+cudaError_t launch_kv_evict(const EvictParams &p, int n_sms, cudaStream_t stream);
+
+struct AttnWeightsParams {
+    const __nv_bfloat16 *q, *k;
+    int64_t q_seq, q_token, q_head, k_seq, k_head, k_row;
+    const int32_t *lens;
+    const float *lse;
+    float *w;
+    int64_t w_seq, w_head;
+    unsigned *status;
+    int B, T, H, Hkv, group, cap;
+    float scale, decay;
+};
+cudaError_t attn_weights_configure();
+cudaError_t launch_attn_weights(const AttnWeightsParams &p, int n_sms, cudaStream_t stream);
+
+constexpr int SHARED_ATTN_MAX_SEQS = 4096;
+constexpr int SHARED_ATTN_PLAN_INTS = SHARED_ATTN_MAX_SEQS + 8;
+constexpr int SHARED_ATTN_M = 128;  // query rows of a tile
+constexpr int SHARED_ATTN_N = 128;  // cached rows of a tile
+struct SharedAttnParams {
+    const __nv_bfloat16 *q, *gate;
+    int64_t q_seq, q_token, q_head, g_seq, g_token, g_head;
+    const int32_t *lens;
+    __nv_bfloat16 *out;
+    float *lse;
+    float *part_o, *part_m, *part_l;  // partials: prefix slots of 128 rows, then own slots of own_rows rows
+    int *plan;                        // [0] tiles per CTA, [1] tiles in all, [8 + b] first tile of sequence b's own rows
+    unsigned *status;
+    int B, T, H, Hkv, group;
+    int prefix_len, own_cap;
+    int prefix_tiles;                 // tiles of 128 prefix rows
+    int prefix_mtiles, own_mtiles;    // tiles of 128 query rows per kv head (prefix), per kv head and sequence (own)
+    int own_rows;                     // rows of an own slot: min(128, T * group)
+    int grid;
+    float scale;
+};
+cudaError_t shared_prefix_attn_configure();
+// pk/ok: maps over K with boxes of 64 dims x 128 rows; pv/ov: maps over V with boxes of 64 dims x 32 rows;
+// prefix maps are 3-D (dim, row, kv head), own maps 4-D (dim, row, kv head, sequence).
+cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &pv, const CUtensorMap &ok,
+                                      const CUtensorMap &ov, const SharedAttnParams &p, cudaStream_t stream);
+
 // Per-thread message of the last failure that had no context (ctx.cu).
 std::string &no_ctx_error();
 

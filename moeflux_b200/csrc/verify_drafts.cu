@@ -1,0 +1,226 @@
+// Verification of drafted tokens from given uniforms (no counterpart in the reference, which decodes one token at a
+// time).
+//
+// Draft i of a sequence is accepted while u_i q_i(x_i) < p_i(x_i): products of two fp32 values are exact in fp64, so the
+// decision is exact.  At the first refusal n the token is drawn from w = max(p_n - q_n, 0), behind the last accepted
+// draft from w = p_n: the lowest v with cumsum(w)[v] > u * sum(w), sums in fp64 (a step of the cumulative sum of 10^5
+// entries is about 10^-5 of the total; fp32 prefix sums would move the border by a hundredth of a step).
+//
+// HBM-bound: of the K+1 rows of a sequence only the refused one of p and q is read, once.  A cluster of CTAs owns a
+// sequence, each a run of `segments` of 1024 entries; a warp sums a segment and keeps the sum in shared memory; the CTAs
+// exchange their totals through distributed shared memory, every CTA finds out whether the border lies in its run, and
+// the one that owns it re-reads the 1024 entries of that segment (from L2).  Order of all sums fixed by the sizes.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace cg = cooperative_groups;
+
+namespace mfc {
+
+namespace {
+
+constexpr int VD_THREADS = 512;
+constexpr int VD_WARPS = VD_THREADS / 32;
+constexpr int VD_SEG = 1024;     // entries of a segment
+constexpr int VD_MAX_SEGS = 512;  // segments of a CTA's run kept in shared memory; longer runs use longer segments
+constexpr int VD_MAX_CLUSTER = 16;
+
+__device__ __forceinline__ double weight(float p, float q) {
+    const double w = (double)p - (double)q;
+    return w > 0.0 ? w : 0.0;  // negative and NaN count as nothing
+}
+
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// entries [v, v + 4) of the row's weights; x: the drafted token whose q is 1 when there are no draft probabilities
+template <bool VEC>
+__device__ __forceinline__ void load_w4(const float *p, const float *q, int x, int v, int V, double (&w)[4]) {
+    float pv[4], qv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (VEC && v + 4 <= V) {
+        const float4 a = *reinterpret_cast<const float4 *>(p + v);
+        pv[0] = a.x; pv[1] = a.y; pv[2] = a.z; pv[3] = a.w;
+        if (q) {
+            const float4 b = *reinterpret_cast<const float4 *>(q + v);
+            qv[0] = b.x; qv[1] = b.y; qv[2] = b.z; qv[3] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            pv[e] = v + e < V ? p[v + e] : 0.0f;
+            if (q) qv[e] = v + e < V ? q[v + e] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = (x == v + e) ? 0.0 : weight(pv[e], qv[e]);
+}
+
+// Sums of the segments [s0, s1) of `seg` entries into s_sum, one warp per segment.
+template <bool VEC>
+__device__ __forceinline__ void sum_segments(const float *p, const float *q, int x, int V, int seg, int s0, int s1, double *s_sum) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int s = s0 + warp; s < s1; s += VD_WARPS) {
+        const int v1 = min((s + 1) * seg, V);
+        double acc = 0.0;
+#pragma unroll 8
+        for (int v = s * seg + 4 * lane; v < v1; v += 128) {
+            double w[4];
+            load_w4<VEC>(p, q, x, v, V, w);
+            acc += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+        acc = warp_sum_f64(acc);
+        if (lane == 0) s_sum[s - s0] = acc;
+    }
+}
+
+__global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyParams p, int seg) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = (int)blockIdx.x / cs;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ double s_sum[VD_MAX_SEGS];
+    __shared__ double s_tot[2];  // this CTA's total, for the first pass and for the pass over p alone
+    __shared__ int s_n;
+
+    const int len = p.draft_lens ? min(p.draft_lens[b], p.K) : p.K;
+    if (warp == 0) {
+        bool refused = false;
+        if (lane < len) {
+            const int x = p.drafts[(size_t)b * p.K + lane];
+            refused = true;
+            if (x >= 0 && x < p.V) {
+                const float px = p.p[(size_t)b * p.p_seq + (size_t)lane * p.p_row + x];
+                const float qx = p.q ? p.q[(size_t)b * p.q_seq + (size_t)lane * p.q_row + x] : 1.0f;
+                refused = !((double)p.u_accept[(size_t)b * p.K + lane] * (double)qx < (double)px);
+            }
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, refused);
+        if (lane == 0) {
+            s_n = m ? __ffs(m) - 1 : max(len, 0);
+        }
+    }
+    __syncthreads();
+    const int n = s_n;
+    if (rank == 0 && tid <= p.K) {  // the accepted drafts, then -1; the drawn token is written behind a cluster barrier
+        p.tokens[(size_t)b * (p.K + 1) + tid] = tid < n ? p.drafts[(size_t)b * p.K + tid] : -1;
+        if (tid == 0) p.n_accepted[b] = n;
+    }
+    if (len < 0) return;  // an idle place: every CTA of the cluster leaves here
+
+    const float *prow = p.p + (size_t)b * p.p_seq + (size_t)n * p.p_row;
+    const bool cut = n < len;
+    const float *qrow = (cut && p.q) ? p.q + (size_t)b * p.q_seq + (size_t)n * p.q_row : nullptr;
+    int x = (cut && !p.q) ? p.drafts[(size_t)b * p.K + n] : -1;
+    const bool vec = !((reinterpret_cast<uintptr_t>(prow) | reinterpret_cast<uintptr_t>(qrow)) & 15);
+    const int n_segs = (p.V + seg - 1) / seg, per = (n_segs + cs - 1) / cs;
+    const int s0 = min(rank * per, n_segs), s1 = min(s0 + per, n_segs);
+
+    double total = 0.0, before = 0.0, mine = 0.0;
+    for (int pass = 0; pass < 2; pass++) {
+        if (vec) sum_segments<true>(prow, qrow, x, p.V, seg, s0, s1, s_sum);
+        else sum_segments<false>(prow, qrow, x, p.V, seg, s0, s1, s_sum);
+        __syncthreads();
+        if (tid == 0) {
+            double t = 0.0;
+            for (int s = 0; s < s1 - s0; s++) t += s_sum[s];
+            s_tot[pass] = t;
+        }
+        cluster.sync();
+        total = before = 0.0;
+        for (int r = 0; r < cs; r++) {
+            const double t = *cluster.map_shared_rank(&s_tot[pass], r);
+            if (r == rank) {
+                before = total;
+                mine = t;
+            }
+            total += t;
+        }
+        if (total > 0.0 || (!qrow && x < 0)) break;
+        qrow = nullptr;  // the residual is zero everywhere: draw from p
+        x = -1;
+    }
+    // a uniform outside [0, 1) counts as the nearest end, so that the border lies in exactly one run
+    const double target = fmin(fmax((double)p.u_sample[b], 0.0), 1.0 - 1.0 / (1ll << 50)) * total;
+    int *tok = p.tokens + (size_t)b * (p.K + 1) + n;
+    if (warp == 0 && s1 > s0 && total > 0.0) {
+        // the border lies in this CTA's run when the sum before the run does not exceed the target and the sum behind
+        // it does; the additions are those every CTA makes, so exactly one run qualifies
+        const bool here = before <= target && before + mine > target;
+        if (here) {
+            double c = before;
+            int s = s0;
+            for (; s < s1 - 1; s++) {
+                if (c + s_sum[s - s0] > target) break;
+                c += s_sum[s - s0];
+            }
+            // the segment, 128 entries a step: a prefix sum over the lanes' groups of four
+            int found = -1, last = -1;
+            const int v1 = min((s + 1) * seg, p.V);
+            for (int v0 = s * seg; v0 < v1 && found < 0; v0 += 128) {
+                double w[4];
+                if (vec) load_w4<true>(prow, qrow, x, v0 + 4 * lane, p.V, w);
+                else load_w4<false>(prow, qrow, x, v0 + 4 * lane, p.V, w);
+                double inc[4];
+                inc[0] = w[0];
+                inc[1] = inc[0] + w[1];
+                inc[2] = inc[1] + w[2];
+                inc[3] = inc[2] + w[3];
+                double run = inc[3];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double up = __shfl_up_sync(0xffffffffu, run, o);
+                    if (lane >= o) run += up;
+                }
+                const double lead = c + (run - inc[3]);
+                int mine_at = 0x7fffffff, mine_last = -1;
+#pragma unroll
+                for (int e = 3; e >= 0; e--) {
+                    if (w[e] > 0.0 && lead + inc[e] > target) mine_at = v0 + 4 * lane + e;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (w[e] > 0.0) mine_last = v0 + 4 * lane + e;
+                const int first = __reduce_min_sync(0xffffffffu, mine_at);
+                last = max(last, __reduce_max_sync(0xffffffffu, mine_last));
+                if (first != 0x7fffffff) found = first;
+                c += __shfl_sync(0xffffffffu, run, 31);
+            }
+            // (the sums of a segment in two orders may differ in the last bit: then its last entry of any weight)
+            if (lane == 0) *tok = found >= 0 ? found : last;
+        }
+    }
+    cluster.sync();  // a CTA's shared memory stays until its peers have read it
+}
+
+}  // namespace
+
+cudaError_t verify_drafts_configure() {
+    return cudaFuncSetAttribute(verify_drafts_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+
+cudaError_t launch_verify_drafts(const VerifyParams &p, int n_sms, cudaStream_t stream) {
+    if (p.B <= 0) return cudaSuccess;
+    // as many CTAs per sequence as keep every SM busy once, but at least four segments each
+    int cs = 1;
+    while (cs < VD_MAX_CLUSTER && p.B * cs * 2 <= 2 * n_sms && (int64_t)p.V > (int64_t)cs * 4 * VD_SEG) cs *= 2;
+    int64_t seg = VD_SEG;  // longer segments where a run would not fit the table of sums
+    while ((p.V + seg - 1) / seg > (int64_t)cs * VD_MAX_SEGS) seg *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.B * cs));
+    cfg.blockDim = dim3(VD_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, verify_drafts_kernel, p, (int)seg);
+}
+
+}  // namespace mfc

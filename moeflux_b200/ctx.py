@@ -12,7 +12,8 @@ from typing import Optional, Sequence
 
 import numpy as np
 
-from ._lib import Config, MfcError, lib, KV_F32, KV_BF16
+from ._lib import (AttnWeights, Config, KvEvict, MfcError, SharedPrefixAttn, VerifyDrafts, lib, KV_F32,
+                   KV_BF16)
 
 _F = C.POINTER(C.c_float)
 _I = C.POINTER(C.c_int32)
@@ -538,6 +539,33 @@ class Ctx:
         rc = self._lib.mfc_mla_sdpa_folded_bf16_dev(self._h, num_heads, cache_len, softmax_scale, q_prime_ptr, q_pe_ptr,
                                                     latent_bf16_ptr, rope_k_bf16_ptr, out_ptr)
         self._check(rc, "mfc_mla_sdpa_folded_bf16_dev")
+
+    # -- serving a batch from cached rows (device pointers and sizes by the fields of the C structs) ---------------
+    def kv_cache_view(self, layer: int, seq_id: int):
+        """(k pointer, v pointer, seq stride, head stride, rows in use) of a full-attention layer's cached rows."""
+        k, v, ss, hs, n = C.c_void_p(), C.c_void_p(), C.c_int64(), C.c_int64(), C.c_int32()
+        rc = self._lib.mfc_kv_cache_view(self._h, layer, seq_id, C.byref(k), C.byref(v), C.byref(ss), C.byref(hs), C.byref(n))
+        self._check(rc, "mfc_kv_cache_view")
+        return k.value, v.value, ss.value, hs.value, n.value
+
+    def shared_prefix_attn_dev(self, **fields):
+        """Attention of a batch whose sequences share a prefix; ``fields`` are those of ``mfc_shared_prefix_attn``."""
+        rc = self._lib.mfc_shared_prefix_attn_dev(self._h, C.byref(SharedPrefixAttn(**fields)))
+        self._check(rc, "mfc_shared_prefix_attn_dev")
+
+    def attn_weights_accumulate_dev(self, **fields):
+        """Adds a step's attention weights to the running sum of every cached row (``mfc_attn_weights``)."""
+        rc = self._lib.mfc_attn_weights_accumulate_dev(self._h, C.byref(AttnWeights(**fields)))
+        self._check(rc, "mfc_attn_weights_accumulate_dev")
+
+    def kv_evict_dev(self, **fields):
+        """Keeps the ``budget`` heaviest rows of every (sequence, kv head), in place (``mfc_kv_evict``)."""
+        self._check(self._lib.mfc_kv_evict_dev(self._h, C.byref(KvEvict(**fields))), "mfc_kv_evict_dev")
+
+    def verify_drafts_dev(self, **fields):
+        """Accepts drafted tokens against the target's probabilities (``mfc_verify_drafts``)."""
+        rc = self._lib.mfc_verify_drafts_dev(self._h, C.byref(VerifyDrafts(**fields)))
+        self._check(rc, "mfc_verify_drafts_dev")
 
     def linear_attn_step_stateless(self, layer: int, qkv, z, alpha, beta, conv_state, ssm_state):
         """Returns (out, new_conv_state, new_ssm_state); inputs are not modified."""

@@ -1,0 +1,493 @@
+"""Serving a batch from cached rows, through the C ABI on a B200, against the operators' definitions in 64 bits:
+attention over a shared prefix, accumulation of attention weights, eviction, verification of drafted tokens.
+
+Tolerances.  Scores: 256 products of bf16 pairs (exact in fp32) summed in fp32, each addition off by at most 2^-23 of the
+partial sum (the tensor core truncates), so |ds| <= 256 * 2^-23 * scale * sum|q k|, plus 2^-22 (|s| + |m|) for the
+exponent's argument.  Probabilities enter P V rounded to bf16 (half a step: 2^-8), outputs are rounded to bf16 once."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+D = 256
+SCALE = 1.0 / 16.0
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def M():
+    import moeflux_b200
+
+    return moeflux_b200
+
+
+@pytest.fixture(scope="module")
+def ctx(M):
+    c = M.Ctx(num_layers=4, max_seq=512, n_seqs=3, kv_dtype=M.KV_BF16)
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield c
+    c.synchronize()
+    c.close()
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rn(g, *shape, scale=1.0, dtype=torch.bfloat16):
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def visible(lens, T, cap):
+    """[B, T, cap]: which own rows each query token sees."""
+    n = lens.view(-1, 1, 1) - (T - 1 - torch.arange(T, device=lens.device)).view(1, T, 1)
+    return torch.arange(cap, device=lens.device).view(1, 1, cap) < n
+
+
+def attn_args(q, gate, pk, pv, ok, ov, lens, out, lse, scale=SCALE):
+    B, T, H, _ = q.shape
+    Hkv = (pk if pk is not None else ok).shape[0 if pk is not None else 1]
+    a = dict(n_seqs=B, n_tokens=T, num_attn_heads=H, num_kv_heads=Hkv, softmax_scale=scale, q=q.data_ptr(),
+             q_seq_stride=q.stride(0), q_token_stride=q.stride(1), q_head_stride=q.stride(2), own_lens=lens.data_ptr(),
+             out=out.data_ptr(), lse=lse.data_ptr() if lse is not None else None)
+    if gate is not None:
+        a.update(gate=gate.data_ptr(), gate_seq_stride=gate.stride(0), gate_token_stride=gate.stride(1),
+                 gate_head_stride=gate.stride(2))
+    if pk is not None:
+        a.update(prefix_k=pk.data_ptr(), prefix_v=pv.data_ptr(), prefix_head_stride=pk.stride(0),
+                 prefix_row_stride=pk.stride(1), prefix_len=pk.shape[1])
+    if ok is not None:
+        a.update(own_k=ok.data_ptr(), own_v=ov.data_ptr(), own_seq_stride=ok.stride(0), own_head_stride=ok.stride(1),
+                 own_row_stride=ok.stride(2), own_cap=ok.shape[2])
+    return a
+
+
+def attn_ref(q, gate, pk, pv, ok, ov, lens, scale=SCALE):
+    """(out, lse, bound on |d out|, bound on |d lse|) in fp64, one sequence at a time."""
+    B, T, H, _ = q.shape
+    Hkv = pk.shape[0] if pk is not None else ok.shape[1]
+    G = H // Hkv
+    outs, lses, bo, bl = [], [], [], []
+    zero = torch.zeros(Hkv, 0, D, device="cuda", dtype=torch.float64)
+    cap = ok.shape[2] if ok is not None else 0
+    P = pk.shape[1] if pk is not None else 0
+    vis = visible(lens, T, cap)
+    for b in range(B):
+        n = max(0, min(int(lens[b]), cap))
+        k = torch.cat([pk.double() if P else zero, ok[b, :, :n].double() if n else zero], 1)
+        v = torch.cat([pv.double() if P else zero, ov[b, :, :n].double() if n else zero], 1)
+        qq = q[b].double().view(T, Hkv, G, D)
+        s = torch.einsum("thgd,hjd->thgj", qq, k) * scale
+        a = torch.einsum("thgd,hjd->thgj", qq.abs(), k.abs()) * scale
+        see = torch.cat([torch.ones(T, P, dtype=torch.bool, device="cuda"), vis[b, :, :n]], 1).view(T, 1, 1, -1)
+        s = s.masked_fill(~see, float("-inf"))
+        z = torch.logsumexp(s, -1, keepdim=True) if s.shape[-1] else torch.full((T, Hkv, G, 1), float("-inf"), device="cuda", dtype=torch.float64)
+        p = torch.nan_to_num(torch.exp(s - z)) * see
+        o = torch.einsum("thgj,hjd->thgd", p, v)
+        ov_abs = torch.einsum("thgj,hjd->thgd", p, v.abs())
+        # error of a score, largest over the rows that matter
+        smax = torch.where(see, s.abs(), 0.0).amax(-1, keepdim=True) if s.shape[-1] else torch.zeros_like(z)
+        amax = torch.where(see, a, 0.0).amax(-1, keepdim=True) if s.shape[-1] else torch.zeros_like(z)
+        ds = 256 * 2.0 ** -23 * amax + 2.0 ** -21 * smax + 2.0 ** -20
+        gt = torch.sigmoid(gate[b].double()).view(T, Hkv, G, D) if gate is not None else 1.0
+        o = o * gt
+        outs.append(o.reshape(T, H, D))
+        bo.append((2.0 ** -8 * o.abs() + (2.0 ** -8 + 2 * ds + 1e-5) * ov_abs * gt).reshape(T, H, D))
+        lses.append(z.reshape(T, H))
+        bl.append(ds.reshape(T, H) + 2.0 ** -22 * torch.nan_to_num(z, neginf=0.0).abs().reshape(T, H))
+    return torch.stack(outs), torch.stack(lses), torch.stack(bo), torch.stack(bl)
+
+
+def check_attn(ctx, q, gate, pk, pv, ok, ov, lens, scale=SCALE):
+    B, T, H, _ = q.shape
+    out = torch.full((B, T, H, D), float("nan"), device="cuda", dtype=torch.bfloat16)
+    lse = torch.full((B, T, H), float("nan"), device="cuda")
+    ctx.shared_prefix_attn_dev(**attn_args(q, gate, pk, pv, ok, ov, lens, out, lse, scale))
+    ctx.synchronize()
+    ro, rl, bo, bl = attn_ref(q, gate, pk, pv, ok, ov, lens, scale)
+    none = torch.isinf(rl)
+    assert torch.equal(torch.isneginf(lse), none)
+    assert ((lse.double() - rl).abs()[~none] <= bl[~none]).all()
+    assert torch.isfinite(out.float()).all()
+    over = (out.double() - ro).abs() - bo
+    assert (over <= 0).all(), (float(over.max()), float((out.double() - ro).abs().max()))
+    return out, lse
+
+
+def lens_for(g, B, T, cap):
+    lens = torch.randint(min(T, cap), cap + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lens[0] = cap
+    if B > 2:
+        lens[1] = 0
+        lens[2] = min(1, cap)  # fewer rows than tokens when T > 1
+    return lens
+
+
+@pytest.mark.parametrize("B,T,H,Hkv,P,cap", [
+    (1, 1, 32, 2, 1, 1), (1, 1, 32, 2, 0, 1), (1, 1, 32, 2, 300, 0), (2, 1, 32, 2, 127, 5), (2, 1, 32, 2, 128, 128),
+    (3, 2, 10, 2, 129, 257), (5, 3, 24, 2, 1000, 300), (9, 1, 7, 1, 515, 130), (4, 16, 16, 1, 200, 64), (3, 9, 16, 1, 0, 300),
+    (40, 4, 32, 2, 2000, 640), (17, 5, 8, 8, 640, 200), (300, 1, 16, 1, 130, 140), (1, 1, 32, 2, 40000, 1), (33, 2, 32, 2, 9000, 40)])
+def test_shared_prefix_attn(ctx, B, T, H, Hkv, P, cap):
+    g = gen(B * 1000 + P + cap)
+    q = rn(g, B, T, H, D, scale=1.5)
+    gate = rn(g, B, T, H, D) if B % 2 else None
+    pk, pv = (rn(g, Hkv, P, D), rn(g, Hkv, P, D)) if P else (None, None)
+    ok, ov = (rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)) if cap else (None, None)
+    check_attn(ctx, q, gate, pk, pv, ok, ov, lens_for(g, B, T, cap))
+
+
+def test_shared_prefix_attn_without_any_row(ctx):
+    g = gen(1)
+    q = rn(g, 3, 2, 32, D)
+    lens = torch.tensor([0, 5, 1], device="cuda", dtype=torch.int32)
+    ok, ov = rn(g, 3, 2, 8, D), rn(g, 3, 2, 8, D)
+    out, lse = check_attn(ctx, q, None, None, None, ok, ov, lens)
+    assert torch.isneginf(lse[0]).all() and (out[0] == 0).all()
+    assert torch.isneginf(lse[2, 0]).all() and (out[2, 0] == 0).all()  # the first of two tokens sees no row yet
+    # no rows of either kind anywhere
+    out.fill_(float("nan"))
+    ctx.shared_prefix_attn_dev(n_seqs=3, n_tokens=2, num_attn_heads=32, num_kv_heads=2, softmax_scale=SCALE, q=q.data_ptr(),
+                               q_seq_stride=q.stride(0), q_token_stride=q.stride(1), q_head_stride=D,
+                               own_lens=torch.zeros_like(lens).data_ptr(), out=out.data_ptr(), lse=lse.data_ptr())
+    ctx.synchronize()
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_shared_prefix_attn_ignores_what_lies_behind_the_lengths(ctx):
+    """NaN and infinities in own rows at and beyond a sequence's length, and queries that grow the running maximum by far
+    more than the rescaling threshold from tile to tile."""
+    g = gen(2)
+    B, T, H, Hkv, P, cap = 6, 2, 32, 2, 700, 500
+    q = rn(g, B, T, H, D, scale=2.0)
+    pk, pv = rn(g, Hkv, P, D), rn(g, Hkv, P, D)
+    pk *= torch.linspace(0.1, 8.0, P, device="cuda").view(1, P, 1).to(torch.bfloat16)
+    ok, ov = rn(g, B, Hkv, cap, D, scale=3.0), rn(g, B, Hkv, cap, D)
+    lens = torch.tensor([0, 1, 127, 128, 129, 499], device="cuda", dtype=torch.int32)
+    for b in range(B):
+        n = int(lens[b])
+        ok[b, :, n:] = float("nan")
+        ov[b, :, n:] = float("nan")
+        ov[b, :, n : n + 3] = float("inf")
+    check_attn(ctx, q, None, pk, pv, ok, ov, lens)
+
+
+def test_shared_prefix_attn_strided(ctx):
+    """q and gate interleaved per head as a projection emits them, rows of a cache with gaps, heads behind rows, and the
+    sequences of a batch that are every other place of a larger cache."""
+    g = gen(3)
+    B, T, H, Hkv, P, cap = 4, 2, 24, 2, 333, 200
+    qg = rn(g, B, T, H, 2 * D)
+    q, gate = qg[..., :D], qg[..., D:]
+    pk = rn(g, P, Hkv, D + 8)[..., :D].transpose(0, 1)
+    pv = rn(g, P, Hkv, D + 8)[..., :D].transpose(0, 1)
+    ok = rn(g, 2 * B, cap, Hkv, D).transpose(1, 2)[::2]
+    ov = rn(g, 2 * B, cap, Hkv, D).transpose(1, 2)[::2]
+    check_attn(ctx, q, gate, pk, pv, ok, ov, lens_for(g, B, T, cap))
+
+
+def test_shared_prefix_attn_lengths_out_of_range_are_reported(ctx, M):
+    g = gen(4)
+    q, pk, pv = rn(g, 3, 1, 32, D), rn(g, 2, 200, D), rn(g, 2, 200, D)
+    ok, ov = rn(g, 3, 2, 64, D), rn(g, 3, 2, 64, D)
+    lens = torch.tensor([64, 65, -1], device="cuda", dtype=torch.int32)
+    out, lse = torch.zeros(3, 1, 32, D, device="cuda", dtype=torch.bfloat16), torch.zeros(3, 1, 32, device="cuda")
+    ctx.shared_prefix_attn_dev(**attn_args(q, None, pk, pv, ok, ov, lens, out, lse))
+    with pytest.raises(M.MfcError, match="range checks"):
+        ctx.synchronize()
+    ro, rl, bo, _ = attn_ref(q, None, pk, pv, ok, ov, torch.tensor([64, 0, 0], device="cuda", dtype=torch.int32))
+    assert ((out.double() - ro).abs() <= bo).all()  # such a sequence counts as empty, the others are right
+    check_attn(ctx, q, None, pk, pv, ok, ov, lens.clamp(0, 64))
+
+
+def test_shared_prefix_attn_repeats_bit_for_bit_and_replays(ctx):
+    g = gen(5)
+    B, T, H, Hkv, P, cap = 20, 3, 32, 2, 1500, 300
+    q, pk, pv = rn(g, B, T, H, D), rn(g, Hkv, P, D), rn(g, Hkv, P, D)
+    ok, ov = rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    lens = lens_for(g, B, T, cap)
+    out, lse = check_attn(ctx, q, None, pk, pv, ok, ov, lens)
+    again, lse2 = torch.zeros_like(out), torch.zeros_like(lse)
+    args = attn_args(q, None, pk, pv, ok, ov, lens, again, lse2)
+    s = torch.cuda.Stream()
+    home = torch.cuda.current_stream().cuda_stream
+    s.wait_stream(torch.cuda.current_stream())
+    ctx.set_stream(s.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        ctx.shared_prefix_attn_dev(**args)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    lens.copy_((lens - 5).clamp(min=0))  # the lengths are read when the graph runs
+    q.mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    ctx.set_stream(home)
+    ro, rl, bo, bl = attn_ref(q, None, pk, pv, ok, ov, lens)
+    assert ((again.double() - ro).abs() <= bo).all()
+
+
+# ---------------------------------------------------------------------------------------------------- weights
+
+
+def weights_args(q, k, lens, lse, w, decay=1.0, scale=SCALE):
+    B, T, H, _ = q.shape
+    return dict(n_seqs=B, n_tokens=T, num_attn_heads=H, num_kv_heads=k.shape[1], softmax_scale=scale, decay=decay,
+                q=q.data_ptr(), q_seq_stride=q.stride(0), q_token_stride=q.stride(1), q_head_stride=q.stride(2),
+                k=k.data_ptr(), k_seq_stride=k.stride(0), k_head_stride=k.stride(1), k_row_stride=k.stride(2), cap=k.shape[2],
+                lens=lens.data_ptr(), lse=lse.data_ptr(), weights=w.data_ptr(), weights_seq_stride=w.stride(0),
+                weights_head_stride=w.stride(1))
+
+
+def weights_ref(q, k, lens, lse, w, decay, scale=SCALE):
+    B, T, H, _ = q.shape
+    Hkv, cap = k.shape[1], k.shape[2]
+    G = H // Hkv
+    res, tol = w.double().clone(), torch.zeros_like(w, dtype=torch.float64)
+    vis = visible(lens, T, cap)
+    for b in range(B):
+        n = max(0, min(int(lens[b]), cap))
+        if n == 0:
+            continue
+        qq, kk = q[b].double().view(T, Hkv, G, D), k[b, :, :n].double()
+        s = torch.einsum("thgd,hjd->thgj", qq, kk) * scale
+        a = torch.einsum("thgd,hjd->thgj", qq.abs(), kk.abs()) * scale
+        z = lse[b].double().view(T, Hkv, G, 1)
+        p = torch.where(vis[b, :, :n].view(T, 1, 1, n), torch.exp(s - z), 0.0)
+        ds = 256 * 2.0 ** -23 * a + 2.0 ** -21 * (s.abs() + z.abs().nan_to_num(posinf=0.0)) + 2.0 ** -20
+        res[b, :, :n] = decay * res[b, :, :n] + p.sum((0, 2))
+        tol[b, :, :n] = torch.where(p > 0, p * ds, 0.0).sum((0, 2)) + 2.0 ** -22 * T * G * res[b, :, :n].abs()
+    return res, tol
+
+
+@pytest.mark.parametrize("B,T,H,Hkv,cap,decay", [
+    (1, 1, 32, 2, 1, 1.0), (1, 1, 32, 2, 1000, 1.0), (3, 1, 7, 1, 65, 0.5), (4, 3, 24, 2, 300, 1.0), (5, 16, 16, 1, 130, 0.96875),
+    (40, 2, 8, 8, 257, 1.0), (2, 5, 32, 2, 5000, 0.96875), (200, 1, 10, 2, 64, 1.0)])
+def test_attn_weights(ctx, B, T, H, Hkv, cap, decay):
+    g = gen(B + cap)
+    q, k = rn(g, B, T, H, D, scale=1.5), rn(g, B, Hkv, cap, D)
+    lens = lens_for(g, B, T, cap)
+    for b in range(B):
+        k[b, :, int(lens[b]):] = float("nan")
+    w = torch.rand(B, Hkv, cap, generator=g, device="cuda")
+    ro, lse, _, _ = attn_ref(q, None, None, None, k, torch.zeros_like(k), lens)
+    lse = lse.float().contiguous()
+    ref, tol = weights_ref(q, k, lens, lse, w, decay)
+    before = w.clone()
+    ctx.attn_weights_accumulate_dev(**weights_args(q, k, lens, lse, w, decay))
+    ctx.synchronize()
+    assert ((w.double() - ref).abs() <= tol).all(), float(((w.double() - ref).abs() - tol).max())
+    unused = torch.arange(cap, device="cuda").view(1, 1, cap) >= lens.view(B, 1, 1)
+    assert torch.equal(w[unused.expand_as(w)], before[unused.expand_as(w)])
+
+
+def test_attn_weights_strided_and_out_of_range(ctx, M):
+    g = gen(7)
+    B, T, H, Hkv, cap = 3, 2, 32, 2, 150
+    q = rn(g, B, T, H, 2 * D)[..., :D]
+    k = rn(g, B, cap, Hkv, D + 8)[..., :D].transpose(1, 2)
+    wide = torch.rand(B, Hkv, cap + 13, generator=g, device="cuda")
+    w, before = wide[..., :cap], wide.clone()
+    lens = torch.tensor([150, 151, 60], device="cuda", dtype=torch.int32)
+    good = torch.tensor([150, 0, 60], device="cuda", dtype=torch.int32)
+    _, lse, _, _ = attn_ref(q, None, None, None, k, torch.zeros_like(k), good)
+    lse = lse.float().contiguous()
+    ref, tol = weights_ref(q, k, good, lse, w, 1.0)
+    ctx.attn_weights_accumulate_dev(**weights_args(q, k, lens, lse, w))
+    with pytest.raises(M.MfcError, match="range checks"):
+        ctx.synchronize()
+    assert ((w.double() - ref).abs() <= tol).all()
+    assert torch.equal(wide[..., cap:], before[..., cap:])
+
+
+# ---------------------------------------------------------------------------------------------------- eviction
+
+
+def evict_ref(k, v, w, pos, lens, nxt, budget, sink, recent):
+    """The rows' new content by the definition, on the host: [(b, h, rows)] of source rows."""
+    out = {}
+    w, pos = w.cpu().tolist(), pos.cpu().tolist()
+    for b in range(k.shape[0]):
+        n = int(lens[b])
+        for h in range(k.shape[1]):
+            def key(j):
+                x, ps = w[b][h][j], pos[b][h][j]
+                if ps < sink or ps >= int(nxt[b]) - recent:
+                    return (0, 0.0, j)
+                return (2, 0.0, j) if x != x else (1, -x, j)
+            new = min(n, budget)
+            kept = set(sorted(range(n), key=key)[:new])
+            movers = iter([j for j in range(budget, n) if j in kept])
+            out[b, h] = [j if j in kept else next(movers) for j in range(new)]
+    return out
+
+
+@pytest.mark.parametrize("B,Hkv,cap,budget,dtype", [
+    (1, 1, 1, 1, "bf16"), (2, 2, 40, 8, "bf16"), (1, 2, 1088, 1024, "bf16"), (3, 1, 700, 699, "f32"), (2, 2, 5000, 77, "bf16"),
+    (70, 2, 300, 128, "f32"), (1, 1, 33000, 20001, "bf16"), (5, 3, 64, 100, "bf16"), (160, 2, 1030, 400, "bf16")])
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+def test_kv_evict(ctx, M, B, Hkv, cap, budget, dtype, kind):
+    g = gen(B * 7 + cap)
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    k, v = rn(g, B, Hkv, cap, D, dtype=dt), rn(g, B, Hkv, cap, D, dtype=dt)
+    w = torch.exp(2 * torch.randn(B, Hkv, cap, generator=g, device="cuda"))
+    if kind == "ties":  # few distinct weights, both zeros, infinities and NaN
+        w = torch.randint(-1, 3, (B, Hkv, cap), generator=g, device="cuda").float()
+        r = torch.rand(B, Hkv, cap, generator=g, device="cuda")
+        w[r < 0.1] = -0.0
+        w[r > 0.96] = float("nan")
+        w[(r > 0.92) & (r < 0.94)] = float("inf")
+        w[(r > 0.90) & (r < 0.92)] = float("-inf")
+    lens = torch.randint(min(budget, cap), cap + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lens[0] = cap
+    if B > 2:
+        lens[1], lens[2] = 0, min(budget, cap)
+    pos = torch.rand(B, Hkv, cap, generator=g, device="cuda").argsort(-1).to(torch.int32)
+    nxt = lens + 3
+    sink, recent = 2, max(3, min(budget, 40) // 4)
+    src = evict_ref(k, v, w, pos, lens, nxt, budget, sink, recent)
+    k0, v0, w0, p0, l0 = (t.clone() for t in (k, v, w, pos, lens))
+    for alias in (False, True):
+        k.copy_(k0)
+        v.copy_(v0)
+        wo, po = (w, pos) if alias else (torch.full_like(w, -7.0), torch.full_like(pos, -7))
+        lo = torch.full_like(lens, -7)
+        ctx.kv_evict_dev(n_seqs=B, num_kv_heads=Hkv, kv_dtype=M.KV_BF16 if dtype == "bf16" else M.KV_F32, cap=cap, k=k.data_ptr(),
+                         v=v.data_ptr(), seq_stride=k.stride(0), head_stride=k.stride(1), row_stride=k.stride(2), budget=budget,
+                         n_sink=sink, n_recent=recent, lens=lens.data_ptr(), next_pos=nxt.data_ptr(), weights=w.data_ptr(),
+                         positions=pos.data_ptr(), map_seq_stride=w.stride(0), map_head_stride=w.stride(1),
+                         weights_out=wo.data_ptr(), positions_out=po.data_ptr(), lens_out=lo.data_ptr())
+        ctx.synchronize()
+        assert torch.equal(lo, lens.clamp(max=budget)) and torch.equal(lens, l0)
+        for (b, h), rows in src.items():
+            n = len(rows)
+            ix = torch.tensor(rows, device="cuda", dtype=torch.long)
+            assert torch.equal(k[b, h, :n], k0[b, h, ix]) and torch.equal(v[b, h, :n], v0[b, h, ix]), (b, h)
+            assert torch.equal(k[b, h, n:], k0[b, h, n:]) and torch.equal(v[b, h, n:], v0[b, h, n:])
+            assert torch.equal(wo[b, h, :n].nan_to_num(-9.0), w0[b, h, ix].nan_to_num(-9.0)) and torch.equal(po[b, h, :n], p0[b, h, ix])
+            rest_w, rest_p = (w0[b, h, n:], p0[b, h, n:]) if alias else (torch.full_like(wo[b, h, n:], -7.0), torch.full_like(po[b, h, n:], -7))
+            assert torch.equal(wo[b, h, n:].nan_to_num(-9.0), rest_w.nan_to_num(-9.0)) and torch.equal(po[b, h, n:], rest_p)
+
+
+def test_kv_evict_strided_rows_and_out_of_range(ctx, M):
+    g = gen(11)
+    B, Hkv, cap, budget = 3, 2, 90, 50
+    kw, vw = rn(g, B, cap, Hkv, D + 8), rn(g, B, cap, Hkv, D + 8)
+    k0, v0 = kw.clone(), vw.clone()
+    w = torch.rand(B, Hkv, cap + 5, generator=g, device="cuda")[..., :cap]
+    pos = torch.arange(cap + 5, device="cuda", dtype=torch.int32).expand(B, Hkv, cap + 5).contiguous()[..., :cap]
+    lens = torch.tensor([90, 91, -2], device="cuda", dtype=torch.int32)
+    nxt, lo = lens.clone(), torch.zeros_like(lens)
+    wo, po = torch.zeros(B, Hkv, cap + 5, device="cuda"), torch.zeros(B, Hkv, cap + 5, device="cuda", dtype=torch.int32)
+    ctx.kv_evict_dev(n_seqs=B, num_kv_heads=Hkv, kv_dtype=M.KV_BF16, cap=cap, k=kw.data_ptr(), v=vw.data_ptr(),
+                     seq_stride=kw.stride(0), head_stride=kw.stride(2), row_stride=kw.stride(1), budget=budget, n_sink=4, n_recent=8,
+                     lens=lens.data_ptr(), next_pos=nxt.data_ptr(), weights=w.data_ptr(), positions=pos.data_ptr(),
+                     map_seq_stride=w.stride(0), map_head_stride=w.stride(1), weights_out=wo.data_ptr(), positions_out=po.data_ptr(),
+                     lens_out=lo.data_ptr())
+    with pytest.raises(M.MfcError, match="range checks"):
+        ctx.synchronize()
+    assert lo.tolist() == [50, 0, 0]
+    assert torch.equal(kw[1:], k0[1:]) and torch.equal(vw[1:], v0[1:]) and torch.equal(kw[..., D:], k0[..., D:])
+    src = evict_ref(k0[:1].transpose(1, 2), None, w[:1], pos[:1], lens[:1], nxt[:1], budget, 4, 8)
+    for (b, h), rows in src.items():
+        ix = torch.tensor(rows, device="cuda", dtype=torch.long)
+        assert torch.equal(kw[b, :50, h, :D], k0[b, ix, h, :D]) and torch.equal(vw[b, :50, h, :D], v0[b, ix, h, :D])
+
+
+# ---------------------------------------------------------------------------------------------------- verification
+
+
+def verify_ref(p, q, x, lens, ua, us):
+    p, x, ua, us = p.cpu().double(), x.cpu(), ua.cpu().double(), us.cpu().double()
+    q = q.cpu().double() if q is not None else None
+    B, K, V = p.shape[0], x.shape[1], p.shape[2]
+    ns, toks = [], []
+    for b in range(B):
+        n_drafts = min(int(lens[b]), K)
+        if n_drafts < 0:
+            ns.append(0)
+            toks.append([-1] * (K + 1))
+            continue
+        n = 0
+        while n < n_drafts:
+            t = int(x[b, n])
+            if not (0 <= t < V and float(ua[b, n]) * (float(q[b, n, t]) if q is not None else 1.0) < float(p[b, n, t])):
+                break
+            n += 1
+        w = p[b, n].clone()
+        if n < n_drafts:
+            if q is not None:
+                w = w - q[b, n]
+            elif 0 <= int(x[b, n]) < V:
+                w[int(x[b, n])] = 0.0
+        w = torch.where(w > 0, w, 0.0)
+        if float(w.sum()) == 0.0:
+            w = torch.where(p[b, n] > 0, p[b, n], 0.0)
+        c = torch.cumsum(w, 0)
+        t = int((c <= float(us[b]) * float(c[-1])).sum()) if float(c[-1]) > 0 else -1
+        ns.append(n)
+        toks.append([int(y) for y in x[b, :n]] + [t] + [-1] * (K - n))
+    return torch.tensor(ns, dtype=torch.int32), torch.tensor(toks, dtype=torch.int32)
+
+
+def call_verify(ctx, p, q, x, lens, ua, us):
+    B, K = x.shape
+    n = torch.full((B,), -5, device="cuda", dtype=torch.int32)
+    tok = torch.full((B, K + 1), -5, device="cuda", dtype=torch.int32)
+    ctx.verify_drafts_dev(n_seqs=B, max_drafts=K, vocab=p.shape[2], target_probs=p.data_ptr(), target_seq_stride=p.stride(0),
+                          target_row_stride=p.stride(1), draft_probs=q.data_ptr() if q is not None else None,
+                          draft_seq_stride=q.stride(0) if q is not None else 0, draft_row_stride=q.stride(1) if q is not None else 0,
+                          draft_tokens=x.data_ptr(), draft_lens=lens.data_ptr() if lens is not None else None, u_accept=ua.data_ptr(),
+                          u_sample=us.data_ptr(), n_accepted=n.data_ptr(), tokens=tok.data_ptr())
+    ctx.synchronize()
+    return n.cpu(), tok.cpu()
+
+
+@pytest.mark.parametrize("B,K,V,sampled,pad", [
+    (1, 1, 1, True, 0), (1, 0, 10, True, 0), (3, 4, 7, True, 0), (2, 4, 1000, False, 0), (9, 8, 4099, True, 1), (64, 3, 1025, True, 3),
+    (1, 5, 131072, True, 0), (200, 2, 2048, False, 0), (2, 32, 50001, True, 0), (1, 1, 1200003, True, 0)])
+def test_verify_drafts(ctx, B, K, V, sampled, pad):
+    g = gen(B + K + V)
+    logits = torch.randn(B, K + 1, V + pad, generator=g, device="cuda") * 2
+    p = torch.softmax(logits[..., :V], -1)
+    ql = logits[:, :K, :V] + 0.7 * torch.randn(B, K, V, generator=g, device="cuda")
+    q = torch.softmax(ql, -1) if sampled else None
+    noise = -torch.log(-torch.log(torch.rand(ql.shape, generator=g, device="cuda").clamp(1e-9, 1 - 1e-7)))
+    x = (ql + noise).argmax(-1).to(torch.int32)  # the draft model's samples
+    if pad:  # rows that start at no 16-byte boundary
+        wide = torch.full((B, K + 1, V + pad), float("nan"), device="cuda")
+        wide[..., :V] = p
+        p = wide[..., :V]
+    lens = torch.randint(0, K + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lens[0] = K
+    if B > 2:
+        lens[1] = -1
+    ua, us = torch.rand(B, K, generator=g, device="cuda"), torch.rand(B, generator=g, device="cuda")
+    n, tok = call_verify(ctx, p, q, x, lens, ua, us)
+    rn_, rt = verify_ref(p, q, x, lens, ua, us)
+    assert torch.equal(n, rn_) and torch.equal(tok, rt)
+
+
+def test_verify_drafts_edges(ctx):
+    V = 3000
+    p = torch.zeros(6, 2, V, device="cuda")
+    q = torch.zeros(6, 1, V, device="cuda")
+    x = torch.zeros(6, 1, device="cuda", dtype=torch.int32)
+    ua = torch.full((6, 1), 0.5, device="cuda")
+    us = torch.zeros(6, device="cuda")
+    p[0, :, 5], q[0, 0, 5], x[0] = 1.0, 1.0, 5                       # equal distributions: accepted, then row 1
+    p[1, :, 7], q[1, 0, 7], x[1] = 0.25, 0.5, 7                      # u q = p exactly: refused; the residual is zero: from p
+    p[2, 0, 9], q[2, 0, 3], x[2] = 1.0, 1.0, 3                       # p(x) = 0: refused, residual at 9
+    x[3] = V                                                         # outside the vocabulary, p all zero: no token
+    p[4, 0, 100:200], q[4, 0, 4], x[4], us[4] = 0.01, 1.0, 4, 1.0 - 2.0 ** -24
+    p[5, 0, 11], p[5, 0, 12], q[5, 0, 0], x[5] = float("nan"), 0.5, 1.0, 0  # a NaN counts as zero
+    n, tok = call_verify(ctx, p, q, x, None, ua, us)
+    assert n.tolist() == [1, 0, 0, 0, 0, 0]
+    assert tok.tolist() == [[5, 5], [7, -1], [9, -1], [-1, -1], [199, -1], [12, -1]]
+    # a uniform outside [0, 1) counts as the nearest end; without draft probabilities the drafted token itself is left out
+    us[:] = torch.tensor([1.0, -1.0, float("nan"), 2.0, float("inf"), 0.0], device="cuda")
+    p[2, 0, 3], ua[2] = 0.25, 0.9
+    n, tok = call_verify(ctx, p, None, x, None, ua, us)
+    assert n.tolist() == [1, 0, 0, 0, 0, 0]
+    assert tok.tolist() == [[5, 5], [7, -1], [9, -1], [-1, -1], [199, -1], [12, -1]]
