@@ -1488,9 +1488,10 @@ bool check_heads(mfc_ctx *c, int n_seqs, int n_tokens, int H, int Hkv, float sca
 }
 bool strides8(int64_t a, int64_t b, int64_t d) { return a % 8 == 0 && b % 8 == 0 && d % 8 == 0; }
 
-// Map over cached bf16 rows (dim 256, row, kv head[, sequence]), boxes of 64 dims x box_rows rows.
+// Map over cached bf16 rows, (64 dims, row, fourth of the 256 dims, kv head, sequence), boxes of `fourths` x box_rows rows:
+// a box lands in shared memory as `fourths` blocks of box_rows 128-byte rows (128-byte swizzle).
 bool make_rows_map(mfc_ctx *c, CUtensorMap *map, const void *base, int64_t rows, int64_t row_stride, int heads, int64_t head_stride,
-                   int seqs, int64_t seq_stride, int rank, int box_rows) {
+                   int seqs, int64_t seq_stride, int fourths, int box_rows) {
     static EncodeTiledFn encode = [] {
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult qres;
@@ -1504,11 +1505,11 @@ bool make_rows_map(mfc_ctx *c, CUtensorMap *map, const void *base, int64_t rows,
     const int64_t most = (int64_t)1 << 39;  // the encoder's limit, in elements of two bytes
     if (row_stride < HEAD_DIM || row_stride >= most || head_stride <= 0 || head_stride >= most || seq_stride <= 0 || seq_stride >= most)
         return fail(c, "the strides of cached rows must be positive, at least 256 elements between rows, and below 2^39");
-    cuuint64_t dims[4] = {(cuuint64_t)HEAD_DIM, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)seqs};
-    cuuint64_t strides[3] = {(cuuint64_t)row_stride * 2, (cuuint64_t)head_stride * 2, (cuuint64_t)seq_stride * 2};
-    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, estr,
+    cuuint64_t dims[5] = {64, (cuuint64_t)rows, HEAD_DIM / 64, (cuuint64_t)heads, (cuuint64_t)seqs};
+    cuuint64_t strides[4] = {(cuuint64_t)row_stride * 2, 128, (cuuint64_t)head_stride * 2, (cuuint64_t)seq_stride * 2};
+    cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)fourths, 1, 1};
+    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void *>(base), dims, strides, box, estr,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(c, "cuTensorMapEncodeTiled failed, code " + std::to_string((int)r));
@@ -1615,11 +1616,11 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
     p.scale = a->softmax_scale;
     CUtensorMap m[4];
     memset(m, 0, sizeof(m));
-    if (has_prefix && (!make_rows_map(c, &m[0], a->prefix_k, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 3, 128) ||
-                       !make_rows_map(c, &m[1], a->prefix_v, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 3, 32)))
+    if (has_prefix && (!make_rows_map(c, &m[0], a->prefix_k, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 2, 128) ||
+                       !make_rows_map(c, &m[1], a->prefix_v, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 4, 64)))
         return -1;
-    if (has_own && (!make_rows_map(c, &m[2], a->own_k, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 4, 128) ||
-                    !make_rows_map(c, &m[3], a->own_v, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 4, 32)))
+    if (has_own && (!make_rows_map(c, &m[2], a->own_k, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 2, 128) ||
+                    !make_rows_map(c, &m[3], a->own_v, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 4, 64)))
         return -1;
     DeviceScope dev(c->cfg.device);
     CK(launch_shared_prefix_attn(m[0], m[1], m[2], m[3], p, c->stream));

@@ -346,8 +346,8 @@ struct SharedAttnParams {
     float scale;
 };
 cudaError_t shared_prefix_attn_configure();
-// pk/ok: maps over K with boxes of 64 dims x 128 rows; pv/ov: maps over V with boxes of 64 dims x 32 rows;
-// prefix maps are 3-D (dim, row, kv head), own maps 4-D (dim, row, kv head, sequence).
+// Maps (64 dims, row, fourth of the dims, kv head, sequence) over the prefix and own rows; boxes of two fourths x 128
+// rows for K, four fourths x 64 rows for V.
 cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &pv, const CUtensorMap &ok,
                                       const CUtensorMap &ov, const SharedAttnParams &p, cudaStream_t stream);
 

@@ -14,8 +14,8 @@
 // and applies the gate.  Lengths are read on the device: every CTA finds its place by a scan over them.
 //
 // CTA (320 threads): warps 0-7 softmax (thread = query row x half of the 128 columns), warp 8 issues every tcgen05.mma,
-// warp 9 every TMA load.  Shared memory: Q 64 KiB and a ring of ten 16 KiB granules that K and V share in the order in
-// which the tensor core takes them (K: 64 dims x 128 rows, V: 256 dims x 32 rows).  Tensor memory (512 columns): O 256,
+// warp 9 every TMA load.  Shared memory: Q 64 KiB and a ring of five 32 KiB granules that K and V share in the order in
+// which the tensor core takes them (K: 128 dims x 128 rows, V: 256 dims x 64 rows).  Tensor memory (512 columns): O 256,
 // S 128, P twice 64 (bf16, the A operand of P V straight from tensor memory).  S is free again as soon as the softmax
 // has read it, so Q K^T of tile j+1 runs under the softmax of tile j, and P V of tile j under that of tile j+1.  O is
 // rescaled only when a row maximum grows by more than 2^8.  P is rounded to bf16 (the type of V: both operands of one
@@ -35,8 +35,8 @@ namespace {
 constexpr int SP_M = SHARED_ATTN_M;
 constexpr int SP_N = SHARED_ATTN_N;
 constexpr int SP_THREADS = 320;
-constexpr int SP_GRAN = 10;                                // granules of the K/V ring
-constexpr uint32_t GRAN_BYTES = 16384;
+constexpr int SP_GRAN = 5;                                 // granules of the K/V ring
+constexpr uint32_t GRAN_BYTES = 32768;
 constexpr uint32_t SP_Q_BOX = SP_M * 128;                  // 64 dims of 128 query rows
 constexpr uint32_t SP_OFF_RING = 4 * SP_Q_BOX;
 constexpr uint32_t SP_OFF_XM = SP_OFF_RING + SP_GRAN * GRAN_BYTES;  // row-maximum / row-sum exchange
@@ -48,11 +48,11 @@ constexpr float LOG2E_SP = 1.4426950408889634f;
 constexpr uint32_t SP_TMEM_COLS = 512;
 constexpr uint32_t TM_O = 0, TM_S = 256, TM_P = 384;       // P: two buffers of 64 columns
 
-__device__ __forceinline__ void tma_load_4d(void *smem_dst, const void *tmap, int c0, int c1, int c2, int c3, uint64_t *bar) {
+__device__ __forceinline__ void tma_load_5d(void *smem_dst, const void *tmap, int c0, int c1, int c2, int c3, int c4, uint64_t *bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(smem_dst)),
-        "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
+        "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
         : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem desc], bf16 inputs, fp32 accumulate; A: lane = row, one 32-bit column = two k
@@ -122,8 +122,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + SP_OFF_BAR);
-    uint64_t *full = bars;                  // [10] TMA: granule landed
-    uint64_t *empty = bars + SP_GRAN;       // [10] tcgen05.commit: the products that read the granule are done
+    uint64_t *full = bars;                  // [5] TMA: granule landed
+    uint64_t *empty = bars + SP_GRAN;       // [5] tcgen05.commit: the products that read the granule are done
     uint64_t *s_ready = bars + 20;          // tcgen05.commit: scores of a tile are in tensor memory
     uint64_t *s_read = bars + 21;           // 8 warps: scores are in registers
     uint64_t *p_ready = bars + 22;          // [2] 8 warps: P of a tile is in tensor memory, O may be added to
@@ -221,26 +221,20 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 mbar_expect_tx(&full[st], GRAN_BYTES);
                 return smem + SP_OFF_RING + st * GRAN_BYTES;
             };
-            auto load_k = [&](const Walk &s, int tile) {
-                for (int d = 0; d < 4 && ok; d++) {
+            // one request per granule: a request occupies its thread for about 180 cycles, whatever its size
+            auto load_k = [&](const Walk &s, int tile) {  // granule: 128 dims (two 64-dim boxes) of 128 rows
+                for (int d = 0; d < 2 && ok; d++) {
                     uint8_t *dst = granule();
                     if (!(ok = dst != nullptr)) break;
-                    uint64_t *bar = &full[gi % SP_GRAN];
-                    if (s.own) tma_load_4d(dst, &ok_map, d * 64, tile * SP_N, s.hk, s.b, bar);
-                    else tma_load_3d(dst, &pk_map, d * 64, tile * SP_N, s.hk, bar);
+                    tma_load_5d(dst, s.own ? &ok_map : &pk_map, 0, tile * SP_N, 2 * d, s.hk, s.own ? s.b : 0, &full[gi % SP_GRAN]);
                     gi++;
                 }
             };
-            auto load_v = [&](const Walk &s, int tile) {
-                for (int r = 0; r < 4 && ok; r++) {
+            auto load_v = [&](const Walk &s, int tile) {  // granule: 256 dims (four 64-dim boxes) of 64 rows
+                for (int r = 0; r < 2 && ok; r++) {
                     uint8_t *dst = granule();
                     if (!(ok = dst != nullptr)) break;
-                    uint64_t *bar = &full[gi % SP_GRAN];
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        if (s.own) tma_load_4d(dst + d * 4096, &ov_map, d * 64, tile * SP_N + r * 32, s.hk, s.b, bar);
-                        else tma_load_3d(dst + d * 4096, &pv_map, d * 64, tile * SP_N + r * 32, s.hk, bar);
-                    }
+                    tma_load_5d(dst, s.own ? &ov_map : &pv_map, 0, tile * SP_N + r * 64, 0, s.hk, s.own ? s.b : 0, &full[gi % SP_GRAN]);
                     gi++;
                 }
             };
@@ -260,20 +254,21 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             constexpr uint32_t IDESC_PV = idesc_bf16(HEAD_DIM, 1);
             const uint64_t q_desc = smem_desc_sw128(smem_u32(smem), 16, 1024);
             const uint64_t k_desc = smem_desc_sw128(smem_u32(smem + SP_OFF_RING), 16, 1024);
-            // V: MN-major; 64-dim boxes 4096 B apart (LBO), 8-row groups 1024 B apart (SBO)
-            const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + SP_OFF_RING), 4096, 1024);
+            // V: MN-major; 64-dim boxes 8192 B apart (LBO), 8-row groups 1024 B apart (SBO)
+            const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + SP_OFF_RING), 8192, 1024);
             unsigned n = 0;   // tiles so far, over all segments
             unsigned seg = 0;
             auto issue_qk = [&](unsigned tile) -> bool {
                 if (tile > 0 && !mbar_wait_bounded(s_read, (tile - 1) & 1u)) return false;
-                for (int d = 0; d < 4; d++) {
+                for (int d = 0; d < 2; d++) {
                     const unsigned st = gi % SP_GRAN;
                     if (!mbar_wait_bounded(&full[st], (gi / SP_GRAN) & 1u)) return false;
                     tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < 4; ks++)
-                        tc_mma_bf16(tmem + TM_S, q_desc + (uint64_t)((d * SP_Q_BOX + ks * 32) >> 4),
-                                    k_desc + (uint64_t)((st * GRAN_BYTES + ks * 32) >> 4), IDESC_QK, d > 0 || ks > 0);
+                    for (int ks = 0; ks < 8; ks++)
+                        tc_mma_bf16(tmem + TM_S, q_desc + (uint64_t)(((2 * d + (ks >> 2)) * SP_Q_BOX + (ks & 3) * 32) >> 4),
+                                    k_desc + (uint64_t)((st * GRAN_BYTES + (ks >> 2) * 16384 + (ks & 3) * 32) >> 4), IDESC_QK,
+                                    d > 0 || ks > 0);
                     tc_commit(&empty[st]);
                     gi++;
                 }
@@ -291,14 +286,14 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                     ok = ok && mbar_wait_bounded(&p_ready[pb], (tile >> 1) & 1u);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int r = 0; r < 4; r++) {
+                    for (int r = 0; r < 2; r++) {
                         const unsigned st = gi % SP_GRAN;
                         ok = mbar_wait_bounded(&full[st], (gi / SP_GRAN) & 1u);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll
-                        for (int ks = 0; ks < 2; ks++)
-                            tc_mma_bf16_ts(tmem + TM_O, tmem + TM_P + pb * 64 + (r * 2 + ks) * 8,
+                        for (int ks = 0; ks < 4; ks++)
+                            tc_mma_bf16_ts(tmem + TM_O, tmem + TM_P + pb * 64 + (r * 4 + ks) * 8,
                                            v_desc + (uint64_t)((st * GRAN_BYTES + ks * 2048) >> 4), IDESC_PV,
                                            j > 0 || r > 0 || ks > 0);
                         tc_commit(&empty[st]);
@@ -339,24 +334,28 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             // ---- Q: this warp brings 16 rows, one 512-byte row per load; rows without a query are zero ----
             const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
             {
-                uint4 v[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int r = 16 * warp + i;
-                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                int64_t off = -1;  // lane i: offset of row 16 * warp + i
+                {
+                    const int r = 16 * warp + (lane & 15);
                     if (r < rows) {
                         const int idx = walk.mt * SP_M + r;
                         const int bt = idx / p.group, hg = idx - bt * p.group;
-                        const int b = walk.own ? walk.b : bt / p.T, t = walk.own ? bt : bt % p.T;
-                        v[i] = *reinterpret_cast<const uint4 *>(p.q + (int64_t)b * p.q_seq + (int64_t)t * p.q_token +
-                                                                (int64_t)(walk.hk * p.group + hg) * p.q_head + 8 * lane);
+                        const int b = walk.own ? walk.b : bt / p.T, t = walk.own ? bt : bt - b * p.T;
+                        off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(walk.hk * p.group + hg) * p.q_head;
                     }
                 }
+                const bool some = 16 * warp < rows;
+                uint4 v[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int r = 16 * warp + i;
-                    *reinterpret_cast<uint4 *>(smem + (lane >> 3) * SP_Q_BOX + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = v[i];
+                    const int64_t o = __shfl_sync(0xffffffffu, off, i);
+                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (some && 16 * warp + i < rows) v[i] = *reinterpret_cast<const uint4 *>(p.q + o + 8 * lane);
                 }
+                uint8_t *qb = smem + (lane >> 3) * SP_Q_BOX + 16 * warp * 128;
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    *reinterpret_cast<uint4 *>(qb + i * 128 + (((lane & 7) ^ (i & 7)) << 4)) = v[i];
             }
             fence_proxy_async_smem();
             tc_fence_before();  // O of the previous segment has been read
@@ -444,18 +443,18 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 if (walk.own && col0 + SP_N > walk.len) {
                     // Rows of the tile at and beyond the sequence's end carry weight zero, but 0 * NaN is NaN: whatever
                     // the cache holds there is cleared before the product.  (The last tile of the segment: its V
-                    // granules are the last four; they cannot be refilled before the product that this thread allows.)
-                    const unsigned g_end = 8 * (n + walk.nt);
-                    for (int r = 0; r < 4; r++) {
-                        const unsigned gidx = g_end - 4 + r, st = gidx % SP_GRAN;
-                        const int bad = max(0, walk.len - col0 - 32 * r);  // first row of the granule to clear
-                        if (bad >= 32) continue;
+                    // granules are the last two; they cannot be refilled before the product that this thread allows.)
+                    const unsigned g_end = 4 * (n + walk.nt);
+                    for (int r = 0; r < 2; r++) {
+                        const unsigned gidx = g_end - 2 + r, st = gidx % SP_GRAN;
+                        const int bad = max(0, walk.len - col0 - 64 * r);  // first row of the granule to clear
+                        if (bad >= 64) continue;
                         ok = warp_wait(&full[st], (gidx / SP_GRAN) & 1u);
                         if (!ok) break;
-                        for (int i = bad * 8 + tid; i < 32 * 8; i += 256)
+                        for (int i = bad * 8 + tid; i < 64 * 8; i += 256)
 #pragma unroll
                             for (int d = 0; d < 4; d++)
-                                *reinterpret_cast<uint4 *>(smem + SP_OFF_RING + st * GRAN_BYTES + d * 4096 + i * 16) =
+                                *reinterpret_cast<uint4 *>(smem + SP_OFF_RING + st * GRAN_BYTES + d * 8192 + i * 16) =
                                     make_uint4(0u, 0u, 0u, 0u);
                     }
                     if (!ok) break;
@@ -477,15 +476,16 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 ok = pair_sync();
                 if (!ok) break;
                 l_run += xl[(hf ^ 1) * SP_M + row];
+                // [dims / 4][rows of the slot][4]: consecutive lanes (rows) store consecutive 16 bytes
                 const size_t slot = (size_t)walk.unit + blockIdx.x;
-                const size_t prow = walk.own ? ((size_t)p.Hkv * p.prefix_mtiles + gridDim.x) * SP_M + slot * p.own_rows + row
-                                             : slot * SP_M + row;
+                const int srows = walk.own ? p.own_rows : SP_M;
+                const size_t row0 = walk.own ? ((size_t)p.Hkv * p.prefix_mtiles + gridDim.x) * SP_M + slot * p.own_rows : slot * SP_M;
                 const bool valid = row < rows;
                 if (valid && hf == 0) {
-                    p.part_m[prow] = m_run == -INFINITY ? -INFINITY : m_run * sl2;
-                    p.part_l[prow] = l_run;
+                    p.part_m[row0 + row] = m_run == -INFINITY ? -INFINITY : m_run * sl2;
+                    p.part_l[row0 + row] = l_run;
                 }
-                float *dst = p.part_o + prow * HEAD_DIM;
+                float4 *dst = reinterpret_cast<float4 *>(p.part_o + row0 * HEAD_DIM) + row;
 #pragma unroll 1
                 for (int c0 = 128 * hf; c0 < 128 * hf + 128; c0 += 32) {
                     float o[32];
@@ -493,8 +493,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                     tc_wait_ld();
                     if (valid)
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4 *>(dst + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 4) dst[(size_t)((c0 + i) >> 2) * srows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
                 ok = pair_sync();  // the other half has read the row sums
             }
@@ -510,64 +509,116 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     if (warp == 0) tmem_dealloc(tmem, SP_TMEM_COLS);
 }
 
-// One CTA (128 threads, two dims each) per query row: joins the partials of the prefix unit and of the own unit in the
-// order of the tile sequence, applies the gate.
-__global__ void __launch_bounds__(128) shared_attn_merge_kernel(const SharedAttnParams p) {
-    const int tid = threadIdx.x;
-    const int h = blockIdx.x % p.H, bt = blockIdx.x / p.H;
-    const int t = bt % p.T, b = bt / p.T;
-    const int hk = h / p.group, hg = h - hk * p.group;
+// Joins the partials of the query rows by log-sum-exp, in a fixed order, and applies the gate.  CTA = 32 consecutive
+// query rows of a kv head (lane = row) x 32 dims; warp w takes the partials w, w + 8, ... of every row (the prefix
+// unit's first, then the own unit's), and the warps' results are joined through shared memory.
+constexpr int MG_WARPS = 8;
+constexpr int MG_DIMS = 32;
+__global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const SharedAttnParams p) {
+    __shared__ float s_m[MG_WARPS][32], s_l[MG_WARPS][32];
+    __shared__ float4 s_o[MG_WARPS][MG_DIMS / 4][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows_hk = p.B * p.T * p.group;
+    const int blocks_hk = (rows_hk + 31) / 32;
+    const int hk = blockIdx.x / blocks_hk, idx = (blockIdx.x - hk * blocks_hk) * 32 + lane;
+    const int d0 = blockIdx.y * MG_DIMS;
     const int run = p.plan[0];
-    const size_t own_base = ((size_t)p.Hkv * p.prefix_mtiles + p.grid) * SP_M;
     // prefix: partials [0, np); own: partials [np, np + no)
-    int np = 0, no = 0;
-    size_t prow = 0, orow = 0;
-    if (p.prefix_tiles > 0) {
-        const int idx = bt * p.group + hg, mt = idx / SP_M;
-        const int unit = hk * p.prefix_mtiles + mt;
-        const int first = unit * p.prefix_tiles / run, last = ((unit + 1) * p.prefix_tiles - 1) / run;
-        np = last - first + 1;
-        prow = ((size_t)unit + first) * SP_M + (idx - mt * SP_M);
-    }
-    const int nt = own_tiles(p, b);
-    if (nt > 0) {
-        const int idx = t * p.group + hg, mt = idx / SP_M;
-        const int u = hk * p.own_mtiles + mt;
-        const int begin = p.plan[8 + b] + u * nt;
-        const int first = begin / run, last = (begin + nt - 1) / run;
-        no = last - first + 1;
-        orow = own_base + ((size_t)b * p.Hkv * p.own_mtiles + u + first) * p.own_rows + (idx - mt * SP_M);
-    }
-    auto part_row = [&](int c) -> size_t { return c < np ? prow + (size_t)c * SP_M : orow + (size_t)(c - np) * p.own_rows; };
-    const int parts = np + no;
-    float M = -INFINITY;
-    for (int c = 0; c < parts; c++) M = fmaxf(M, p.part_m[part_row(c)]);
-    float L = 0.0f;
-    float2 acc = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-    for (int c = 0; c < parts; c++) {
-        const size_t r = part_row(c);
-        const float m = p.part_m[r];
-        const float w = m == -INFINITY ? 0.0f : ex2_approx(m - M);
-        const float2 o = *reinterpret_cast<const float2 *>(p.part_o + r * HEAD_DIM + 2 * tid);
-        L += w * p.part_l[r];
-        if (w != 0.0f) {  // a partial without weight contributes nothing, whatever it holds
-            acc.x = fmaf(w, o.x, acc.x);
-            acc.y = fmaf(w, o.y, acc.y);
+    int np = 0, no = 0, b = 0, t = 0, hg = 0, pr = 0, orow = 0;
+    size_t p0 = 0, o0 = 0;  // first row of the first slot
+    if (idx < rows_hk) {
+        const int bt = idx / p.group;
+        hg = idx - bt * p.group;
+        b = bt / p.T;
+        t = bt - b * p.T;
+        if (p.prefix_tiles > 0) {
+            const int mt = idx / SP_M, unit = hk * p.prefix_mtiles + mt;
+            const int first = unit * p.prefix_tiles / run, last = ((unit + 1) * p.prefix_tiles - 1) / run;
+            np = last - first + 1;
+            p0 = ((size_t)unit + first) * SP_M;
+            pr = idx - mt * SP_M;
         }
+        const int nt = own_tiles(p, b);
+        if (nt > 0) {
+            const int i = t * p.group + hg, mt = i / SP_M, u = hk * p.own_mtiles + mt;
+            const int begin = p.plan[8 + b] + u * nt;
+            const int first = begin / run, last = (begin + nt - 1) / run;
+            no = last - first + 1;
+            o0 = ((size_t)p.Hkv * p.prefix_mtiles + p.grid) * SP_M + ((size_t)b * p.Hkv * p.own_mtiles + u + first) * p.own_rows;
+            orow = i - mt * SP_M;
+        }
+    }
+    float M = -INFINITY, L = 0.0f;
+    float4 acc[MG_DIMS / 4];
+#pragma unroll
+    for (int i = 0; i < MG_DIMS / 4; i++) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = warp; c < np + no; c += MG_WARPS) {
+        const bool pre = c < np;
+        const int srows = pre ? SP_M : p.own_rows, r = pre ? pr : orow;
+        const size_t row0 = pre ? p0 + (size_t)c * SP_M : o0 + (size_t)(c - np) * p.own_rows;
+        const float4 *src = reinterpret_cast<const float4 *>(p.part_o + row0 * HEAD_DIM) + r;
+        float4 o[MG_DIMS / 4];
+#pragma unroll
+        for (int i = 0; i < MG_DIMS / 4; i++) o[i] = src[(size_t)(d0 / 4 + i) * srows];
+        const float m = p.part_m[row0 + r], l = p.part_l[row0 + r];
+        if (m == -INFINITY) continue;  // no weight: contributes nothing, whatever it holds
+        const float mn = fmaxf(M, m);
+        const float wa = M == -INFINITY ? 0.0f : ex2_approx(M - mn), wb = ex2_approx(m - mn);
+        M = mn;
+        L = L * wa + l * wb;
+#pragma unroll
+        for (int i = 0; i < MG_DIMS / 4; i++) {
+            acc[i].x = fmaf(wb, o[i].x, acc[i].x * wa);
+            acc[i].y = fmaf(wb, o[i].y, acc[i].y * wa);
+            acc[i].z = fmaf(wb, o[i].z, acc[i].z * wa);
+            acc[i].w = fmaf(wb, o[i].w, acc[i].w * wa);
+        }
+    }
+    s_m[warp][lane] = M;
+    s_l[warp][lane] = L;
+#pragma unroll
+    for (int i = 0; i < MG_DIMS / 4; i++) s_o[warp][i][lane] = acc[i];
+    __syncthreads();
+    // thread = (row of the 32, four dims): eight threads write 64 consecutive bytes of a row
+    const int row = threadIdx.x >> 3, q4 = threadIdx.x & 7;
+    const int idx2 = (blockIdx.x - hk * blocks_hk) * 32 + row;
+    if (idx2 >= rows_hk) return;
+    M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < MG_WARPS; w++) M = fmaxf(M, s_m[w][row]);
+    L = 0.0f;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < MG_WARPS; w++) {
+        const float m = s_m[w][row];
+        if (m == -INFINITY) continue;
+        const float wt = ex2_approx(m - M);
+        const float4 o = s_o[w][q4][row];
+        L += wt * s_l[w][row];
+        a.x = fmaf(wt, o.x, a.x);
+        a.y = fmaf(wt, o.y, a.y);
+        a.z = fmaf(wt, o.z, a.z);
+        a.w = fmaf(wt, o.w, a.w);
     }
     const bool none = M == -INFINITY;
     const float inv = none ? 0.0f : 1.0f / L;
-    acc.x *= inv;
-    acc.y *= inv;
+    a.x *= inv;
+    a.y *= inv;
+    a.z *= inv;
+    a.w *= inv;
+    const int bt = idx2 / p.group, h = hk * p.group + (idx2 - bt * p.group);
+    const int d = d0 + 4 * q4;
     if (p.gate) {
-        const uint32_t gb = *reinterpret_cast<const uint32_t *>(p.gate + (int64_t)b * p.g_seq + (int64_t)t * p.g_token +
-                                                                (int64_t)h * p.g_head + 2 * tid);
-        acc.x *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb & 0xffffu))));
-        acc.y *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb >> 16))));
+        const int bb = bt / p.T, tt = bt - bb * p.T;
+        const uint2 gb = *reinterpret_cast<const uint2 *>(p.gate + (int64_t)bb * p.g_seq + (int64_t)tt * p.g_token + (int64_t)h * p.g_head + d);
+        a.x *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.x & 0xffffu))));
+        a.y *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.x >> 16))));
+        a.z *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.y & 0xffffu))));
+        a.w *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.y >> 16))));
     }
-    *reinterpret_cast<uint32_t *>(p.out + (size_t)blockIdx.x * HEAD_DIM + 2 * tid) = pack_bf16x2(acc.x, acc.y);
-    if (p.lse && tid == 0) p.lse[blockIdx.x] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    const size_t orw = (size_t)bt * p.H + h;
+    *reinterpret_cast<uint2 *>(p.out + orw * HEAD_DIM + d) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+    if (p.lse && d == 0) p.lse[orw] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace
@@ -582,7 +633,8 @@ cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &
     shared_prefix_attn_kernel<<<p.grid, SP_THREADS, SP_SMEM, stream>>>(pk, pv, ok, ov, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    shared_attn_merge_kernel<<<(unsigned)(p.B * p.T * p.H), 128, 0, stream>>>(p);
+    const unsigned blocks = (unsigned)(p.Hkv * ((p.B * p.T * p.group + 31) / 32));
+    shared_attn_merge_kernel<<<dim3(blocks, HEAD_DIM / MG_DIMS), 32 * MG_WARPS, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
