@@ -335,7 +335,7 @@ struct SharedAttnParams {
     __nv_bfloat16 *out;
     float *lse;
     float *part_o, *part_m, *part_l;  // partials: prefix slots of 128 rows, then own slots of own_rows rows
-    int *plan;                        // [0] tiles per CTA, [1] tiles in all, [8 + b] first tile of sequence b's own rows
+    int *plan;                        // [0] own tiles per CTA, [8 + b] first own tile of sequence b
     unsigned *status;
     int B, T, H, Hkv, group;
     int prefix_len, own_cap;

@@ -8,20 +8,24 @@
 // same 128 x 128 tiles with the unused query rows idle: such a tile takes 2048 tensor cycles for 128 KiB of rows, a
 // third of what HBM needs to deliver them, so the idle rows cost nothing.
 //
-// Work split: the 128-row tiles of all units -- (kv head, 128 query rows) over the prefix, (sequence, kv head) over its
-// own rows -- form one sequence, cut into equal runs, one persistent CTA per run and SM.  A CTA writes one un-normalised
-// partial (o, m, l) per unit it touches; merge_kernel joins the partials of a query row by log-sum-exp, in a fixed order,
-// and applies the gate.  Lengths are read on the device: every CTA finds its place by a scan over them.
+// Work split: the 128-row tiles of the prefix units (kv head, 128 query rows) form one sequence, those of the own units
+// (sequence, kv head) another; both are cut into equal runs, and the persistent CTA of an SM takes one run of each (of the
+// own tiles counted from the last CTA, so that a small call's two kinds meet on different SMs).  An own unit costs a
+// segment start and end (about 10 us in all) for a few tiles, so they are spread over all CTAs.  A CTA writes one
+// un-normalised partial (o, m, l) per unit it touches; the merge kernel joins the partials of a query row by log-sum-exp,
+// in a fixed order, and applies the gate.  Lengths are read on the device: every CTA finds its place by a scan over them.
 //
-// CTA (320 threads): warps 0-7 softmax (thread = query row x half of the 128 columns), warp 8 issues every tcgen05.mma,
-// warp 9 every TMA load.  Shared memory: Q 64 KiB and a ring of five 32 KiB granules that K and V share in the order in
+// CTA (576 threads): warps 0-15 softmax (thread = query row x a quarter of the 128 columns), warp 16 issues every
+// tcgen05.mma, warp 17 every TMA load.  Shared memory: Q 64 KiB and a ring of five 32 KiB granules that K and V share in the order in
 // which the tensor core takes them (K: 128 dims x 128 rows, V: 256 dims x 64 rows).  Tensor memory (512 columns): O 256,
 // S 128, P twice 64 (bf16, the A operand of P V straight from tensor memory).  S is free again as soon as the softmax
-// has read it, so Q K^T of tile j+1 runs under the softmax of tile j, and P V of tile j under that of tile j+1.  O is
-// rescaled only when a row maximum grows by more than 2^8.  P is rounded to bf16 (the type of V: both operands of one
+// has read it, so Q K^T of tile j+1 runs under the softmax of tile j, and P V of tile j under that of tile j+1.  A row's
+// reference maximum moves, and O is rescaled, only when some score exceeds it by more than 2^8: the warps of a quadrant
+// ask one another with one barrier reduction and exchange row maxima only then.  P is rounded to bf16 (the type of V: both operands of one
 // instruction have the same type); the row sums l are taken before that rounding.
-// Every mbarrier wait is bounded; a wait that runs out sets a status bit, and the CTA waits for its copies in flight,
-// frees its tensor memory and leaves.
+// Every mbarrier wait is bounded.  When one runs out the CTA sets a flag that ends all its waits; the softmax warps still
+// walk their tiles, without work, so that the block barriers among them stay paired; then a status bit is set, the CTA
+// waits for its copies in flight, frees its tensor memory and leaves.
 #include <math.h>
 
 #include "common.cuh"
@@ -34,7 +38,8 @@ namespace {
 
 constexpr int SP_M = SHARED_ATTN_M;
 constexpr int SP_N = SHARED_ATTN_N;
-constexpr int SP_THREADS = 320;
+constexpr int SP_SOFT = 16;                                // softmax warps: four per quadrant of tensor memory
+constexpr int SP_THREADS = 32 * (SP_SOFT + 2);
 constexpr int SP_GRAN = 5;                                 // granules of the K/V ring
 constexpr uint32_t GRAN_BYTES = 32768;
 constexpr uint32_t SP_Q_BOX = SP_M * 128;                  // 64 dims of 128 query rows
@@ -66,26 +71,47 @@ __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem,
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                 "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+// the 128 threads of a quadrant: barrier, and whether any of them passed a non-zero value
+__device__ __forceinline__ bool quad_any(int quad, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v), "r"(quad + 1)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void quad_sync(int quad) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
+
 __device__ __forceinline__ int own_len(const SharedAttnParams &p, int b) {
     const int n = p.lens[b];
     return (n < 0 || n > p.own_cap) ? 0 : n;
 }
 __device__ __forceinline__ int own_tiles(const SharedAttnParams &p, int b) { return (own_len(p, b) + SP_N - 1) / SP_N; }
 
-// A segment: the tiles [t0, t0 + nt) of one unit.  Every role of a CTA walks the same segments by itself.
+// A segment: the tiles [t0, t0 + nt) of one unit.  Every role of a CTA walks the same segments by itself: first its run
+// of the prefix tiles, then its run of the own tiles.
 struct Walk {
-    int at, end;        // tiles of the launch-wide sequence left to this CTA
-    int b, begin;       // own region: sequence at hand and its first tile
+    int at, end;          // prefix tiles left to this CTA
+    int own_at, own_end;  // own tiles left to it
+    int b, begin;         // sequence at hand and its first own tile
     // the segment at hand
     bool own;
-    int unit;           // index among the units of its kind
-    int hk, mt;         // kv head, tile of 128 query rows
-    int t0, nt, len;    // len: rows of the unit
+    int unit;             // index among the units of its kind
+    int hk, mt;           // kv head, tile of 128 query rows
+    int t0, nt, len;      // len: rows of the unit
 
     __device__ __forceinline__ bool next(const SharedAttnParams &p) {
-        if (at >= end) return false;
-        const int total_p = p.Hkv * p.prefix_mtiles * p.prefix_tiles;
-        if (at < total_p) {
+        if (at < end) {
             own = false;
             unit = at / p.prefix_tiles;
             hk = unit / p.prefix_mtiles;
@@ -93,24 +119,26 @@ struct Walk {
             t0 = at - unit * p.prefix_tiles;
             nt = min(p.prefix_tiles - t0, end - at);
             len = p.prefix_len;
-        } else {
-            const int per = p.Hkv * p.own_mtiles;
-            int nb = own_tiles(p, b);
-            while (at >= begin + per * nb) {
-                begin += per * nb;
-                b++;
-                nb = own_tiles(p, b);
-            }
-            own = true;
-            const int u = (at - begin) / nb;
-            hk = u / p.own_mtiles;
-            mt = u - hk * p.own_mtiles;
-            unit = b * per + u;
-            t0 = at - begin - u * nb;
-            nt = min(nb - t0, end - at);
-            len = own_len(p, b);
+            at += nt;
+            return true;
         }
-        at += nt;
+        if (own_at >= own_end) return false;
+        const int per = p.Hkv * p.own_mtiles;
+        int nb = own_tiles(p, b);
+        while (own_at >= begin + per * nb) {
+            begin += per * nb;
+            b++;
+            nb = own_tiles(p, b);
+        }
+        own = true;
+        const int u = (own_at - begin) / nb;
+        hk = u / p.own_mtiles;
+        mt = u - hk * p.own_mtiles;
+        unit = b * per + u;
+        t0 = own_at - begin - u * nb;
+        nt = min(nb - t0, own_end - own_at);
+        len = own_len(p, b);
+        own_at += nt;
         return true;
     }
 };
@@ -124,15 +152,14 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + SP_OFF_BAR);
     uint64_t *full = bars;                  // [5] TMA: granule landed
     uint64_t *empty = bars + SP_GRAN;       // [5] tcgen05.commit: the products that read the granule are done
-    uint64_t *s_ready = bars + 20;          // tcgen05.commit: scores of a tile are in tensor memory
-    uint64_t *s_read = bars + 21;           // 8 warps: scores are in registers
-    uint64_t *p_ready = bars + 22;          // [2] 8 warps: P of a tile is in tensor memory, O may be added to
-    uint64_t *pv_done = bars + 24;          // [2] tcgen05.commit: P V of a tile has been accumulated
-    uint64_t *q_ready = bars + 26;          // 8 warps: the segment's Q is in shared memory, O has been read out
-    uint64_t *x_ready = bars + 27;          // [4] 2 warps: both column halves of a lane quadrant have published
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 31);
-    volatile int *s_fail = reinterpret_cast<volatile int *>(bars + 32);
-    int *s_scan = reinterpret_cast<int *>(bars + 33);  // [10] + location [2]
+    uint64_t *s_ready = bars + 10;          // tcgen05.commit: scores of a tile are in tensor memory
+    uint64_t *s_read = bars + 11;           // softmax warps: scores are in registers
+    uint64_t *p_ready = bars + 12;          // [2] softmax warps: P of a tile is in tensor memory, O may be added to
+    uint64_t *pv_done = bars + 14;          // [2] tcgen05.commit: P V of a tile has been accumulated
+    uint64_t *q_ready = bars + 16;          // softmax warps: the segment's Q is in shared memory, O has been read out
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+    volatile int *s_fail = reinterpret_cast<volatile int *>(bars + 18);
+    int *s_scan = reinterpret_cast<int *>(bars + 19);  // one per warp, then the place [2]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -158,45 +185,43 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             mbar_init(&empty[i], 1);
         }
         mbar_init(s_ready, 1);
-        mbar_init(s_read, 8);
+        mbar_init(s_read, SP_SOFT);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&p_ready[i], 8);
+            mbar_init(&p_ready[i], SP_SOFT);
             mbar_init(&pv_done[i], 1);
         }
-        mbar_init(q_ready, 8);
-        for (int i = 0; i < 4; i++) mbar_init(&x_ready[i], 2);
+        mbar_init(q_ready, SP_SOFT);
         *s_fail = 0;
         mbar_fence_init();
     }
     __syncthreads();
     const int total_p = p.Hkv * p.prefix_mtiles * p.prefix_tiles;
-    int base = 0, total = total_p;
+    int base = 0, total_own = 0;
     for (int w = 0; w < SP_THREADS / 32; w++) {
         if (w < warp) base += s_scan[w];
-        total += s_scan[w];
+        total_own += s_scan[w];
     }
-    const int run = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int run = (total_p + (int)gridDim.x - 1) / (int)gridDim.x, own_run = max(1, (total_own + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int own_cta = (int)gridDim.x - 1 - (int)blockIdx.x;
     Walk walk;
-    walk.at = min((int)blockIdx.x * run, total);
-    walk.end = min(walk.at + run, total);
+    walk.at = min((int)blockIdx.x * run, total_p);
+    walk.end = min(walk.at + run, total_p);
+    walk.own_at = min(own_cta * own_run, total_own);
+    walk.own_end = min(walk.own_at + own_run, total_own);
     {
-        int first = total_p + base + inc - mine;
-        const int want = max(walk.at, total_p);
+        int first = base + inc - mine;
         for (int b = b_lo; b < b_hi; b++) {
             const int n = per_seq * own_tiles(p, b);
             if (blockIdx.x == 0) p.plan[8 + b] = first;
-            if (want >= first && want < first + n) {
-                s_scan[10] = b;
-                s_scan[11] = first;
+            if (walk.own_at >= first && walk.own_at < first + n) {
+                s_scan[SP_THREADS / 32] = b;
+                s_scan[SP_THREADS / 32 + 1] = first;
             }
             first += n;
         }
-        if (blockIdx.x == 0 && tid == 0) {
-            p.plan[0] = run;
-            p.plan[1] = total;
-        }
+        if (blockIdx.x == 0 && tid == 0) p.plan[0] = own_run;
     }
-    if (walk.at >= walk.end) return;  // more CTAs than tiles
+    if (walk.at >= walk.end && walk.own_at >= walk.own_end) return;  // more CTAs than tiles
 
     if (warp == 0) {
         tmem_alloc(tmem_slot, SP_TMEM_COLS);
@@ -205,13 +230,13 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    walk.b = s_scan[10];  // used only when the run reaches the own region (then some thread has set them)
-    walk.begin = s_scan[11];
+    walk.b = s_scan[SP_THREADS / 32];  // used only when the CTA has own tiles (then some thread has set them)
+    walk.begin = s_scan[SP_THREADS / 32 + 1];
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
     unsigned gi = 0;  // granules requested (producer) or consumed (issuer)
 
-    if (warp == 9) {
+    if (warp == SP_SOFT + 1) {
         // ================= producer: one lane issues every TMA load =================
         if (lane == 0) {
             auto granule = [&]() -> uint8_t * {  // waits until the next granule is free, arms its barrier
@@ -238,6 +263,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                     gi++;
                 }
             };
+            // The first requests wait for the query rows: those asked for behind every CTA's first 160 KiB came 6 us later.
+            ok = mbar_wait_bounded(q_ready, 0);
             while (ok && walk.next(p)) {
                 load_k(walk, walk.t0);
                 for (int j = 0; j < walk.nt && ok; j++) {
@@ -247,7 +274,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             }
             if (!ok) *s_fail = 1;
         }
-    } else if (warp == 8) {
+    } else if (warp == SP_SOFT) {
         // ================= issuer: one lane drives the tensor core =================
         if (lane == 0) {
             constexpr uint32_t IDESC_QK = idesc_bf16(SP_N, 0);
@@ -307,12 +334,12 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             if (!ok) *s_fail = 1;
         }
     } else {
-        // ================= softmax warps: thread = (query row, half of the columns) =================
-        const int quad = warp & 3, hf = warp >> 2;
+        // ================= softmax warps: thread = (query row, quarter of the columns) =================
+        const int quad = warp & 3, qt = warp >> 2;
         const int row = 32 * quad + lane;  // query row of the tile = lane of tensor memory
         const uint32_t lane_base = tmem + ((uint32_t)(32 * quad) << 16);
-        __nv_bfloat16 *xm = reinterpret_cast<__nv_bfloat16 *>(smem + SP_OFF_XM);  // [2 tiles][2 halves][128 rows]
-        float *xl = reinterpret_cast<float *>(smem + SP_OFF_XM);                  // [2 halves][128 rows]
+        __nv_bfloat16 *xm = reinterpret_cast<__nv_bfloat16 *>(smem + SP_OFF_XM);  // [4 quarters][128 rows] row maxima
+        float *xl = reinterpret_cast<float *>(smem);                              // [4][128] row sums, where Q was
         const float sl2 = p.scale * LOG2E_SP;
         const int tg = p.T * p.group;
         auto warp_arrive = [&](uint64_t *bar) {
@@ -322,40 +349,32 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         auto warp_wait = [&](uint64_t *bar, unsigned parity) -> bool {
             return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity) && *s_fail == 0);
         };
-        unsigned x_phase = 0;
-        auto pair_sync = [&]() -> bool {  // the two warps of a quadrant
-            warp_arrive(&x_ready[quad]);
-            const bool done = warp_wait(&x_ready[quad], x_phase & 1u);
-            x_phase++;
-            return done;
+        auto give_up = [&]() {
+            if (lane == 0) *s_fail = 1;
         };
         unsigned n = 0;
-        while (ok && walk.next(p)) {
-            // ---- Q: this warp brings 16 rows, one 512-byte row per load; rows without a query are zero ----
+        while (walk.next(p)) {
+            // ---- Q: this warp brings 8 rows, one 512-byte row per load; rows without a query are zero ----
             const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
             {
-                int64_t off = -1;  // lane i: offset of row 16 * warp + i
-                {
-                    const int r = 16 * warp + (lane & 15);
-                    if (r < rows) {
-                        const int idx = walk.mt * SP_M + r;
-                        const int bt = idx / p.group, hg = idx - bt * p.group;
-                        const int b = walk.own ? walk.b : bt / p.T, t = walk.own ? bt : bt - b * p.T;
-                        off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(walk.hk * p.group + hg) * p.q_head;
-                    }
+                int64_t off = 0;  // lane i: offset of row 8 * warp + i
+                const int r = 8 * warp + (lane & 7);
+                if (r < rows) {
+                    const int idx = walk.mt * SP_M + r;
+                    const int bt = idx / p.group, hg = idx - bt * p.group;
+                    const int b = walk.own ? walk.b : bt / p.T, t = walk.own ? bt : bt - b * p.T;
+                    off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(walk.hk * p.group + hg) * p.q_head;
                 }
-                const bool some = 16 * warp < rows;
-                uint4 v[16];
+                uint4 v[8];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
+                for (int i = 0; i < 8; i++) {
                     const int64_t o = __shfl_sync(0xffffffffu, off, i);
                     v[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (some && 16 * warp + i < rows) v[i] = *reinterpret_cast<const uint4 *>(p.q + o + 8 * lane);
+                    if (8 * warp + i < rows) v[i] = *reinterpret_cast<const uint4 *>(p.q + o + 8 * lane);
                 }
-                uint8_t *qb = smem + (lane >> 3) * SP_Q_BOX + 16 * warp * 128;
+                uint8_t *qb = smem + (lane >> 3) * SP_Q_BOX + 8 * warp * 128;
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    *reinterpret_cast<uint4 *>(qb + i * 128 + (((lane & 7) ^ (i & 7)) << 4)) = v[i];
+                for (int i = 0; i < 8; i++) *reinterpret_cast<uint4 *>(qb + i * 128 + (((lane & 7) ^ i) << 4)) = v[i];
             }
             fence_proxy_async_smem();
             tc_fence_before();  // O of the previous segment has been read
@@ -365,80 +384,78 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             int lim = walk.len;
             if (walk.own) lim = walk.len - (p.T - 1 - (walk.mt * SP_M + row) / p.group);
             const int safe = walk.own ? walk.len - (p.T - 1) : walk.len;  // columns that every row sees
-            const bool live = 32 * quad < rows;                           // some row of this warp carries a query
-            float m_run = -INFINITY, l_run = 0.0f;  // l_run: this thread's half of the columns
-            for (int j = 0; j < walk.nt && ok; j++) {
+            const bool live = 32 * quad < rows;                           // some row of this quadrant carries a query
+            float m_run = -INFINITY, l_run = 0.0f;  // m_run: reference maximum of the row; l_run: this thread's quarter
+            for (int j = 0; j < walk.nt; j++) {
                 const unsigned tile = n + j, pb = tile & 1u;
                 const int col0 = (walk.t0 + j) * SP_N;
-                ok = warp_wait(s_ready, tile & 1u);
-                if (!ok) break;
+                ok = ok && warp_wait(s_ready, tile & 1u);
+                if (!ok) give_up();
                 tc_fence_after();
-                float s[64];
+                float s[32];
                 if (live) {
-                    tmem_ld32(lane_base + TM_S + 64 * hf, s);
-                    tmem_ld32(lane_base + TM_S + 64 * hf + 32, s + 32);
+                    tmem_ld32(lane_base + TM_S + 32 * qt, s);
                     tc_wait_ld();
                 }
                 tc_fence_before();
                 warp_arrive(s_read);
                 float corr = 1.0f;
-                bool warp_rescale = false;
-                uint32_t pk[32];
+                bool rescale = false;
+                uint32_t pk[16];
                 if (live) {
-                    const int c0 = col0 + 64 * hf;
+                    const int c0 = col0 + 32 * qt;
                     if (col0 + SP_N > safe) {
 #pragma unroll
-                        for (int c = 0; c < 64; c++)
+                        for (int c = 0; c < 32; c++)
                             if (c0 + c >= lim) s[c] = -INFINITY;
                     }
-                    float mx = s[0];
+                    float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int c = 1; c < 64; c++) mx = fmaxf(mx, s[c]);
-                    // both halves of a row use one maximum: each rounds its own up to bf16 (the running maximum only
-                    // has to bound the scores, roughly) and takes the larger
-                    const __nv_bfloat16 mx_b = __float2bfloat16_ru(mx);
-                    xm[(pb * 2 + hf) * SP_M + row] = mx_b;
-                    ok = pair_sync();
-                    if (!ok) break;
-                    const float m_tile = fmaxf(__bfloat162float(mx_b), __bfloat162float(xm[(pb * 2 + (hf ^ 1)) * SP_M + row]));
-                    const float m_new = fmaxf(m_run, m_tile);
-                    const bool need = (m_new - m_run) * sl2 > 8.0f;  // also true for the first finite maximum
-                    warp_rescale = __any_sync(0xffffffffu, need);
-                    if (warp_rescale) {
+                    for (int c = 4; c < 32; c++) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                    // true as well for the first finite maximum (m_run = -inf)
+                    rescale = quad_any(quad, (mx - m_run) * sl2 > 8.0f);
+                    if (rescale) {
+                        // one maximum for all quarters of a row: each rounds its own up to bf16 (the reference only has
+                        // to bound the scores, roughly), the largest counts
+                        const __nv_bfloat16 mx_b = __float2bfloat16_ru(mx);
+                        xm[qt * SP_M + row] = mx_b;
+                        quad_sync(quad);
+                        float m_new = m_run;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) m_new = fmaxf(m_new, __bfloat162float(xm[k * SP_M + row]));
                         corr = m_new == -INFINITY ? 1.0f : ex2_approx((m_run - m_new) * sl2);
                         m_run = m_new;
+                        quad_sync(quad);  // the exchange area is free again
                     }
                     const float mb = m_run == -INFINITY ? 0.0f : m_run * sl2;
-                    float rs = 0.0f;
+                    float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2) {
+                    for (int c = 0; c < 32; c += 2) {
                         const float p0 = ex2_approx(fmaf(s[c], sl2, -mb));
                         const float p1 = ex2_approx(fmaf(s[c + 1], sl2, -mb));
-                        rs += p0 + p1;
+                        rs[(c >> 1) & 3] += p0 + p1;
                         pk[c >> 1] = pack_bf16x2(p0, p1);
                     }
-                    l_run = l_run * corr + rs;
+                    l_run = l_run * corr + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
                 }
                 // P buffer pb was last read by P V of tile - 2
-                if (tile >= 2) {
-                    ok = warp_wait(&pv_done[pb], ((tile - 2) >> 1) & 1u);
-                    if (!ok) break;
-                }
-                if (warp_rescale && j > 0) {  // O may be touched once P V of the tile before has been added
-                    ok = warp_wait(&pv_done[pb ^ 1u], ((tile - 1) >> 1) & 1u);
-                    if (!ok) break;
+                if (tile >= 2) ok = ok && warp_wait(&pv_done[pb], ((tile - 2) >> 1) & 1u);
+                if (rescale && j > 0) {  // O may be touched once P V of the tile before has been added
+                    ok = ok && warp_wait(&pv_done[pb ^ 1u], ((tile - 1) >> 1) & 1u);
                     tc_fence_after();
+                    if (ok)
 #pragma unroll 1
-                    for (int c0 = 128 * hf; c0 < 128 * hf + 128; c0 += 32) {
-                        float o[32];
-                        tmem_ld32(lane_base + TM_O + c0, o);
-                        tc_wait_ld();
+                        for (int c0 = 64 * qt; c0 < 64 * qt + 64; c0 += 32) {
+                            float o[32];
+                            tmem_ld32(lane_base + TM_O + c0, o);
+                            tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] *= corr;
-                        tmem_st32(lane_base + TM_O + c0, *reinterpret_cast<float(*)[32]>(&o[0]));
-                    }
+                            for (int i = 0; i < 32; i++) o[i] *= corr;
+                            tmem_st32(lane_base + TM_O + c0, *reinterpret_cast<float(*)[32]>(&o[0]));
+                        }
                 }
-                if (live) tmem_st32(lane_base + TM_P + pb * 64 + 32 * hf, *reinterpret_cast<float(*)[32]>(&pk[0]));
+                if (live && ok) tmem_st16(lane_base + TM_P + pb * 64 + 16 * qt, pk);
                 tc_wait_st();
                 if (walk.own && col0 + SP_N > walk.len) {
                     // Rows of the tile at and beyond the sequence's end carry weight zero, but 0 * NaN is NaN: whatever
@@ -449,62 +466,60 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                         const unsigned gidx = g_end - 2 + r, st = gidx % SP_GRAN;
                         const int bad = max(0, walk.len - col0 - 64 * r);  // first row of the granule to clear
                         if (bad >= 64) continue;
-                        ok = warp_wait(&full[st], (gidx / SP_GRAN) & 1u);
+                        ok = ok && warp_wait(&full[st], (gidx / SP_GRAN) & 1u);
                         if (!ok) break;
-                        for (int i = bad * 8 + tid; i < 64 * 8; i += 256)
+                        for (int i = bad * 8 + tid; i < 64 * 8; i += 32 * SP_SOFT)
 #pragma unroll
                             for (int d = 0; d < 4; d++)
                                 *reinterpret_cast<uint4 *>(smem + SP_OFF_RING + st * GRAN_BYTES + d * 8192 + i * 16) =
                                     make_uint4(0u, 0u, 0u, 0u);
                     }
-                    if (!ok) break;
                     fence_proxy_async_smem();
                 }
+                if (!ok) give_up();
                 tc_fence_before();
                 warp_arrive(&p_ready[pb]);
             }
-            if (!ok) break;
             // ---- the segment's partial ----
             n += walk.nt;
-            ok = warp_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u);
-            if (!ok) break;
+            ok = ok && warp_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u);
+            if (!ok) give_up();
             tc_fence_after();
             if (live) {
-                ok = pair_sync();  // the exchange area may still be read by the other half
-                if (!ok) break;
-                xl[hf * SP_M + row] = l_run;
-                ok = pair_sync();
-                if (!ok) break;
-                l_run += xl[(hf ^ 1) * SP_M + row];
+                xl[qt * SP_M + row] = l_run;
+                quad_sync(quad);
+                l_run = (xl[row] + xl[SP_M + row]) + (xl[2 * SP_M + row] + xl[3 * SP_M + row]);
                 // [dims / 4][rows of the slot][4]: consecutive lanes (rows) store consecutive 16 bytes
-                const size_t slot = (size_t)walk.unit + blockIdx.x;
+                const size_t slot = (size_t)walk.unit + (walk.own ? own_cta : (int)blockIdx.x);
                 const int srows = walk.own ? p.own_rows : SP_M;
                 const size_t row0 = walk.own ? ((size_t)p.Hkv * p.prefix_mtiles + gridDim.x) * SP_M + slot * p.own_rows : slot * SP_M;
-                const bool valid = row < rows;
-                if (valid && hf == 0) {
+                const bool valid = ok && row < rows;
+                if (valid && qt == 0) {
                     p.part_m[row0 + row] = m_run == -INFINITY ? -INFINITY : m_run * sl2;
                     p.part_l[row0 + row] = l_run;
                 }
                 float4 *dst = reinterpret_cast<float4 *>(p.part_o + row0 * HEAD_DIM) + row;
+                if (ok)
 #pragma unroll 1
-                for (int c0 = 128 * hf; c0 < 128 * hf + 128; c0 += 32) {
-                    float o[32];
-                    tmem_ld32(lane_base + TM_O + c0, o);
-                    tc_wait_ld();
-                    if (valid)
+                    for (int c0 = 64 * qt; c0 < 64 * qt + 64; c0 += 32) {
+                        float o[32];
+                        tmem_ld32(lane_base + TM_O + c0, o);
+                        tc_wait_ld();
+                        if (valid)
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) dst[(size_t)((c0 + i) >> 2) * srows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                }
-                ok = pair_sync();  // the other half has read the row sums
+                            for (int i = 0; i < 32; i += 4) dst[(size_t)((c0 + i) >> 2) * srows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
             }
+            // every quadrant has read its row sums before Q of the next segment lands on them
+            if (walk.at < walk.end || walk.own_at < walk.own_end)
+                asm volatile("barrier.cta.sync 5, %0;" ::"n"(32 * SP_SOFT) : "memory");
         }
-        if (!ok && lane == 0) *s_fail = 1;
     }
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && *s_fail) atomicOr(p.status, STATUS_TMA_TIMEOUT);
     // on the ordinary path every granule has been used; after a failure the copies in flight land before the CTA leaves
-    if (warp == 9 && lane == 0 && *s_fail)
+    if (warp == SP_SOFT + 1 && lane == 0 && *s_fail)
         for (unsigned k = gi > SP_GRAN ? gi - SP_GRAN : 0; k < gi; k++) mbar_wait_bounded(&full[k % SP_GRAN], (k / SP_GRAN) & 1u);
     if (warp == 0) tmem_dealloc(tmem, SP_TMEM_COLS);
 }
@@ -522,7 +537,7 @@ __global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const 
     const int blocks_hk = (rows_hk + 31) / 32;
     const int hk = blockIdx.x / blocks_hk, idx = (blockIdx.x - hk * blocks_hk) * 32 + lane;
     const int d0 = blockIdx.y * MG_DIMS;
-    const int run = p.plan[0];
+    const int own_run = p.plan[0], run = (p.Hkv * p.prefix_mtiles * p.prefix_tiles + p.grid - 1) / p.grid;
     // prefix: partials [0, np); own: partials [np, np + no)
     int np = 0, no = 0, b = 0, t = 0, hg = 0, pr = 0, orow = 0;
     size_t p0 = 0, o0 = 0;  // first row of the first slot
@@ -542,7 +557,7 @@ __global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const 
         if (nt > 0) {
             const int i = t * p.group + hg, mt = i / SP_M, u = hk * p.own_mtiles + mt;
             const int begin = p.plan[8 + b] + u * nt;
-            const int first = begin / run, last = (begin + nt - 1) / run;
+            const int first = begin / own_run, last = (begin + nt - 1) / own_run;
             no = last - first + 1;
             o0 = ((size_t)p.Hkv * p.prefix_mtiles + p.grid) * SP_M + ((size_t)b * p.Hkv * p.own_mtiles + u + first) * p.own_rows;
             orow = i - mt * SP_M;
