@@ -90,6 +90,18 @@ __device__ __forceinline__ bool quad_any(int quad, bool v) {
         : "memory");
     return r != 0;
 }
+// One lane of a converged warp, always the same.  The warps that issue TMA and tensor-core instructions run their loops
+// as whole warps and let this lane issue: addresses and descriptors are then uniform values for the compiler, where a
+// lane-0 branch around the whole loop cost 75 cycles per issued instruction.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)::"memory");
+    return r != 0;
+}
 __device__ __forceinline__ void quad_sync(int quad) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
 
 __device__ __forceinline__ int own_len(const SharedAttnParams &p, int b) {
@@ -233,106 +245,115 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     walk.b = s_scan[SP_THREADS / 32];  // used only when the CTA has own tiles (then some thread has set them)
     walk.begin = s_scan[SP_THREADS / 32 + 1];
     const uint32_t tmem = *tmem_slot;
+    auto warp_wait = [&](uint64_t *bar, unsigned parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity) && *s_fail == 0);
+    };
     bool ok = true;
     unsigned gi = 0;  // granules requested (producer) or consumed (issuer)
 
     if (warp == SP_SOFT + 1) {
         // ================= producer: one lane issues every TMA load =================
-        if (lane == 0) {
-            auto granule = [&]() -> uint8_t * {  // waits until the next granule is free, arms its barrier
-                const unsigned st = gi % SP_GRAN, round = gi / SP_GRAN;
-                if (round > 0 && !mbar_wait_bounded(&empty[st], (round - 1) & 1u)) return nullptr;
-                if (*s_fail) return nullptr;
-                mbar_expect_tx(&full[st], GRAN_BYTES);
-                return smem + SP_OFF_RING + st * GRAN_BYTES;
-            };
-            // one request per granule: a request occupies its thread for about 180 cycles, whatever its size
-            auto load_k = [&](const Walk &s, int tile) {  // granule: 128 dims (two 64-dim boxes) of 128 rows
-                for (int d = 0; d < 2 && ok; d++) {
-                    uint8_t *dst = granule();
-                    if (!(ok = dst != nullptr)) break;
-                    tma_load_5d(dst, s.own ? &ok_map : &pk_map, 0, tile * SP_N, 2 * d, s.hk, s.own ? s.b : 0, &full[gi % SP_GRAN]);
-                    gi++;
+        auto granule = [&]() -> bool {  // waits until the next granule is free
+            const unsigned st = gi % SP_GRAN, round = gi / SP_GRAN;
+            return round == 0 || warp_wait(&empty[st], (round - 1) & 1u);
+        };
+        // one request per granule: a request costs its thread about 180 cycles, whatever its size
+        auto load_k = [&](const Walk &s, int tile) {  // granule: 128 dims (two 64-dim boxes) of 128 rows
+            for (int d = 0; d < 2 && ok; d++) {
+                ok = granule();
+                if (!ok) break;
+                const unsigned st = gi % SP_GRAN;
+                if (elect_one()) {
+                    mbar_expect_tx(&full[st], GRAN_BYTES);
+                    tma_load_5d(smem + SP_OFF_RING + st * GRAN_BYTES, s.own ? &ok_map : &pk_map, 0, tile * SP_N, 2 * d, s.hk, s.own ? s.b : 0,
+                                &full[st]);
                 }
-            };
-            auto load_v = [&](const Walk &s, int tile) {  // granule: 256 dims (four 64-dim boxes) of 64 rows
-                for (int r = 0; r < 2 && ok; r++) {
-                    uint8_t *dst = granule();
-                    if (!(ok = dst != nullptr)) break;
-                    tma_load_5d(dst, s.own ? &ov_map : &pv_map, 0, tile * SP_N + r * 64, 0, s.hk, s.own ? s.b : 0, &full[gi % SP_GRAN]);
-                    gi++;
-                }
-            };
-            // The first requests wait for the query rows: those asked for behind every CTA's first 160 KiB came 6 us later.
-            ok = mbar_wait_bounded(q_ready, 0);
-            while (ok && walk.next(p)) {
-                load_k(walk, walk.t0);
-                for (int j = 0; j < walk.nt && ok; j++) {
-                    if (j + 1 < walk.nt) load_k(walk, walk.t0 + j + 1);
-                    load_v(walk, walk.t0 + j);
-                }
+                gi++;
             }
-            if (!ok) *s_fail = 1;
+        };
+        auto load_v = [&](const Walk &s, int tile) {  // granule: 256 dims (four 64-dim boxes) of 64 rows
+            for (int r = 0; r < 2 && ok; r++) {
+                ok = granule();
+                if (!ok) break;
+                const unsigned st = gi % SP_GRAN;
+                if (elect_one()) {
+                    mbar_expect_tx(&full[st], GRAN_BYTES);
+                    tma_load_5d(smem + SP_OFF_RING + st * GRAN_BYTES, s.own ? &ov_map : &pv_map, 0, tile * SP_N + r * 64, 0, s.hk,
+                                s.own ? s.b : 0, &full[st]);
+                }
+                gi++;
+            }
+        };
+        // The first requests wait for the query rows: those asked for behind every CTA's first 160 KiB came 6 us later.
+        ok = warp_wait(q_ready, 0);
+        while (ok && walk.next(p)) {
+            load_k(walk, walk.t0);
+            for (int j = 0; j < walk.nt && ok; j++) {
+                if (j + 1 < walk.nt) load_k(walk, walk.t0 + j + 1);
+                load_v(walk, walk.t0 + j);
+            }
         }
+        if (!ok) *s_fail = 1;
     } else if (warp == SP_SOFT) {
         // ================= issuer: one lane drives the tensor core =================
-        if (lane == 0) {
-            constexpr uint32_t IDESC_QK = idesc_bf16(SP_N, 0);
-            constexpr uint32_t IDESC_PV = idesc_bf16(HEAD_DIM, 1);
-            const uint64_t q_desc = smem_desc_sw128(smem_u32(smem), 16, 1024);
-            const uint64_t k_desc = smem_desc_sw128(smem_u32(smem + SP_OFF_RING), 16, 1024);
-            // V: MN-major; 64-dim boxes 8192 B apart (LBO), 8-row groups 1024 B apart (SBO)
-            const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + SP_OFF_RING), 8192, 1024);
-            unsigned n = 0;   // tiles so far, over all segments
-            unsigned seg = 0;
-            auto issue_qk = [&](unsigned tile) -> bool {
-                if (tile > 0 && !mbar_wait_bounded(s_read, (tile - 1) & 1u)) return false;
-                for (int d = 0; d < 2; d++) {
-                    const unsigned st = gi % SP_GRAN;
-                    if (!mbar_wait_bounded(&full[st], (gi / SP_GRAN) & 1u)) return false;
-                    tc_fence_after();
+        constexpr uint32_t IDESC_QK = idesc_bf16(SP_N, 0);
+        constexpr uint32_t IDESC_PV = idesc_bf16(HEAD_DIM, 1);
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(smem), 16, 1024);
+        const uint64_t k_desc = smem_desc_sw128(smem_u32(smem + SP_OFF_RING), 16, 1024);
+        // V: MN-major; 64-dim boxes 8192 B apart (LBO), 8-row groups 1024 B apart (SBO)
+        const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + SP_OFF_RING), 8192, 1024);
+        unsigned n = 0;   // tiles so far, over all segments
+        unsigned seg = 0;
+        auto issue_qk = [&](unsigned tile) -> bool {
+            if (tile > 0 && !warp_wait(s_read, (tile - 1) & 1u)) return false;
+            for (int d = 0; d < 2; d++) {
+                const unsigned st = gi % SP_GRAN;
+                if (!warp_wait(&full[st], (gi / SP_GRAN) & 1u)) return false;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t qd = q_desc + (uint64_t)((2 * d * SP_Q_BOX) >> 4), kd = k_desc + (uint64_t)((st * GRAN_BYTES) >> 4);
 #pragma unroll
                     for (int ks = 0; ks < 8; ks++)
-                        tc_mma_bf16(tmem + TM_S, q_desc + (uint64_t)(((2 * d + (ks >> 2)) * SP_Q_BOX + (ks & 3) * 32) >> 4),
-                                    k_desc + (uint64_t)((st * GRAN_BYTES + (ks >> 2) * 16384 + (ks & 3) * 32) >> 4), IDESC_QK,
-                                    d > 0 || ks > 0);
+                        tc_mma_bf16(tmem + TM_S, qd + (uint64_t)(((ks >> 2) * SP_Q_BOX + (ks & 3) * 32) >> 4),
+                                    kd + (uint64_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4), IDESC_QK, d > 0 || ks > 0);
                     tc_commit(&empty[st]);
-                    gi++;
+                    if (d == 1) tc_commit(s_ready);
                 }
-                tc_commit(s_ready);
-                return true;
-            };
-            while (ok && walk.next(p)) {
-                ok = mbar_wait_bounded(q_ready, seg & 1u);
+                gi++;
+            }
+            return true;
+        };
+        while (ok && walk.next(p)) {
+            ok = warp_wait(q_ready, seg & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            ok = issue_qk(n);
+            for (int j = 0; j < walk.nt && ok; j++) {
+                if (j + 1 < walk.nt) ok = issue_qk(n + j + 1);
+                const unsigned tile = n + j, pb = tile & 1u;
+                ok = ok && warp_wait(&p_ready[pb], (tile >> 1) & 1u);
                 if (!ok) break;
-                tc_fence_after();
-                ok = issue_qk(n);
-                for (int j = 0; j < walk.nt && ok; j++) {
-                    if (j + 1 < walk.nt) ok = issue_qk(n + j + 1);
-                    const unsigned tile = n + j, pb = tile & 1u;
-                    ok = ok && mbar_wait_bounded(&p_ready[pb], (tile >> 1) & 1u);
+                for (int r = 0; r < 2; r++) {
+                    const unsigned st = gi % SP_GRAN;
+                    ok = warp_wait(&full[st], (gi / SP_GRAN) & 1u);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int r = 0; r < 2; r++) {
-                        const unsigned st = gi % SP_GRAN;
-                        ok = mbar_wait_bounded(&full[st], (gi / SP_GRAN) & 1u);
-                        if (!ok) break;
-                        tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t vd = v_desc + (uint64_t)((st * GRAN_BYTES) >> 4);
+                        const uint32_t pa = tmem + TM_P + pb * 64 + r * 32;
 #pragma unroll
                         for (int ks = 0; ks < 4; ks++)
-                            tc_mma_bf16_ts(tmem + TM_O, tmem + TM_P + pb * 64 + (r * 4 + ks) * 8,
-                                           v_desc + (uint64_t)((st * GRAN_BYTES + ks * 2048) >> 4), IDESC_PV,
-                                           j > 0 || r > 0 || ks > 0);
+                            tc_mma_bf16_ts(tmem + TM_O, pa + ks * 8, vd + (uint64_t)((ks * 2048) >> 4), IDESC_PV, j > 0 || r > 0 || ks > 0);
                         tc_commit(&empty[st]);
-                        gi++;
+                        if (r == 1) tc_commit(&pv_done[pb]);
                     }
-                    if (ok) tc_commit(&pv_done[pb]);
+                    gi++;
                 }
-                n += walk.nt;
-                seg++;
             }
-            if (!ok) *s_fail = 1;
+            n += walk.nt;
+            seg++;
         }
+        if (!ok) *s_fail = 1;
     } else {
         // ================= softmax warps: thread = (query row, quarter of the columns) =================
         const int quad = warp & 3, qt = warp >> 2;
@@ -345,9 +366,6 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         auto warp_arrive = [&](uint64_t *bar) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
-        };
-        auto warp_wait = [&](uint64_t *bar, unsigned parity) -> bool {
-            return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity) && *s_fail == 0);
         };
         auto give_up = [&]() {
             if (lane == 0) *s_fail = 1;
