@@ -15,13 +15,15 @@
 // un-normalised partial (o, m, l) per unit it touches; the merge kernel joins the partials of a query row by log-sum-exp,
 // in a fixed order, and applies the gate.  Lengths are read on the device: every CTA finds its place by a scan over them.
 //
-// CTA (576 threads): warps 0-15 softmax (thread = query row x a quarter of the 128 columns), warp 16 issues every
-// tcgen05.mma, warp 17 every TMA load.  Shared memory: Q 64 KiB and a ring of five 32 KiB granules that K and V share in the order in
+// CTA (320 threads): warps 0-7 softmax (thread = query row x half of the 128 columns), warp 8 issues every tcgen05.mma,
+// warp 9 every TMA load.  Shared memory: Q 64 KiB and a ring of five 32 KiB granules that K and V share in the order in
 // which the tensor core takes them (K: 128 dims x 128 rows, V: 256 dims x 64 rows).  Tensor memory (512 columns): O 256,
 // S 128, P twice 64 (bf16, the A operand of P V straight from tensor memory).  S is free again as soon as the softmax
-// has read it, so Q K^T of tile j+1 runs under the softmax of tile j, and P V of tile j under that of tile j+1.  A row's
-// reference maximum moves, and O is rescaled, only when some score exceeds it by more than 2^8: the warps of a quadrant
-// ask one another with one barrier reduction and exchange row maxima only then.  P is rounded to bf16 (the type of V: both operands of one
+// has read it, so Q K^T of tile j+1 runs under the softmax of tile j, and P V of tile j under that of tile j+1.  The
+// reference that a row's exponents are taken against is the maximum of its first tile and moves, with a rescaling of O,
+// only when some score exceeds it by more than 2^32 (fp32 and bf16 have the exponents to spare, and no digits are lost):
+// so no maximum stands before the exponentials of a tile; its rows' maxima are taken along with them, and the two halves
+// of a row ask one another with one barrier reduction whether either must move, which redoes the tile.  P is rounded to bf16 (the type of V: both operands of one
 // instruction have the same type); the row sums l are taken before that rounding.
 // Every mbarrier wait is bounded.  When one runs out the CTA sets a flag that ends all its waits; the softmax warps still
 // walk their tiles, without work, so that the block barriers among them stay paired; then a status bit is set, the CTA
@@ -38,7 +40,7 @@ namespace {
 
 constexpr int SP_M = SHARED_ATTN_M;
 constexpr int SP_N = SHARED_ATTN_N;
-constexpr int SP_SOFT = 16;                                // softmax warps: four per quadrant of tensor memory
+constexpr int SP_SOFT = 8;                                 // softmax warps: two per quadrant of tensor memory
 constexpr int SP_THREADS = 32 * (SP_SOFT + 2);
 constexpr int SP_GRAN = 5;                                 // granules of the K/V ring
 constexpr uint32_t GRAN_BYTES = 32768;
@@ -71,19 +73,13 @@ __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem,
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-                 "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
-// the 128 threads of a quadrant: barrier, and whether any of them passed a non-zero value
+// the 64 threads of a quadrant's rows: barrier, and whether any of them passed a non-zero value
 __device__ __forceinline__ bool quad_any(int quad, bool v) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+        "barrier.cta.red.or.pred q, %2, 64, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
         : "r"((uint32_t)v), "r"(quad + 1)
@@ -102,7 +98,7 @@ __device__ __forceinline__ bool elect_one() {
         : "=r"(r)::"memory");
     return r != 0;
 }
-__device__ __forceinline__ void quad_sync(int quad) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
+__device__ __forceinline__ void quad_sync(int quad) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
 
 __device__ __forceinline__ int own_len(const SharedAttnParams &p, int b) {
     const int n = p.lens[b];
@@ -355,12 +351,12 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         }
         if (!ok) *s_fail = 1;
     } else {
-        // ================= softmax warps: thread = (query row, quarter of the columns) =================
-        const int quad = warp & 3, qt = warp >> 2;
+        // ================= softmax warps: thread = (query row, half of the columns) =================
+        const int quad = warp & 3, hf = warp >> 2;
         const int row = 32 * quad + lane;  // query row of the tile = lane of tensor memory
         const uint32_t lane_base = tmem + ((uint32_t)(32 * quad) << 16);
-        __nv_bfloat16 *xm = reinterpret_cast<__nv_bfloat16 *>(smem + SP_OFF_XM);  // [4 quarters][128 rows] row maxima
-        float *xl = reinterpret_cast<float *>(smem);                              // [4][128] row sums, where Q was
+        float *xm = reinterpret_cast<float *>(smem + SP_OFF_XM);  // [2 halves][128 rows] row maxima
+        float *xl = reinterpret_cast<float *>(smem);              // [2][128] row sums, where Q was
         const float sl2 = p.scale * LOG2E_SP;
         const int tg = p.T * p.group;
         auto warp_arrive = [&](uint64_t *bar) {
@@ -372,27 +368,27 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         };
         unsigned n = 0;
         while (walk.next(p)) {
-            // ---- Q: this warp brings 8 rows, one 512-byte row per load; rows without a query are zero ----
+            // ---- Q: this warp brings 16 rows, one 512-byte row per load; rows without a query are zero ----
             const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
             {
-                int64_t off = 0;  // lane i: offset of row 8 * warp + i
-                const int r = 8 * warp + (lane & 7);
+                int64_t off = 0;  // lane i: offset of row 16 * warp + i
+                const int r = 16 * warp + (lane & 15);
                 if (r < rows) {
                     const int idx = walk.mt * SP_M + r;
                     const int bt = idx / p.group, hg = idx - bt * p.group;
                     const int b = walk.own ? walk.b : bt / p.T, t = walk.own ? bt : bt - b * p.T;
                     off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(walk.hk * p.group + hg) * p.q_head;
                 }
-                uint4 v[8];
+                uint4 v[16];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < 16; i++) {
                     const int64_t o = __shfl_sync(0xffffffffu, off, i);
                     v[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (8 * warp + i < rows) v[i] = *reinterpret_cast<const uint4 *>(p.q + o + 8 * lane);
+                    if (16 * warp + i < rows) v[i] = *reinterpret_cast<const uint4 *>(p.q + o + 8 * lane);
                 }
-                uint8_t *qb = smem + (lane >> 3) * SP_Q_BOX + 8 * warp * 128;
+                uint8_t *qb = smem + (lane >> 3) * SP_Q_BOX + 16 * warp * 128;
 #pragma unroll
-                for (int i = 0; i < 8; i++) *reinterpret_cast<uint4 *>(qb + i * 128 + (((lane & 7) ^ i) << 4)) = v[i];
+                for (int i = 0; i < 16; i++) *reinterpret_cast<uint4 *>(qb + i * 128 + (((lane & 7) ^ (i & 7)) << 4)) = v[i];
             }
             fence_proxy_async_smem();
             tc_fence_before();  // O of the previous segment has been read
@@ -403,59 +399,74 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             if (walk.own) lim = walk.len - (p.T - 1 - (walk.mt * SP_M + row) / p.group);
             const int safe = walk.own ? walk.len - (p.T - 1) : walk.len;  // columns that every row sees
             const bool live = 32 * quad < rows;                           // some row of this quadrant carries a query
-            float m_run = -INFINITY, l_run = 0.0f;  // m_run: reference maximum of the row; l_run: this thread's quarter
+            float m_run = -INFINITY, l_run = 0.0f;  // m_run: reference of the row's exponents; l_run: this thread's half
             for (int j = 0; j < walk.nt; j++) {
                 const unsigned tile = n + j, pb = tile & 1u;
                 const int col0 = (walk.t0 + j) * SP_N;
                 ok = ok && warp_wait(s_ready, tile & 1u);
                 if (!ok) give_up();
                 tc_fence_after();
-                float s[32];
+                float s[64];
                 if (live) {
-                    tmem_ld32(lane_base + TM_S + 32 * qt, s);
+                    tmem_ld32(lane_base + TM_S + 64 * hf, s);
+                    tmem_ld32(lane_base + TM_S + 64 * hf + 32, s + 32);
                     tc_wait_ld();
                 }
                 tc_fence_before();
                 warp_arrive(s_read);
                 float corr = 1.0f;
                 bool rescale = false;
-                uint32_t pk[16];
+                uint32_t pk[32];
                 if (live) {
-                    const int c0 = col0 + 32 * qt;
+                    const int c0 = col0 + 64 * hf;
                     if (col0 + SP_N > safe) {
 #pragma unroll
-                        for (int c = 0; c < 32; c++)
+                        for (int c = 0; c < 64; c++)
                             if (c0 + c >= lim) s[c] = -INFINITY;
                     }
-                    float mx4[4] = {s[0], s[1], s[2], s[3]};
+                    auto row_max = [&]() {
+                        float a = fmaxf(s[0], s[1]), b = fmaxf(s[2], s[3]);
 #pragma unroll
-                    for (int c = 4; c < 32; c++) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    // true as well for the first finite maximum (m_run = -inf)
-                    rescale = quad_any(quad, (mx - m_run) * sl2 > 8.0f);
-                    if (rescale) {
-                        // one maximum for all quarters of a row: each rounds its own up to bf16 (the reference only has
-                        // to bound the scores, roughly), the largest counts
-                        const __nv_bfloat16 mx_b = __float2bfloat16_ru(mx);
-                        xm[qt * SP_M + row] = mx_b;
+                        for (int c = 4; c < 64; c += 4) {
+                            a = fmaxf(a, fmaxf(s[c], s[c + 1]));
+                            b = fmaxf(b, fmaxf(s[c + 2], s[c + 3]));
+                        }
+                        return fmaxf(a, b);
+                    };
+                    auto move_reference = [&](float mx) {  // to the maximum of the row so far
+                        xm[hf * SP_M + row] = mx;
                         quad_sync(quad);
-                        float m_new = m_run;
-#pragma unroll
-                        for (int k = 0; k < 4; k++) m_new = fmaxf(m_new, __bfloat162float(xm[k * SP_M + row]));
+                        const float m_new = fmaxf(m_run, fmaxf(mx, xm[(hf ^ 1) * SP_M + row]));
                         corr = m_new == -INFINITY ? 1.0f : ex2_approx((m_run - m_new) * sl2);
                         m_run = m_new;
                         quad_sync(quad);  // the exchange area is free again
-                    }
-                    const float mb = m_run == -INFINITY ? 0.0f : m_run * sl2;
-                    float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    };
+                    if (j == 0) move_reference(row_max());
+                    float rs;
+                    auto to_p = [&]() {
+                        const float mb = m_run == -INFINITY ? 0.0f : m_run * sl2;
+                        float r0 = 0.0f, r1 = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float p0 = ex2_approx(fmaf(s[c], sl2, -mb));
-                        const float p1 = ex2_approx(fmaf(s[c + 1], sl2, -mb));
-                        rs[(c >> 1) & 3] += p0 + p1;
-                        pk[c >> 1] = pack_bf16x2(p0, p1);
+                        for (int c = 0; c < 64; c += 2) {
+                            const float p0 = ex2_approx(fmaf(s[c], sl2, -mb));
+                            const float p1 = ex2_approx(fmaf(s[c + 1], sl2, -mb));
+                            r0 += p0;
+                            r1 += p1;
+                            pk[c >> 1] = pack_bf16x2(p0, p1);
+                        }
+                        rs = r0 + r1;
+                    };
+                    to_p();
+                    if (j > 0) {
+                        const float mx = row_max();
+                        // true as well for the first finite score of a row (m_run = -inf)
+                        rescale = quad_any(quad, (mx - m_run) * sl2 > 32.0f);
+                        if (rescale) {
+                            move_reference(mx);
+                            to_p();
+                        }
                     }
-                    l_run = l_run * corr + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+                    l_run = l_run * corr + rs;
                 }
                 // P buffer pb was last read by P V of tile - 2
                 if (tile >= 2) ok = ok && warp_wait(&pv_done[pb], ((tile - 2) >> 1) & 1u);
@@ -464,7 +475,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                     tc_fence_after();
                     if (ok)
 #pragma unroll 1
-                        for (int c0 = 64 * qt; c0 < 64 * qt + 64; c0 += 32) {
+                        for (int c0 = 128 * hf; c0 < 128 * hf + 128; c0 += 32) {
                             float o[32];
                             tmem_ld32(lane_base + TM_O + c0, o);
                             tc_wait_ld();
@@ -473,7 +484,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                             tmem_st32(lane_base + TM_O + c0, *reinterpret_cast<float(*)[32]>(&o[0]));
                         }
                 }
-                if (live && ok) tmem_st16(lane_base + TM_P + pb * 64 + 16 * qt, pk);
+                if (live && ok) tmem_st32(lane_base + TM_P + pb * 64 + 32 * hf, *reinterpret_cast<float(*)[32]>(&pk[0]));
                 tc_wait_st();
                 if (walk.own && col0 + SP_N > walk.len) {
                     // Rows of the tile at and beyond the sequence's end carry weight zero, but 0 * NaN is NaN: whatever
@@ -504,22 +515,22 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             if (!ok) give_up();
             tc_fence_after();
             if (live) {
-                xl[qt * SP_M + row] = l_run;
+                xl[hf * SP_M + row] = l_run;
                 quad_sync(quad);
-                l_run = (xl[row] + xl[SP_M + row]) + (xl[2 * SP_M + row] + xl[3 * SP_M + row]);
+                l_run = xl[row] + xl[SP_M + row];
                 // [dims / 4][rows of the slot][4]: consecutive lanes (rows) store consecutive 16 bytes
                 const size_t slot = (size_t)walk.unit + (walk.own ? own_cta : (int)blockIdx.x);
                 const int srows = walk.own ? p.own_rows : SP_M;
                 const size_t row0 = walk.own ? ((size_t)p.Hkv * p.prefix_mtiles + gridDim.x) * SP_M + slot * p.own_rows : slot * SP_M;
                 const bool valid = ok && row < rows;
-                if (valid && qt == 0) {
+                if (valid && hf == 0) {
                     p.part_m[row0 + row] = m_run == -INFINITY ? -INFINITY : m_run * sl2;
                     p.part_l[row0 + row] = l_run;
                 }
                 float4 *dst = reinterpret_cast<float4 *>(p.part_o + row0 * HEAD_DIM) + row;
                 if (ok)
 #pragma unroll 1
-                    for (int c0 = 64 * qt; c0 < 64 * qt + 64; c0 += 32) {
+                    for (int c0 = 128 * hf; c0 < 128 * hf + 128; c0 += 32) {
                         float o[32];
                         tmem_ld32(lane_base + TM_O + c0, o);
                         tc_wait_ld();
