@@ -50,6 +50,7 @@ constexpr uint32_t SP_OFF_XM = SP_OFF_RING + SP_GRAN * GRAN_BYTES;  // row-maxim
 constexpr uint32_t SP_OFF_BAR = SP_OFF_XM + 1024;
 constexpr uint32_t SP_SMEM = SP_OFF_BAR + 512 + 1024;      // + alignment slack
 static_assert(SP_SMEM <= 232448, "shared memory of an SM");
+constexpr unsigned SP_SPINS = 1u << 22;                     // polls of a bounded wait, each a hardware-defined short time
 constexpr float LOG2E_SP = 1.4426950408889634f;
 
 constexpr uint32_t SP_TMEM_COLS = 512;
@@ -241,8 +242,23 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     walk.b = s_scan[SP_THREADS / 32];  // used only when the CTA has own tiles (then some thread has set them)
     walk.begin = s_scan[SP_THREADS / 32 + 1];
     const uint32_t tmem = *tmem_slot;
+    // Bounded waits of a whole warp, on one barrier or on three at once (a wait that succeeds at once still costs a round
+    // trip to shared memory, so the issuer asks for all it needs in one go).  The failure flag is looked at only after a
+    // poll that found nothing.
     auto warp_wait = [&](uint64_t *bar, unsigned parity) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity) && *s_fail == 0);
+        for (unsigned i = 0; i < SP_SPINS; i++) {
+            if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+            if (*s_fail) return false;
+        }
+        return false;
+    };
+    auto warp_wait3 = [&](uint64_t *b0, unsigned p0, uint64_t *b1, unsigned p1, uint64_t *b2, unsigned p2) -> bool {
+        for (unsigned i = 0; i < SP_SPINS; i++) {
+            const bool r0 = mbar_try_wait(b0, p0), r1 = mbar_try_wait(b1, p1), r2 = mbar_try_wait(b2, p2);
+            if (__all_sync(0xffffffffu, r0 && r1 && r2)) return true;
+            if (*s_fail) return false;
+        }
+        return false;
     };
     bool ok = true;
     unsigned gi = 0;  // granules requested (producer) or consumed (issuer)
@@ -301,22 +317,24 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         unsigned n = 0;   // tiles so far, over all segments
         unsigned seg = 0;
         auto issue_qk = [&](unsigned tile) -> bool {
-            if (tile > 0 && !warp_wait(s_read, (tile - 1) & 1u)) return false;
-            for (int d = 0; d < 2; d++) {
-                const unsigned st = gi % SP_GRAN;
-                if (!warp_wait(&full[st], (gi / SP_GRAN) & 1u)) return false;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t qd = q_desc + (uint64_t)((2 * d * SP_Q_BOX) >> 4), kd = k_desc + (uint64_t)((st * GRAN_BYTES) >> 4);
+            const unsigned sa = gi % SP_GRAN, sb = (gi + 1) % SP_GRAN;
+            // s_read: the softmax has taken the scores of the tile before (a phase ahead of the first tile passes at once)
+            if (!warp_wait3(s_read, (tile - 1) & 1u, &full[sa], (gi / SP_GRAN) & 1u, &full[sb], ((gi + 1) / SP_GRAN) & 1u)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    const uint64_t qd = q_desc + (uint64_t)((2 * d * SP_Q_BOX) >> 4);
+                    const uint64_t kd = k_desc + (uint64_t)(((d ? sb : sa) * GRAN_BYTES) >> 4);
 #pragma unroll
                     for (int ks = 0; ks < 8; ks++)
                         tc_mma_bf16(tmem + TM_S, qd + (uint64_t)(((ks >> 2) * SP_Q_BOX + (ks & 3) * 32) >> 4),
                                     kd + (uint64_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4), IDESC_QK, d > 0 || ks > 0);
-                    tc_commit(&empty[st]);
-                    if (d == 1) tc_commit(s_ready);
+                    tc_commit(&empty[d ? sb : sa]);
                 }
-                gi++;
+                tc_commit(s_ready);
             }
+            gi += 2;
             return true;
         };
         while (ok && walk.next(p)) {
@@ -327,24 +345,23 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             for (int j = 0; j < walk.nt && ok; j++) {
                 if (j + 1 < walk.nt) ok = issue_qk(n + j + 1);
                 const unsigned tile = n + j, pb = tile & 1u;
-                ok = ok && warp_wait(&p_ready[pb], (tile >> 1) & 1u);
+                const unsigned sa = gi % SP_GRAN, sb = (gi + 1) % SP_GRAN;
+                ok = ok && warp_wait3(&p_ready[pb], (tile >> 1) & 1u, &full[sa], (gi / SP_GRAN) & 1u, &full[sb], ((gi + 1) / SP_GRAN) & 1u);
                 if (!ok) break;
-                for (int r = 0; r < 2; r++) {
-                    const unsigned st = gi % SP_GRAN;
-                    ok = warp_wait(&full[st], (gi / SP_GRAN) & 1u);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t vd = v_desc + (uint64_t)((st * GRAN_BYTES) >> 4);
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const uint64_t vd = v_desc + (uint64_t)(((r ? sb : sa) * GRAN_BYTES) >> 4);
                         const uint32_t pa = tmem + TM_P + pb * 64 + r * 32;
 #pragma unroll
                         for (int ks = 0; ks < 4; ks++)
                             tc_mma_bf16_ts(tmem + TM_O, pa + ks * 8, vd + (uint64_t)((ks * 2048) >> 4), IDESC_PV, j > 0 || r > 0 || ks > 0);
-                        tc_commit(&empty[st]);
-                        if (r == 1) tc_commit(&pv_done[pb]);
+                        tc_commit(&empty[r ? sb : sa]);
                     }
-                    gi++;
+                    tc_commit(&pv_done[pb]);
                 }
+                gi += 2;
             }
             n += walk.nt;
             seg++;
@@ -442,29 +459,29 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                         quad_sync(quad);  // the exchange area is free again
                     };
                     if (j == 0) move_reference(row_max());
-                    float rs;
+                    float rs, mx;
                     auto to_p = [&]() {
                         const float mb = m_run == -INFINITY ? 0.0f : m_run * sl2;
-                        float r0 = 0.0f, r1 = 0.0f;
+                        float r0 = 0.0f, r1 = 0.0f, a = s[0], b = s[1];
 #pragma unroll
                         for (int c = 0; c < 64; c += 2) {
                             const float p0 = ex2_approx(fmaf(s[c], sl2, -mb));
                             const float p1 = ex2_approx(fmaf(s[c + 1], sl2, -mb));
+                            a = fmaxf(a, s[c]);
+                            b = fmaxf(b, s[c + 1]);
                             r0 += p0;
                             r1 += p1;
                             pk[c >> 1] = pack_bf16x2(p0, p1);
                         }
                         rs = r0 + r1;
+                        mx = fmaxf(a, b);
                     };
                     to_p();
-                    if (j > 0) {
-                        const float mx = row_max();
-                        // true as well for the first finite score of a row (m_run = -inf)
-                        rescale = quad_any(quad, (mx - m_run) * sl2 > 32.0f);
-                        if (rescale) {
-                            move_reference(mx);
-                            to_p();
-                        }
+                    // true as well for the first finite score of a row (m_run = -inf)
+                    rescale = quad_any(quad, (mx - m_run) * sl2 > 32.0f);
+                    if (rescale) {
+                        move_reference(mx);
+                        to_p();
                     }
                     l_run = l_run * corr + rs;
                 }
