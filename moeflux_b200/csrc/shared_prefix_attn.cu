@@ -165,7 +165,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     uint64_t *s_read = bars + 11;           // softmax warps: scores are in registers
     uint64_t *p_ready = bars + 12;          // [2] softmax warps: P of a tile is in tensor memory, O may be added to
     uint64_t *pv_done = bars + 14;          // [2] tcgen05.commit: P V of a tile has been accumulated
-    uint64_t *q_ready = bars + 16;          // softmax warps: the segment's Q is in shared memory, O has been read out
+    uint64_t *q_ready = bars + 16;          // softmax warps: the segment's Q is in shared memory
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
     volatile int *s_fail = reinterpret_cast<volatile int *>(bars + 18);
     int *s_scan = reinterpret_cast<int *>(bars + 19);  // one per warp, then the place [2]
@@ -372,8 +372,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         const int quad = warp & 3, hf = warp >> 2;
         const int row = 32 * quad + lane;  // query row of the tile = lane of tensor memory
         const uint32_t lane_base = tmem + ((uint32_t)(32 * quad) << 16);
-        float *xm = reinterpret_cast<float *>(smem + SP_OFF_XM);  // [2 halves][128 rows] row maxima
-        float *xl = reinterpret_cast<float *>(smem);              // [2][128] row sums, where Q was
+        float *xm = reinterpret_cast<float *>(smem + SP_OFF_XM);  // [2 halves][128 rows] row maxima, row sums
         const float sl2 = p.scale * LOG2E_SP;
         const int tg = p.T * p.group;
         auto warp_arrive = [&](uint64_t *bar) {
@@ -383,34 +382,39 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         auto give_up = [&]() {
             if (lane == 0) *s_fail = 1;
         };
-        unsigned n = 0;
-        while (walk.next(p)) {
-            // ---- Q: this warp brings 16 rows, one 512-byte row per load; rows without a query are zero ----
-            const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
-            {
-                int64_t off = 0;  // lane i: offset of row 16 * warp + i
-                const int r = 16 * warp + (lane & 15);
-                if (r < rows) {
-                    const int idx = walk.mt * SP_M + r;
-                    const int bt = idx / p.group, hg = idx - bt * p.group;
-                    const int b = walk.own ? walk.b : bt / p.T, t = walk.own ? bt : bt - b * p.T;
-                    off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(walk.hk * p.group + hg) * p.q_head;
-                }
-                uint4 v[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int64_t o = __shfl_sync(0xffffffffu, off, i);
-                    v[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (16 * warp + i < rows) v[i] = *reinterpret_cast<const uint4 *>(p.q + o + 8 * lane);
-                }
-                uint8_t *qb = smem + (lane >> 3) * SP_Q_BOX + 16 * warp * 128;
-#pragma unroll
-                for (int i = 0; i < 16; i++) *reinterpret_cast<uint4 *>(qb + i * 128 + (((lane & 7) ^ (i & 7)) << 4)) = v[i];
+        // Q of a segment: this warp copies 16 rows, one 512-byte row per instruction, without registers in between; rows
+        // without a query are zero.  The copies are complete, for this thread, after q_landed().
+        auto request_q = [&](const Walk &w) {
+            const int rows = w.own ? min(SP_M, tg - w.mt * SP_M) : min(SP_M, p.B * tg - w.mt * SP_M);
+            int64_t off = 0;  // lane i: offset of row 16 * warp + i
+            const int r = 16 * warp + (lane & 15);
+            if (r < rows) {
+                const int idx = w.mt * SP_M + r;
+                const int bt = idx / p.group, hg = idx - bt * p.group;
+                const int b = w.own ? w.b : bt / p.T, t = w.own ? bt : bt - b * p.T;
+                off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(w.hk * p.group + hg) * p.q_head;
             }
+            const uint32_t qb = smem_u32(smem + (lane >> 3) * SP_Q_BOX + 16 * warp * 128);
+#pragma unroll 4
+            for (int i = 0; i < 16; i++) {
+                const int64_t o = __shfl_sync(0xffffffffu, off, i);
+                const uint32_t bytes = 16 * warp + i < rows ? 16u : 0u;  // 0: the 16 bytes are filled with zeros
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(qb + i * 128 + (((lane & 7) ^ (i & 7)) << 4)),
+                             "l"(p.q + o + 8 * lane), "r"(bytes)
+                             : "memory");
+            }
+        };
+        auto q_landed = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async_smem();
-            tc_fence_before();  // O of the previous segment has been read
             warp_arrive(q_ready);
-
+        };
+        unsigned n = 0;
+        bool more = walk.next(p);
+        request_q(walk);  // (a CTA without a tile has left)
+        q_landed();
+        while (more) {
+            const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
             // columns of the unit this row sees
             int lim = walk.len;
             if (walk.own) lim = walk.len - (p.T - 1 - (walk.mt * SP_M + row) / p.group);
@@ -526,19 +530,23 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 tc_fence_before();
                 warp_arrive(&p_ready[pb]);
             }
-            // ---- the segment's partial ----
-            n += walk.nt;
+            // ---- the segment's partial; the next segment's Q comes in meanwhile ----
+            const Walk seg = walk;
+            more = walk.next(p);
+            if (more) request_q(walk);  // the products that read Q of this segment are done: their scores have been read
+            n += seg.nt;
             ok = ok && warp_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u);
             if (!ok) give_up();
             tc_fence_after();
+            if (more) q_landed();  // its first scores are computed under the stores below
             if (live) {
-                xl[hf * SP_M + row] = l_run;
+                xm[hf * SP_M + row] = l_run;
                 quad_sync(quad);
-                l_run = xl[row] + xl[SP_M + row];
+                l_run = xm[row] + xm[SP_M + row];
                 // [dims / 4][rows of the slot][4]: consecutive lanes (rows) store consecutive 16 bytes
-                const size_t slot = (size_t)walk.unit + (walk.own ? own_cta : (int)blockIdx.x);
-                const int srows = walk.own ? p.own_rows : SP_M;
-                const size_t row0 = walk.own ? ((size_t)p.Hkv * p.prefix_mtiles + gridDim.x) * SP_M + slot * p.own_rows : slot * SP_M;
+                const size_t slot = (size_t)seg.unit + (seg.own ? own_cta : (int)blockIdx.x);
+                const int srows = seg.own ? p.own_rows : SP_M;
+                const size_t row0 = seg.own ? ((size_t)p.Hkv * p.prefix_mtiles + gridDim.x) * SP_M + slot * p.own_rows : slot * SP_M;
                 const bool valid = ok && row < rows;
                 if (valid && hf == 0) {
                     p.part_m[row0 + row] = m_run == -INFINITY ? -INFINITY : m_run * sl2;
@@ -556,9 +564,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                             for (int i = 0; i < 32; i += 4) dst[(size_t)((c0 + i) >> 2) * srows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
             }
-            // every quadrant has read its row sums before Q of the next segment lands on them
-            if (walk.at < walk.end || walk.own_at < walk.own_end)
-                asm volatile("barrier.cta.sync 5, %0;" ::"n"(32 * SP_SOFT) : "memory");
+            if (live) quad_sync(quad);  // the exchange area is free again
+            tc_fence_before();          // O has been read: P of the next segment's first tile says so to the issuer
         }
     }
     tc_fence_before();
