@@ -21,7 +21,7 @@ namespace mfc {
 
 namespace {
 
-constexpr int VD_THREADS = 512;
+constexpr int VD_THREADS = 256;
 constexpr int VD_WARPS = VD_THREADS / 32;
 constexpr int VD_SEG = 1024;     // entries of a segment
 constexpr int VD_MAX_SEGS = 512;  // segments of a CTA's run kept in shared memory; longer runs use longer segments
@@ -205,9 +205,9 @@ cudaError_t verify_drafts_configure() {
 
 cudaError_t launch_verify_drafts(const VerifyParams &p, int n_sms, cudaStream_t stream) {
     if (p.B <= 0) return cudaSuccess;
-    // as many CTAs per sequence as keep every SM busy once, but at least four segments each
+    // CTAs per sequence: up to eight a SM in all, but at least two segments each
     int cs = 1;
-    while (cs < VD_MAX_CLUSTER && p.B * cs * 2 <= 2 * n_sms && (int64_t)p.V > (int64_t)cs * 4 * VD_SEG) cs *= 2;
+    while (cs < VD_MAX_CLUSTER && p.B * cs < 8 * n_sms && (int64_t)p.V > (int64_t)cs * 2 * VD_SEG) cs *= 2;
     int64_t seg = VD_SEG;  // longer segments where a run would not fit the table of sums
     while ((p.V + seg - 1) / seg > (int64_t)cs * VD_MAX_SEGS) seg *= 2;
     cudaLaunchConfig_t cfg = {};
