@@ -98,6 +98,7 @@ struct mfc_ctx {
     unsigned *tickets = nullptr, *group_tickets = nullptr, *status = nullptr;
     unsigned *mv_sched = nullptr;  // two pairs (tile counter, finished CTAs) of the one-vector projection kernel, used in turn
     unsigned mv_launches = 0;
+    int *evict_counts = nullptr;   // moves of every unit of an eviction
     int *serve_plan = nullptr;     // tile plan of a shared-prefix attention call (written by its main kernel, read by its merge)
     bool mv_overlap = true;        // tuning "matvec_overlap"
     struct MvMap {
@@ -865,7 +866,7 @@ mfc_ctx *mfc_open(const mfc_config *cfg) {
          DA(sc_o, (size_t)c->max_parts * 16 * HEAD_DIM, false) && DA(sc_m, (size_t)c->max_parts * 16, false) &&
          DA(sc_l, (size_t)c->max_parts * 16, false) && DA(tickets, mb * g.num_kv_heads, true) &&
          DA(group_tickets, c->max_parts, true) && DA(status, 1, true) && DA(mv_sched, 4, true) &&
-         DA(serve_plan, SHARED_ATTN_PLAN_INTS, true) &&
+         DA(serve_plan, SHARED_ATTN_PLAN_INTS, true) && DA(evict_counts, EVICT_MAX_UNITS, true) &&
          DA(phase_trace, (size_t)mfc_ctx::MAX_TRACE_CTAS * PHASE_TRACE_WORDS, true) && DA(st_q, mb * qd, false) &&
          DA(st_gate, mb * qd, false) && DA(st_k, mb * kvd, false) && DA(st_v, mb * kvd, false) &&
          DA(st_out, mb * qd, false) && DA(st_qkv, mb * c->conv_dim, false) && DA(st_z, mb * vd, false) &&
@@ -1748,9 +1749,34 @@ int mfc_kv_evict_dev(mfc_ctx *c, const mfc_kv_evict *a) try {
     p.budget = a->budget;
     p.n_sink = a->n_sink;
     p.n_recent = a->n_recent;
+    p.max_moves = a->budget < a->cap ? (a->budget < a->cap - a->budget ? a->budget : a->cap - a->budget) : 1;
+    // the moves are listed in the split-K scratch: as many sequences per launch as their lists fit
+    const size_t list_bytes = sizeof(int2) * (size_t)p.max_moves * p.Hkv, scratch = sizeof(float) * (size_t)c->max_parts * 16 * HEAD_DIM;
+    int64_t per_launch = (int64_t)(scratch / list_bytes);
+    if (per_launch > EVICT_MAX_UNITS / p.Hkv) per_launch = EVICT_MAX_UNITS / p.Hkv;
+    if (per_launch < 1) {
+        fail(c, "the moves of one sequence exceed the scratch reserved at open: fewer kv heads or rows per call");
+        return -1;
+    }
+    p.moves = (int2 *)c->sc_o;
+    p.counts = c->evict_counts;
     DeviceScope dev(c->cfg.device);
-    CK(launch_kv_evict(p, c->n_sms, c->stream));
-    c->launches += 1;
+    for (int b0 = 0; b0 < a->n_seqs; b0 += (int)per_launch) {
+        EvictParams q = p;
+        q.B = a->n_seqs - b0 < per_launch ? a->n_seqs - b0 : (int)per_launch;
+        q.k += (int64_t)b0 * p.seq_stride;
+        q.v += (int64_t)b0 * p.seq_stride;
+        q.lens += b0;
+        q.next_pos += b0;
+        q.lens_out += b0;
+        q.w += (int64_t)b0 * p.map_seq;
+        q.pos += (int64_t)b0 * p.map_seq;
+        q.w_out += (int64_t)b0 * p.map_seq;
+        q.pos_out += (int64_t)b0 * p.map_seq;
+        int launches = 0;
+        CK(launch_kv_evict(q, c->n_sms, c->stream, &launches));
+        c->launches += launches;
+    }
     return 0;
 } catch (...) {
     return -1;

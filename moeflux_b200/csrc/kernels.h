@@ -306,9 +306,14 @@ struct EvictParams {
     int32_t *pos_out, *lens_out;
     unsigned *status;
     int B, Hkv, cap, budget, n_sink, n_recent;
+    int2 *moves;    // scratch [units][max_moves]: (destination, source) rows
+    int *counts;    // scratch [units]: moves of a unit
+    int max_moves;  // most moves of a unit: min(budget, cap - budget), at least 1
+    int fused;      // filled by the launcher: the selecting CTA copies the rows itself
 };
+constexpr int EVICT_MAX_UNITS = 8192;  // (sequence, kv head) units of one launch
 cudaError_t kv_evict_configure();
-cudaError_t launch_kv_evict(const EvictParams &p, int n_sms, cudaStream_t stream);
+cudaError_t launch_kv_evict(EvictParams p, int n_sms, cudaStream_t stream, int *launches);
 
 struct AttnWeightsParams {
     const __nv_bfloat16 *q, *k;

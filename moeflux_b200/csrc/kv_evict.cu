@@ -8,12 +8,13 @@
 // over its budget moves a few rows, where an order-preserving compaction would move half the cache).  Sources lie at or
 // beyond the budget and destinations below it, so the moves need no order among themselves.
 //
-// HBM-bound for large caches: 8 bytes per row for the selection, 4 KiB (bf16: 2 KiB) per moved row; a small one is bound
-// by the latency of the selection's steps.  A cluster of CTAs owns a unit; each holds the keys of a contiguous run of
-// rows in shared memory, so weights and positions are read once.  The border key is found by a radix selection
-// (11 + 11 + 10 bits) whose histograms are summed through distributed shared memory.  A warp walks its rows 32 at a time:
-// ballots give the ranks of ties, and the holes and movers it finds go to a list of its own, in shared memory; the moves
-// are dealt over all warps of the cluster, which find move j by a search over the lists' lengths.
+// Two kernels.  The selection is bound by latency (8 bytes per row, then some ten dependent steps): a cluster of CTAs owns
+// a unit, each holds the keys of a contiguous run of rows in shared memory; the border key is found by a radix selection
+// (11 + 11 + 10 bits) whose histograms are summed through distributed shared memory; a warp walks its rows 32 at a time,
+// ballots give the ranks of ties, holes and movers, and the pairs (destination, source) go to a list in device memory.
+// The copy is bound by HBM (4 KiB per moved row, bf16: 2 KiB): all moves of all units are dealt evenly over all SMs,
+// whatever the units' sizes (with the copies in the selecting CTAs, 8 sequences of 7 to 20 thousand rows took twice as
+// long).  A small call -- EV_FUSED_ROWS rows per unit at most -- copies in the selecting CTA and saves the second launch.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -25,13 +26,16 @@ namespace mfc {
 
 namespace {
 
-constexpr int EV_THREADS = 512;
+constexpr int EV_THREADS = 1024;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;
 constexpr int EV_MAX_CLUSTER = 16;
-constexpr int EV_MOVES = 8;
-constexpr int EV_MIN_ROWS = 2048;
-constexpr int EV_MAX_ROWS_PER_CTA = 16384;  // 8 bytes of shared memory each: 128 KiB
+constexpr int EV_MAX_ROWS_PER_CTA = 16384;  // 4 bytes of shared memory each: 64 KiB
+constexpr int EV_MIN_ROWS = 2048;           // rows per CTA below which a cluster does not grow
+constexpr int EV_FUSED_ROWS = 2048;
+constexpr int EV_LISTS = EV_MAX_CLUSTER * EV_WARPS;  // warps of a unit
+static_assert(EV_LISTS <= EV_THREADS, "one thread per warp of a unit");
+static_assert(EV_BINS / 4 <= EV_THREADS, "four bins per thread");
 
 __device__ __forceinline__ uint32_t weight_key(float w, bool safe) {
     if (safe) return 0xffffffffu;
@@ -42,7 +46,7 @@ __device__ __forceinline__ uint32_t weight_key(float w, bool safe) {
 
 // Exclusive prefix sum of v over the block's threads; *total: the sum.  Contains two __syncthreads.
 __device__ __forceinline__ int block_scan(int v, int *s_warp, int *total) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     int inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -51,58 +55,69 @@ __device__ __forceinline__ int block_scan(int v, int *s_warp, int *total) {
     }
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    int base = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < EV_WARPS; w++) {
-        const int t = s_warp[w];
-        if (w < warp) base += t;
-        sum += t;
-    }
+    const int mine = lane < warps ? s_warp[lane] : 0;  // at most 32 warps
+    const int base = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    *total = __reduce_add_sync(0xffffffffu, mine);
     __syncthreads();
-    *total = sum;
     return base + inc - v;
 }
 
-constexpr int EV_LISTS = EV_MAX_CLUSTER * EV_WARPS;  // lists of a unit, one per warp
-static_assert(EV_LISTS <= EV_THREADS, "one thread per list");
+// Copies the rows of `cnt` <= MOVES moves, both tensors; lane u < MOVES holds move u as (destination, source) rows.
+template <int MOVES>
+__device__ __forceinline__ void copy_rows(const EvictParams &p, size_t base, int2 move, int cnt) {
+    const int lane = threadIdx.x & 31;
+    const int vecs = p.row_bytes >> 4;  // 16-byte pieces of a row: 32 or 64
+    for (int v = lane; v < vecs; v += 32) {
+        uint4 kx[MOVES], vx[MOVES];
+#pragma unroll
+        for (int u = 0; u < MOVES; u++) {
+            const size_t so = base + (size_t)__shfl_sync(0xffffffffu, move.y, u) * p.row_stride + (size_t)v * 16;
+            if (u < cnt) {
+                kx[u] = *reinterpret_cast<const uint4 *>(p.k + so);
+                vx[u] = *reinterpret_cast<const uint4 *>(p.v + so);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < MOVES; u++) {
+            const size_t dof = base + (size_t)__shfl_sync(0xffffffffu, move.x, u) * p.row_stride + (size_t)v * 16;
+            if (u < cnt) {
+                *reinterpret_cast<uint4 *>(p.k + dof) = kx[u];
+                *reinterpret_cast<uint4 *>(p.v + dof) = vx[u];
+            }
+        }
+    }
+}
 
 struct EvShared {
     uint4 hist[3][EV_BINS / 4];
     int warp_sum[EV_WARPS];
-    int holes[EV_WARPS], movers[EV_WARPS];          // of this CTA's warps, for its peers
-    int hole0[EV_LISTS + 1], mover0[EV_LISTS + 1];  // first hole / mover of every list of the unit
-    int digit, above;                               // result of a selection pass
+    int ties[EV_WARPS];
+    int holes[EV_WARPS], movers[EV_WARPS];      // of this CTA's warps, for its peers
+    int hole0[EV_LISTS], mover0[EV_LISTS];      // rank of the first hole / mover of every warp of the unit
+    int digit, above;                           // result of a selection pass
 };
 
-// the list that holds element j: the largest l with first[l] <= j
-__device__ __forceinline__ int find_list(const int *first, int lists, int j) {
-    int lo = 0, hi = lists - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (first[mid] <= j) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
-__global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictParams p, int rows_cap) {
-    extern __shared__ uint32_t dyn[];  // [rows_cap] keys; [rows_cap] lists: a warp's range holds its holes from the front,
-                                       // its movers from the back
+__global__ void __launch_bounds__(EV_THREADS, 1) kv_evict_select_kernel(const EvictParams p) {
+    extern __shared__ uint32_t keys[];
     __shared__ EvShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int unit = (int)blockIdx.x / cs;
     const int b = unit / p.Hkv, h = unit % p.Hkv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint32_t *keys = dyn, *list = dyn + rows_cap;
 
+    for (int i = tid; i < 3 * EV_BINS / 4; i += EV_THREADS) (&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
     int n = p.lens[b];
+    const long long recent = (long long)p.next_pos[b] - p.n_recent;
     if (n < 0 || n > p.cap) {
         if (rank == 0 && h == 0 && tid == 0) atomicOr(p.status, STATUS_BAD_ITEM);
         n = 0;
     }
     const int kept_n = min(n, p.budget);
-    if (rank == 0 && h == 0 && tid == 0) p.lens_out[b] = kept_n;
+    if (rank == 0 && tid == 0) {
+        if (h == 0) p.lens_out[b] = kept_n;
+        if (n <= p.budget) p.counts[unit] = 0;
+    }
     const size_t m0 = (size_t)b * p.map_seq + (size_t)h * p.map_head;
     const float *w = p.w + m0;
     const int32_t *pos = p.pos + m0;
@@ -112,24 +127,34 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictParams 
     // this CTA's run of rows
     const int chunk = (n + cs - 1) / cs;
     const int r0 = min(rank * chunk, n), r1 = min(r0 + chunk, n), rows = r1 - r0;
-
-    if (n <= p.budget) {  // nothing to evict (the same decision in every CTA of the cluster)
-        for (int i = r0 + tid; i < r1; i += EV_THREADS) {
-            w_out[i] = w[i];
-            pos_out[i] = pos[i];
-        }
-        return;
-    }
-
-    for (int i = tid; i < 3 * EV_BINS / 4; i += EV_THREADS) (&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
-    const long long recent = (long long)p.next_pos[b] - p.n_recent;
+    const bool all = n <= p.budget;  // nothing to evict (the same decision in every CTA of the cluster)
     __syncthreads();
-    for (int i = tid; i < rows; i += EV_THREADS) {
-        const int ps = pos[r0 + i];
-        const uint32_t k = weight_key(w[r0 + i], ps < p.n_sink || ps >= recent);
-        keys[i] = k;
-        atomicAdd(reinterpret_cast<unsigned *>(sh.hist[0]) + (k >> 21), 1u);
+    // keys, and the rows below the budget as if none were evicted (the moves overwrite the holes)
+    for (int i0 = tid; i0 < rows; i0 += 4 * EV_THREADS) {
+        float wv[4];
+        int ps[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int i = i0 + u * EV_THREADS;
+            wv[u] = i < rows ? w[r0 + i] : 0.0f;
+            ps[u] = i < rows ? pos[r0 + i] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int i = i0 + u * EV_THREADS;
+            if (i >= rows) break;
+            if (r0 + i < kept_n) {
+                if (w_out != w) w_out[r0 + i] = wv[u];
+                if (pos_out != pos) pos_out[r0 + i] = ps[u];
+            }
+            if (!all) {
+                const uint32_t k = weight_key(wv[u], ps[u] < p.n_sink || ps[u] >= recent);
+                keys[i] = k;
+                atomicAdd(reinterpret_cast<unsigned *>(sh.hist[0]) + (k >> 21), 1u);
+            }
+        }
     }
+    if (all) return;
 
     // radix selection: after pass k the leading digits of the border key are known, and how many kept rows share them
     uint32_t border = 0;
@@ -145,11 +170,13 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictParams 
                 if ((k >> known) == (border >> known)) atomicAdd(reinterpret_cast<unsigned *>(sh.hist[ps]) + ((k >> shift) & (bins - 1)), 1u);
             }
         }
-        cluster.sync();
+        if (cs > 1) cluster.sync();
+        else __syncthreads();
         // every CTA sums the histograms of all; thread t owns the four bins below bins - 4t, from the largest down
         const int quad = bins / 4 - 1 - tid;
         uint4 c = make_uint4(0u, 0u, 0u, 0u);
         if (quad >= 0)
+#pragma unroll 4
             for (int r = 0; r < cs; r++) {
                 const uint4 h4 = *cluster.map_shared_rank(&sh.hist[ps][quad], r);
                 c.x += h4.x;
@@ -174,8 +201,8 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictParams 
         __syncthreads();
     }
     // rows whose key equals the border: the `need` lowest ones are kept; those of the CTAs before this one come first
-    int tie = 0;
-    for (int r = 0; r < rank; r++) tie += (int)*(cluster.map_shared_rank(reinterpret_cast<unsigned *>(sh.hist[2]), r) + (border & 1023u));
+    int tie0 = 0;
+    for (int r = 0; r < rank; r++) tie0 += (int)*(cluster.map_shared_rank(reinterpret_cast<unsigned *>(sh.hist[2]), r) + (border & 1023u));
 
     // warp w owns the rows [w0, w1) of the run
     const int per = ((rows + EV_WARPS - 1) / EV_WARPS + 31) & ~31;
@@ -184,113 +211,148 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictParams 
     int ties = 0;
     for (int i = w0 + lane; i < w1; i += 32) ties += keys[i] == border;
     ties = __reduce_add_sync(0xffffffffu, ties);
-    if (lane == 0) sh.warp_sum[warp] = ties;
+    if (lane == 0) sh.ties[warp] = ties;
     __syncthreads();
-    for (int k = 0; k < warp; k++) tie += sh.warp_sum[k];
-    int holes = 0, movers = 0;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const int i = i0 + lane, r = r0 + i;
+    tie0 += __reduce_add_sync(0xffffffffu, lane < warp ? sh.ties[lane] : 0);
+    // the 32 rows from i0 on: which are holes, which movers
+    auto classify = [&](int i0, int &tie, unsigned &holes, unsigned &movers) {
+        const int i = i0 + lane;
         const bool in = i < w1;
         const uint32_t k = in ? keys[i] : 0u;
         const bool eq = in && k == border;
         const unsigned eqs = __ballot_sync(0xffffffffu, eq);
         const bool kept = in && (k > border || (eq && tie + __popc(eqs & below) < need));
-        const bool hole = in && !kept && r < p.budget, mover = kept && r >= p.budget;
-        const unsigned hs = __ballot_sync(0xffffffffu, hole), ms = __ballot_sync(0xffffffffu, mover);
-        if (hole) list[w0 + holes + __popc(hs & below)] = (uint32_t)r;
-        if (mover) list[w1 - 1 - movers - __popc(ms & below)] = (uint32_t)r;
-        if (kept && !mover) {  // stays where it is
-            if (w_out != w) w_out[r] = w[r];
-            if (pos_out != pos) pos_out[r] = pos[r];
-        }
+        holes = __ballot_sync(0xffffffffu, in && !kept && r0 + i < p.budget);
+        movers = __ballot_sync(0xffffffffu, kept && r0 + i >= p.budget);
         tie += __popc(eqs);
-        holes += __popc(hs);
-        movers += __popc(ms);
+    };
+    int n_holes = 0, n_movers = 0, tie = tie0;
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+        unsigned hs, ms;
+        classify(i0, tie, hs, ms);
+        n_holes += __popc(hs);
+        n_movers += __popc(ms);
     }
     if (lane == 0) {
-        sh.holes[warp] = holes;
-        sh.movers[warp] = movers;
+        sh.holes[warp] = n_holes;
+        sh.movers[warp] = n_movers;
     }
-    cluster.sync();
-
-    // every CTA learns where each list of the unit starts
-    const int lists = cs * EV_WARPS;
-    int moves, all_movers;
+    if (cs > 1) cluster.sync();
+    else __syncthreads();
+    // ranks of every warp's first hole and mover within the unit
+    int moves;
     {
+        const int lists = cs * EV_WARPS;
         const int r = tid / EV_WARPS, k = tid % EV_WARPS;
         const int nh = tid < lists ? *cluster.map_shared_rank(&sh.holes[k], r) : 0, nm = tid < lists ? *cluster.map_shared_rank(&sh.movers[k], r) : 0;
-        const int h0 = block_scan(nh, sh.warp_sum, &moves), q0 = block_scan(nm, sh.warp_sum, &all_movers);
+        int same;  // holes and movers are equally many
+        const int h0 = block_scan(nh, sh.warp_sum, &moves), q0 = block_scan(nm, sh.warp_sum, &same);
         if (tid < lists) {
             sh.hole0[tid] = h0;
             sh.mover0[tid] = q0;
         }
         __syncthreads();
     }
-    // row of the j-th hole / mover
-    auto pick = [&](int j, bool want_hole) -> int {
-        const int l = find_list(want_hole ? sh.hole0 : sh.mover0, lists, j);
-        const int r = l / EV_WARPS, k = l % EV_WARPS;
-        const int rr = max(0, min((r + 1) * chunk, n) - min(r * chunk, n));  // rows of that CTA, its warp's range
-        const int pw = ((rr + EV_WARPS - 1) / EV_WARPS + 31) & ~31;
-        const int a = min(k * pw, rr), z = min(a + pw, rr);
-        return (int)*cluster.map_shared_rank(&list[want_hole ? a + (j - sh.hole0[l]) : z - 1 - (j - sh.mover0[l])], r);
-    };
-    const size_t base = (size_t)b * p.seq_stride + (size_t)h * p.head_stride;
-    const int vecs = p.row_bytes >> 4;  // 16-byte pieces of a row: 32 or 64
-    const int warps = cs * EV_WARPS;
-    // EV_MOVES moves a turn, both tensors: EV_MOVES * 32 bytes of each lane's loads in flight together
-    for (int j0 = (rank * EV_WARPS + warp) * EV_MOVES; j0 < moves; j0 += warps * EV_MOVES) {
-        const int cnt = min(EV_MOVES, moves - j0);
-        int row = 0;  // lane u: destination of move u; lane EV_MOVES + u: its source
-        if ((lane & (EV_MOVES - 1)) < cnt && lane < 2 * EV_MOVES) row = pick(j0 + (lane & (EV_MOVES - 1)), lane < EV_MOVES);
-        const int src_row = __shfl_down_sync(0xffffffffu, row, EV_MOVES);
-        if (lane < cnt) {
-            w_out[row] = w[src_row];
-            pos_out[row] = pos[src_row];
-        }
-        for (int v = lane; v < vecs; v += 32) {
-            uint4 kx[EV_MOVES], vx[EV_MOVES];
-#pragma unroll
-            for (int u = 0; u < EV_MOVES; u++) {
-                const size_t so = base + (size_t)__shfl_sync(0xffffffffu, row, EV_MOVES + u) * p.row_stride + (size_t)v * 16;
-                if (u < cnt) {
-                    kx[u] = *reinterpret_cast<const uint4 *>(p.k + so);
-                    vx[u] = *reinterpret_cast<const uint4 *>(p.v + so);
-                }
+    int2 *list = p.moves + (size_t)unit * p.max_moves;
+    int hole = sh.hole0[rank * EV_WARPS + warp], mover = sh.mover0[rank * EV_WARPS + warp];
+    tie = tie0;
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+        unsigned hs, ms;
+        classify(i0, tie, hs, ms);
+        if (hs >> lane & 1u) list[hole + __popc(hs & below)].x = r0 + i0 + lane;
+        if (ms >> lane & 1u) list[mover + __popc(ms & below)].y = r0 + i0 + lane;
+        hole += __popc(hs);
+        mover += __popc(ms);
+    }
+    if (rank == 0 && tid == 0) p.counts[unit] = moves;
+    if (cs > 1) {
+        cluster.sync();  // a CTA's counts stay until its peers have read them
+    } else if (p.fused) {
+        __syncthreads();
+        const size_t base = (size_t)b * p.seq_stride + (size_t)h * p.head_stride;
+        for (int j0 = warp * 2; j0 < moves; j0 += EV_WARPS * 2) {
+            const int cnt = min(2, moves - j0);
+            int2 mv = make_int2(0, 0);
+            if (lane < cnt) {
+                mv = list[j0 + lane];
+                w_out[mv.x] = w[mv.y];
+                pos_out[mv.x] = pos[mv.y];
             }
-#pragma unroll
-            for (int u = 0; u < EV_MOVES; u++) {
-                const size_t dof = base + (size_t)__shfl_sync(0xffffffffu, row, u) * p.row_stride + (size_t)v * 16;
-                if (u < cnt) {
-                    *reinterpret_cast<uint4 *>(p.k + dof) = kx[u];
-                    *reinterpret_cast<uint4 *>(p.v + dof) = vx[u];
-                }
-            }
+            copy_rows<2>(p, base, mv, cnt);
         }
     }
-    cluster.sync();  // a CTA's lists stay until its peers have read them
+}
+
+// The moves of all units, dealt evenly: CTA c takes the c-th of equal runs of the units' lists laid end to end.
+constexpr int EC_THREADS = 256;
+constexpr int EC_MOVES = 4;  // a warp's moves a turn: 8 rows in flight, 64 bytes of each lane's loads per tensor
+__global__ void __launch_bounds__(EC_THREADS) kv_evict_copy_kernel(const EvictParams p) {
+    extern __shared__ int first[];  // [units + 1] first move of every unit
+    __shared__ int s_warp[EC_THREADS / 32];
+    const int units = p.B * p.Hkv, tid = threadIdx.x, lane = tid & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the lists are written by the kernel before
+    const int per = (units + EC_THREADS - 1) / EC_THREADS;
+    const int u0 = min(tid * per, units), u1 = min(u0 + per, units);
+    int sum = 0, total;
+    for (int u = u0; u < u1; u++) sum += p.counts[u];
+    int at = block_scan(sum, s_warp, &total);
+    for (int u = u0; u < u1; u++) {
+        first[u] = at;
+        at += p.counts[u];
+    }
+    if (tid == 0) first[units] = total;
+    __syncthreads();
+    const int run = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int j1 = min(((int)blockIdx.x + 1) * run, total);
+    for (int j = (int)blockIdx.x * run + (tid >> 5) * EC_MOVES; j < j1; j += EC_THREADS / 32 * EC_MOVES) {
+        int lo = 0, hi = units - 1;  // the unit that holds move j
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first[mid] <= j) lo = mid;
+            else hi = mid - 1;
+        }
+        // a turn's moves may reach into the next units: one unit at a time
+        for (int a = j, z = min(j + EC_MOVES, j1); a < z;) {
+            while (first[lo + 1] <= a) lo++;
+            const int cnt = min(z, first[lo + 1]) - a;
+            const int b = lo / p.Hkv, h = lo % p.Hkv;
+            int2 mv = make_int2(0, 0);
+            if (lane < cnt) {
+                mv = p.moves[(size_t)lo * p.max_moves + (a - first[lo]) + lane];
+                const size_t m0 = (size_t)b * p.map_seq + (size_t)h * p.map_head;
+                p.w_out[m0 + mv.x] = p.w[m0 + mv.y];
+                p.pos_out[m0 + mv.x] = p.pos[m0 + mv.y];
+            }
+            copy_rows<EC_MOVES>(p, (size_t)b * p.seq_stride + (size_t)h * p.head_stride, mv, cnt);
+            a += cnt;
+        }
+    }
 }
 
 }  // namespace
 
 cudaError_t kv_evict_configure() {
-    cudaError_t e = cudaFuncSetAttribute(kv_evict_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = cudaFuncSetAttribute(kv_evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(kv_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MAX_ROWS_PER_CTA * 8);
+    e = cudaFuncSetAttribute(kv_evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MAX_ROWS_PER_CTA * 4);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(kv_evict_copy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (EVICT_MAX_UNITS + 1) * 4);
 }
 
-cudaError_t launch_kv_evict(const EvictParams &p, int n_sms, cudaStream_t stream) {
+cudaError_t launch_kv_evict(EvictParams p, int n_sms, cudaStream_t stream, int *launches) {
     const int units = p.B * p.Hkv;
+    *launches = 0;
     if (units <= 0) return cudaSuccess;
-    // As many CTAs per unit as keep every SM busy twice, but at least EV_MIN_ROWS rows each: a small unit is over sooner
-    // without the exchanges through distributed shared memory.
+    // As many CTAs per unit as there are SMs for, but at least EV_MIN_ROWS rows each: a small unit is over sooner without
+    // the exchanges through distributed shared memory (1088 rows: 14.7 us in one CTA, 18.9 in eight).
     int cs = 1;
-    while (cs < EV_MAX_CLUSTER && ((int64_t)units * cs < 2 * n_sms || p.cap > cs * EV_MAX_ROWS_PER_CTA) && p.cap > cs * EV_MIN_ROWS) cs *= 2;
+    while (cs < EV_MAX_CLUSTER && ((int64_t)units * cs * 2 <= n_sms || p.cap > cs * EV_MAX_ROWS_PER_CTA) && p.cap > cs * EV_MIN_ROWS) cs *= 2;
+    p.fused = cs == 1 && p.cap <= EV_FUSED_ROWS;
     const int rows_cap = (p.cap + cs - 1) / cs;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * cs));
     cfg.blockDim = dim3(EV_THREADS);
-    cfg.dynamicSmemBytes = (size_t)rows_cap * 8;
+    cfg.dynamicSmemBytes = (size_t)rows_cap * 4;
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -298,7 +360,23 @@ cudaError_t launch_kv_evict(const EvictParams &p, int n_sms, cudaStream_t stream
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_evict_kernel, p, rows_cap);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kv_evict_select_kernel, p);
+    if (e != cudaSuccess) return e;
+    *launches = 1;
+    if (p.fused) return cudaSuccess;
+    cudaLaunchConfig_t cc = {};
+    cc.gridDim = dim3((unsigned)(n_sms * 4));
+    cc.blockDim = dim3(EC_THREADS);
+    cc.dynamicSmemBytes = (size_t)(units + 1) * 4;
+    cc.stream = stream;
+    cudaLaunchAttribute pd[1];
+    pd[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pd[0].val.programmaticStreamSerializationAllowed = 1;
+    cc.attrs = pd;
+    cc.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cc, kv_evict_copy_kernel, p);
+    if (e == cudaSuccess) *launches = 2;
+    return e;
 }
 
 }  // namespace mfc

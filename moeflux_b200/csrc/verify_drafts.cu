@@ -12,6 +12,7 @@
 // the one that owns it re-reads the 1024 entries of that segment (from L2).  Order of all sums fixed by the sizes.
 #include <cooperative_groups.h>
 
+#include <stdlib.h>
 #include "common.cuh"
 #include "kernels.h"
 
@@ -21,7 +22,7 @@ namespace mfc {
 
 namespace {
 
-constexpr int VD_THREADS = 256;
+constexpr int VD_THREADS = 128;
 constexpr int VD_WARPS = VD_THREADS / 32;
 constexpr int VD_SEG = 1024;     // entries of a segment
 constexpr int VD_MAX_SEGS = 512;  // segments of a CTA's run kept in shared memory; longer runs use longer segments
@@ -67,8 +68,22 @@ __device__ __forceinline__ void sum_segments(const float *p, const float *q, int
     for (int s = s0 + warp; s < s1; s += VD_WARPS) {
         const int v1 = min((s + 1) * seg, V);
         double acc = 0.0;
-#pragma unroll 8
-        for (int v = s * seg + 4 * lane; v < v1; v += 128) {
+        int v0 = s * seg;
+        if (VEC && x < 0) {  // whole steps of 512 entries: eight loads of a lane in flight
+            for (; v0 + 512 <= v1; v0 += 512) {
+                float4 a[4], b[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) a[u] = *reinterpret_cast<const float4 *>(p + v0 + 4 * lane + 128 * u);
+#pragma unroll
+                for (int u = 0; u < 4; u++) b[u] = q ? *reinterpret_cast<const float4 *>(q + v0 + 4 * lane + 128 * u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                double t[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    t[u] = (weight(a[u].x, b[u].x) + weight(a[u].y, b[u].y)) + (weight(a[u].z, b[u].z) + weight(a[u].w, b[u].w));
+                acc += (t[0] + t[1]) + (t[2] + t[3]);
+            }
+        }
+        for (int v = v0 + 4 * lane; v < v1; v += 128) {
             double w[4];
             load_w4<VEC>(p, q, x, v, V, w);
             acc += (w[0] + w[1]) + (w[2] + w[3]);
@@ -208,6 +223,7 @@ cudaError_t launch_verify_drafts(const VerifyParams &p, int n_sms, cudaStream_t 
     // CTAs per sequence: up to eight a SM in all, but at least two segments each
     int cs = 1;
     while (cs < VD_MAX_CLUSTER && p.B * cs < 8 * n_sms && (int64_t)p.V > (int64_t)cs * 2 * VD_SEG) cs *= 2;
+    if (getenv("VDCS")) cs = atoi(getenv("VDCS"));
     int64_t seg = VD_SEG;  // longer segments where a run would not fit the table of sums
     while ((p.V + seg - 1) / seg > (int64_t)cs * VD_MAX_SEGS) seg *= 2;
     cudaLaunchConfig_t cfg = {};
