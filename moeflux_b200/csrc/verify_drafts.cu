@@ -12,7 +12,6 @@
 // the one that owns it re-reads the 1024 entries of that segment (from L2).  Order of all sums fixed by the sizes.
 #include <cooperative_groups.h>
 
-#include <stdlib.h>
 #include "common.cuh"
 #include "kernels.h"
 
@@ -36,6 +35,17 @@ __device__ __forceinline__ double weight(float p, float q) {
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// inclusive prefix sum over the lanes
+__device__ __forceinline__ double warp_scan_f64(double v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+    }
     return v;
 }
 
@@ -105,8 +115,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
     const int len = p.draft_lens ? min(p.draft_lens[b], p.K) : p.K;
     if (warp == 0) {
         bool refused = false;
+        // (the drafted tokens are asked for beside the length, not behind it)
+        const int x = lane < p.K ? p.drafts[(size_t)b * p.K + lane] : -1;
         if (lane < len) {
-            const int x = p.drafts[(size_t)b * p.K + lane];
             refused = true;
             if (x >= 0 && x < p.V) {
                 const float px = p.p[(size_t)b * p.p_seq + (size_t)lane * p.p_row + x];
@@ -140,10 +151,11 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
         if (vec) sum_segments<true>(prow, qrow, x, p.V, seg, s0, s1, s_sum);
         else sum_segments<false>(prow, qrow, x, p.V, seg, s0, s1, s_sum);
         __syncthreads();
-        if (tid == 0) {
+        if (warp == 0) {
             double t = 0.0;
-            for (int s = 0; s < s1 - s0; s++) t += s_sum[s];
-            s_tot[pass] = t;
+            for (int s = lane; s < s1 - s0; s += 32) t += s_sum[s];
+            t = warp_sum_f64(t);
+            if (lane == 0) s_tot[pass] = t;
         }
         cluster.sync();
         total = before = 0.0;
@@ -167,46 +179,79 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
         // it does; the additions are those every CTA makes, so exactly one run qualifies
         const bool here = before <= target && before + mine > target;
         if (here) {
-            double c = before;
-            int s = s0;
-            for (; s < s1 - 1; s++) {
-                if (c + s_sum[s - s0] > target) break;
-                c += s_sum[s - s0];
-            }
-            // the segment, 128 entries a step: a prefix sum over the lanes' groups of four
-            int found = -1, last = -1;
-            const int v1 = min((s + 1) * seg, p.V);
-            for (int v0 = s * seg; v0 < v1 && found < 0; v0 += 128) {
-                double w[4];
-                if (vec) load_w4<true>(prow, qrow, x, v0 + 4 * lane, p.V, w);
-                else load_w4<false>(prow, qrow, x, v0 + 4 * lane, p.V, w);
-                double inc[4];
-                inc[0] = w[0];
-                inc[1] = inc[0] + w[1];
-                inc[2] = inc[1] + w[2];
-                inc[3] = inc[2] + w[3];
-                double run = inc[3];
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double up = __shfl_up_sync(0xffffffffu, run, o);
-                    if (lane >= o) run += up;
+            // Three levels, each a sum over lanes: the segment, the step of 128 entries in it, the entry.  Sums of the same
+            // entries in two orders may differ in the last bit; where a level then finds no place, its last one counts.
+            // (Entries without weight are never the last one.)
+            double c = before, c_last = before;
+            int s = -1, s_last = s0;
+            for (int k0 = s0; k0 < s1 && s < 0; k0 += 32) {
+                const double v = k0 + lane < s1 ? s_sum[k0 + lane - s0] : 0.0;
+                const double run = warp_scan_f64(v);
+                const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && c + run > target), any = __ballot_sync(0xffffffffu, v > 0.0);
+                const int l = over ? __ffs(over) - 1 : (any ? 31 - __clz(any) : -1);
+                if (l >= 0) {
+                    const double ahead = c + __shfl_sync(0xffffffffu, run - v, l);
+                    if (over) {
+                        s = k0 + l;
+                        c = ahead;
+                        break;
+                    }
+                    s_last = k0 + l;
+                    c_last = ahead;
                 }
-                const double lead = c + (run - inc[3]);
-                int mine_at = 0x7fffffff, mine_last = -1;
-#pragma unroll
-                for (int e = 3; e >= 0; e--) {
-                    if (w[e] > 0.0 && lead + inc[e] > target) mine_at = v0 + 4 * lane + e;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (w[e] > 0.0) mine_last = v0 + 4 * lane + e;
-                const int first = __reduce_min_sync(0xffffffffu, mine_at);
-                last = max(last, __reduce_max_sync(0xffffffffu, mine_last));
-                if (first != 0x7fffffff) found = first;
                 c += __shfl_sync(0xffffffffu, run, 31);
             }
-            // (the sums of a segment in two orders may differ in the last bit: then its last entry of any weight)
-            if (lane == 0) *tok = found >= 0 ? found : last;
+            if (s < 0) {
+                s = s_last;
+                c = c_last;
+            }
+            auto load4 = [&](int v, double (&w)[4]) {
+                if (vec) load_w4<true>(prow, qrow, x, v, p.V, w);
+                else load_w4<false>(prow, qrow, x, v, p.V, w);
+            };
+            const int v1 = min((s + 1) * seg, p.V);
+            int step = -1, step_last = s * seg;
+            c_last = c;
+            for (int v0 = s * seg; v0 < v1 && step < 0; v0 += 8 * 128) {
+                double part[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    double w[4] = {0.0, 0.0, 0.0, 0.0};
+                    if (v0 + 128 * u < v1) load4(v0 + 128 * u + 4 * lane, w);
+                    part[u] = (w[0] + w[1]) + (w[2] + w[3]);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; u++) part[u] = warp_sum_f64(part[u]);
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    if (step >= 0 || !(part[u] > 0.0)) continue;
+                    if (c + part[u] > target) {
+                        step = v0 + 128 * u;
+                    } else {
+                        step_last = v0 + 128 * u;
+                        c_last = c;
+                        c += part[u];
+                    }
+                }
+            }
+            if (step < 0) {
+                step = step_last;
+                c = c_last;
+            }
+            double w[4];
+            load4(step + 4 * lane, w);
+            const double i0 = w[0], i1 = i0 + w[1], i2 = i1 + w[2], i3 = i2 + w[3];
+            const double lead = c + (warp_scan_f64(i3) - i3);
+            int at = 0x7fffffff, end = -1;
+            if (w[3] > 0.0 && lead + i3 > target) at = step + 4 * lane + 3;
+            if (w[2] > 0.0 && lead + i2 > target) at = step + 4 * lane + 2;
+            if (w[1] > 0.0 && lead + i1 > target) at = step + 4 * lane + 1;
+            if (w[0] > 0.0 && lead + i0 > target) at = step + 4 * lane;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (w[e] > 0.0) end = step + 4 * lane + e;
+            const int first = __reduce_min_sync(0xffffffffu, at), fin = __reduce_max_sync(0xffffffffu, end);
+            if (lane == 0) *tok = first != 0x7fffffff ? first : fin;
         }
     }
     cluster.sync();  // a CTA's shared memory stays until its peers have read it
@@ -220,10 +265,10 @@ cudaError_t verify_drafts_configure() {
 
 cudaError_t launch_verify_drafts(const VerifyParams &p, int n_sms, cudaStream_t stream) {
     if (p.B <= 0) return cudaSuccess;
-    // CTAs per sequence: up to eight a SM in all, but at least two segments each
+    // As many CTAs per sequence as are resident at once (seven a SM), but at least two segments each.  128 sequences of
+    // 131072 entries: 134, 74, 46, 32, 38 us with 1, 2, 4, 8, 16.
     int cs = 1;
-    while (cs < VD_MAX_CLUSTER && p.B * cs < 8 * n_sms && (int64_t)p.V > (int64_t)cs * 2 * VD_SEG) cs *= 2;
-    if (getenv("VDCS")) cs = atoi(getenv("VDCS"));
+    while (cs < VD_MAX_CLUSTER && (int64_t)p.B * cs * 2 <= 7 * n_sms && (int64_t)p.V > (int64_t)cs * 2 * VD_SEG) cs *= 2;
     int64_t seg = VD_SEG;  // longer segments where a run would not fit the table of sums
     while ((p.V + seg - 1) / seg > (int64_t)cs * VD_MAX_SEGS) seg *= 2;
     cudaLaunchConfig_t cfg = {};
