@@ -1679,8 +1679,14 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *c, const mfc_attn_weights *a) try {
     p.cap = a->cap;
     p.scale = a->softmax_scale;
     p.decay = a->decay;
+    if ((int64_t)p.B * p.Hkv * ((p.cap + 127) / 128) >= ((int64_t)1 << 30)) {
+        fail(c, "too many rows in one call");
+        return -1;
+    }
+    CUtensorMap k_map;
+    if (!make_rows_map(c, &k_map, a->k, a->cap, a->k_row_stride, p.Hkv, a->k_head_stride, p.B, a->k_seq_stride, 2, 128)) return -1;
     DeviceScope dev(c->cfg.device);
-    CK(launch_attn_weights(p, c->n_sms, c->stream));
+    CK(launch_attn_weights(k_map, p, c->n_sms, c->stream));
     c->launches += 1;
     return 0;
 } catch (...) {

@@ -327,7 +327,8 @@ struct AttnWeightsParams {
     float scale, decay;
 };
 cudaError_t attn_weights_configure();
-cudaError_t launch_attn_weights(const AttnWeightsParams &p, int n_sms, cudaStream_t stream);
+// k_map: over the cached K rows as for the attention call (boxes of two fourths x 128 rows)
+cudaError_t launch_attn_weights(const CUtensorMap &k_map, const AttnWeightsParams &p, int n_sms, cudaStream_t stream);
 
 constexpr int SHARED_ATTN_MAX_SEQS = 4096;
 constexpr int SHARED_ATTN_PLAN_INTS = SHARED_ATTN_MAX_SEQS + 8;

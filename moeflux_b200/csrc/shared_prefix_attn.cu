@@ -56,13 +56,6 @@ constexpr float LOG2E_SP = 1.4426950408889634f;
 constexpr uint32_t SP_TMEM_COLS = 512;
 constexpr uint32_t TM_O = 0, TM_S = 256, TM_P = 384;       // P: two buffers of 64 columns
 
-__device__ __forceinline__ void tma_load_5d(void *smem_dst, const void *tmap, int c0, int c1, int c2, int c3, int c4, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
-        "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
-        : "memory");
-}
 // D[tmem] (+)= A[tmem] * B[smem desc], bf16 inputs, fp32 accumulate; A: lane = row, one 32-bit column = two k
 __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                                uint32_t accumulate) {

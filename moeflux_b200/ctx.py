@@ -12,7 +12,7 @@ from typing import Optional, Sequence
 
 import numpy as np
 
-from ._lib import (AttnWeights, Config, KvEvict, MfcError, SharedPrefixAttn, VerifyDrafts, lib, KV_F32,
+from ._lib import (AttnWeights, Config, KvEvict, MfcError, SharedPrefixAttn, VerifyDrafts, lib, packer, KV_F32,
                    KV_BF16)
 
 _F = C.POINTER(C.c_float)
@@ -42,6 +42,11 @@ def _u16(a, n: int, name: str):
         raise ValueError(f"{name}: expected {n} bf16 values, got {a.size}")
     return a
 
+
+_pack_shared_prefix_attn = packer(SharedPrefixAttn)
+_pack_attn_weights = packer(AttnWeights)
+_pack_kv_evict = packer(KvEvict)
+_pack_verify_drafts = packer(VerifyDrafts)
 
 _LIVE = weakref.WeakSet()
 
@@ -550,22 +555,19 @@ class Ctx:
 
     def shared_prefix_attn_dev(self, **fields):
         """Attention of a batch whose sequences share a prefix; ``fields`` are those of ``mfc_shared_prefix_attn``."""
-        rc = self._lib.mfc_shared_prefix_attn_dev(self._h, C.byref(SharedPrefixAttn(**fields)))
-        self._check(rc, "mfc_shared_prefix_attn_dev")
+        self._check(self._lib.mfc_shared_prefix_attn_dev(self._h, _pack_shared_prefix_attn(**fields)), "mfc_shared_prefix_attn_dev")
 
     def attn_weights_accumulate_dev(self, **fields):
         """Adds a step's attention weights to the running sum of every cached row (``mfc_attn_weights``)."""
-        rc = self._lib.mfc_attn_weights_accumulate_dev(self._h, C.byref(AttnWeights(**fields)))
-        self._check(rc, "mfc_attn_weights_accumulate_dev")
+        self._check(self._lib.mfc_attn_weights_accumulate_dev(self._h, _pack_attn_weights(**fields)), "mfc_attn_weights_accumulate_dev")
 
     def kv_evict_dev(self, **fields):
         """Keeps the ``budget`` heaviest rows of every (sequence, kv head), in place (``mfc_kv_evict``)."""
-        self._check(self._lib.mfc_kv_evict_dev(self._h, C.byref(KvEvict(**fields))), "mfc_kv_evict_dev")
+        self._check(self._lib.mfc_kv_evict_dev(self._h, _pack_kv_evict(**fields)), "mfc_kv_evict_dev")
 
     def verify_drafts_dev(self, **fields):
         """Accepts drafted tokens against the target's probabilities (``mfc_verify_drafts``)."""
-        rc = self._lib.mfc_verify_drafts_dev(self._h, C.byref(VerifyDrafts(**fields)))
-        self._check(rc, "mfc_verify_drafts_dev")
+        self._check(self._lib.mfc_verify_drafts_dev(self._h, _pack_verify_drafts(**fields)), "mfc_verify_drafts_dev")
 
     def linear_attn_step_stateless(self, layer: int, qkv, z, alpha, beta, conv_state, ssm_state):
         """Returns (out, new_conv_state, new_ssm_state); inputs are not modified."""
