@@ -98,8 +98,8 @@ struct mfc_ctx {
     unsigned *tickets = nullptr, *group_tickets = nullptr, *status = nullptr;
     unsigned *mv_sched = nullptr;  // two pairs (tile counter, finished CTAs) of the one-vector projection kernel, used in turn
     unsigned mv_launches = 0;
-    int *evict_counts = nullptr;   // moves of every unit of an eviction
     int *serve_plan = nullptr;     // tile plan of a shared-prefix attention call (written by its main kernel, read by its merge)
+    int *evict_counts = nullptr;   // moves of every unit of an eviction
     bool mv_overlap = true;        // tuning "matvec_overlap"
     struct MvMap {
         const uint32_t *w;

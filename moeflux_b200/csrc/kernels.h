@@ -340,8 +340,8 @@ struct SharedAttnParams {
     const int32_t *lens;
     __nv_bfloat16 *out;
     float *lse;
+    int *plan;                        // [0], [1]: prefix and own tiles per CTA, [8 + b]: first own tile of sequence b
     float *part_o, *part_m, *part_l;  // partials: prefix slots of 128 rows, then own slots of own_rows rows
-    int *plan;                        // [0] own tiles per CTA, [8 + b] first own tile of sequence b
     unsigned *status;
     int B, T, H, Hkv, group;
     int prefix_len, own_cap;

@@ -9,11 +9,9 @@
 // third of what HBM needs to deliver them, so the idle rows cost nothing.
 //
 // Work split: the 128-row tiles of the prefix units (kv head, 128 query rows) form one sequence, those of the own units
-// (sequence, kv head) another; both are cut into equal runs, and the persistent CTA of an SM takes one run of each (of the
-// own tiles counted from the last CTA, so that a small call's two kinds meet on different SMs).  An own unit costs a
-// segment start and end (about 10 us in all) for a few tiles, so they are spread over all CTAs.  A CTA writes one
+// (sequence, kv head) another; both are cut into equal runs for the persistent CTAs, one per SM (see Plan).  A CTA writes one
 // un-normalised partial (o, m, l) per unit it touches; the merge kernel joins the partials of a query row by log-sum-exp,
-// in a fixed order, and applies the gate.  Lengths are read on the device: every CTA finds its place by a scan over them.
+// in a fixed order, and applies the gate.  Lengths are read on the device.
 //
 // CTA (320 threads): warps 0-7 softmax (thread = query row x half of the 128 columns), warp 8 issues every tcgen05.mma,
 // warp 9 every TMA load.  Shared memory: Q 64 KiB and a ring of five 32 KiB granules that K and V share in the order in
@@ -100,6 +98,70 @@ __device__ __forceinline__ int own_len(const SharedAttnParams &p, int b) {
 }
 __device__ __forceinline__ int own_tiles(const SharedAttnParams &p, int b) { return (own_len(p, b) + SP_N - 1) / SP_N; }
 
+// How a call's tiles are dealt to CTAs: the prefix tiles in runs of `run` to the CTAs 0, 1, ..., the own tiles in runs of
+// `own_run` to the CTAs grid - 1, grid - 2, ....  Either every CTA takes a run of both, or (a call with few tiles per CTA,
+// where a second segment's start and end cost more than its tiles) the first `prefix_ctas` take prefix tiles only and the
+// others own tiles only.  The choice minimises the longest CTA, a segment counted as SP_SEG_COST tiles on top of its own
+// (measured: 5.4 thousand cycles to write a partial of 128 rows, about 4 thousand to fill and drain, against 2.3 thousand
+// per tile) and an own tile, whose rows come from HBM and not from L2, as a quarter more; the split has to win by a tenth
+// (64 sequences x 4 tokens over 32768 rows, where the two estimates meet: 284 us dealt to all, 302 us split).  Every warp
+// computes the plan by itself from the lengths; 32 splits, one a lane, are looked at.
+struct Plan {
+    int run, own_run;
+    int total_own;
+    int chunk, lane_begin;  // lane l covers sequences [l * chunk, ...): its first own tile
+};
+constexpr float SP_SEG_COST = 4.0f, SP_OWN_TILE_COST = 1.25f, SP_SPLIT_GAIN = 0.9f;
+
+__device__ __forceinline__ Plan make_plan(const SharedAttnParams &p, bool *bad) {
+    const int lane = threadIdx.x & 31;
+    const int per = p.Hkv * p.own_mtiles, total_p = p.Hkv * p.prefix_mtiles * p.prefix_tiles;
+    Plan pl;
+    pl.chunk = (p.B + 31) / 32;
+    const int b_lo = min(lane * pl.chunk, p.B), b_hi = min(b_lo + pl.chunk, p.B);
+    int mine = 0, some = 0;
+    bool off = false;
+    for (int b = b_lo; b < b_hi; b++) {
+        const int nt = own_tiles(p, b);
+        mine += per * nt;
+        some += nt > 0;
+        off |= p.lens[b] < 0 || p.lens[b] > p.own_cap;
+    }
+    *bad = off;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+    }
+    pl.lane_begin = inc - mine;
+    pl.total_own = __shfl_sync(0xffffffffu, inc, 31);
+    const float units_p = (float)(p.Hkv * p.prefix_mtiles), units_o = (float)(per * (int)__reduce_add_sync(0xffffffffu, some));
+    auto cost = [&](int tiles, float units, int ctas, float tile_cost) {
+        const float inv = __frcp_rn((float)ctas), run = ceilf((float)tiles * inv);
+        return tile_cost * run + SP_SEG_COST * fminf(run, 1.0f + units * inv);
+    };
+    int ctas = p.grid;  // for the prefix; grid: both kinds on every CTA
+    if (total_p > 0 && pl.total_own > 0) {
+        float best = SP_SPLIT_GAIN * (cost(total_p, units_p, p.grid, 1.0f) + cost(pl.total_own, units_o, p.grid, SP_OWN_TILE_COST));
+        int at = p.grid;
+        const int c = (lane + 1) * p.grid / 33;  // a split: c CTAs for the prefix
+        if (c >= 1) {
+            const float t = fmaxf(cost(total_p, units_p, c, 1.0f), cost(pl.total_own, units_o, p.grid - c, SP_OWN_TILE_COST));
+            if (t < best) {
+                best = t;
+                at = c;
+            }
+        }
+        // the least cost of all lanes, the smallest split among equals
+        const unsigned least = __reduce_min_sync(0xffffffffu, __float_as_uint(best));
+        ctas = (int)__reduce_min_sync(0xffffffffu, __float_as_uint(best) == least ? (unsigned)at : 0xffffffffu);
+    }
+    const int own_ctas = ctas == p.grid ? p.grid : p.grid - ctas;
+    pl.run = (total_p + ctas - 1) / ctas;
+    pl.own_run = max(1, (pl.total_own + own_ctas - 1) / own_ctas);
+    return pl;
+}
 // A segment: the tiles [t0, t0 + nt) of one unit.  Every role of a CTA walks the same segments by itself: first its run
 // of the prefix tiles, then its run of the own tiles.
 struct Walk {
@@ -152,6 +214,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + SP_OFF_BAR);
+    // (bars[11 .. 13] and bars[16] count the softmax warps, the others one arrival)
     uint64_t *full = bars;                  // [5] TMA: granule landed
     uint64_t *empty = bars + SP_GRAN;       // [5] tcgen05.commit: the products that read the granule are done
     uint64_t *s_ready = bars + 10;          // tcgen05.commit: scores of a tile are in tensor memory
@@ -161,79 +224,52 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     uint64_t *q_ready = bars + 16;          // softmax warps: the segment's Q is in shared memory
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
     volatile int *s_fail = reinterpret_cast<volatile int *>(bars + 18);
-    int *s_scan = reinterpret_cast<int *>(bars + 19);  // one per warp, then the place [2]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    // ---- scan over the lengths: tiles in all, this CTA's run, its first sequence ----
-    const int per_seq = p.Hkv * p.own_mtiles;
-    const int chunk = (p.B + SP_THREADS - 1) / SP_THREADS;
-    const int b_lo = min(tid * chunk, p.B), b_hi = min(b_lo + chunk, p.B);
-    int mine = 0;
-    for (int b = b_lo; b < b_hi; b++) {
-        mine += per_seq * own_tiles(p, b);
-        if (blockIdx.x == 0 && (p.lens[b] < 0 || p.lens[b] > p.own_cap)) atomicOr(p.status, STATUS_BAD_ITEM);
-    }
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-    }
-    if (lane == 31) s_scan[warp] = inc;
-    if (tid == 0) {
-        for (int i = 0; i < SP_GRAN; i++) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
-        mbar_init(s_ready, 1);
-        mbar_init(s_read, SP_SOFT);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&p_ready[i], SP_SOFT);
-            mbar_init(&pv_done[i], 1);
-        }
-        mbar_init(q_ready, SP_SOFT);
-        *s_fail = 0;
-        mbar_fence_init();
-    }
-    __syncthreads();
-    const int total_p = p.Hkv * p.prefix_mtiles * p.prefix_tiles;
-    int base = 0, total_own = 0;
-    for (int w = 0; w < SP_THREADS / 32; w++) {
-        if (w < warp) base += s_scan[w];
-        total_own += s_scan[w];
-    }
-    const int run = (total_p + (int)gridDim.x - 1) / (int)gridDim.x, own_run = max(1, (total_own + (int)gridDim.x - 1) / (int)gridDim.x);
-    const int own_cta = (int)gridDim.x - 1 - (int)blockIdx.x;
-    Walk walk;
-    walk.at = min((int)blockIdx.x * run, total_p);
-    walk.end = min(walk.at + run, total_p);
-    walk.own_at = min(own_cta * own_run, total_own);
-    walk.own_end = min(walk.own_at + own_run, total_own);
-    {
-        int first = base + inc - mine;
-        for (int b = b_lo; b < b_hi; b++) {
-            const int n = per_seq * own_tiles(p, b);
-            if (blockIdx.x == 0) p.plan[8 + b] = first;
-            if (walk.own_at >= first && walk.own_at < first + n) {
-                s_scan[SP_THREADS / 32] = b;
-                s_scan[SP_THREADS / 32 + 1] = first;
-            }
-            first += n;
-        }
-        if (blockIdx.x == 0 && tid == 0) p.plan[0] = own_run;
-    }
-    if (walk.at >= walk.end && walk.own_at >= walk.own_end) return;  // more CTAs than tiles
-
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge kernel may prepare itself
     if (warp == 0) {
         tmem_alloc(tmem_slot, SP_TMEM_COLS);
         tmem_relinquish();
     }
+    if (warp == 1) {
+        if (lane < 17) mbar_init(&bars[lane], (lane >= 11 && lane <= 13) || lane == 16 ? SP_SOFT : 1);
+        if (lane == 17) *s_fail = 0;
+        mbar_fence_init();
+    }
+    __syncwarp();
+    // ---- every warp by itself: the plan, this CTA's runs, its first sequence ----
+    const int own_cta = (int)gridDim.x - 1 - (int)blockIdx.x;
+    Walk walk;
+    {
+        bool bad;
+        const Plan pl = make_plan(p, &bad);
+        if (bad && blockIdx.x == 0 && warp == 0) atomicOr(p.status, STATUS_BAD_ITEM);
+        const int total_p = p.Hkv * p.prefix_mtiles * p.prefix_tiles;
+        walk.at = min((int)blockIdx.x * pl.run, total_p);
+        walk.end = min(walk.at + pl.run, total_p);
+        walk.own_at = (int)min((long long)own_cta * pl.own_run, (long long)pl.total_own);
+        walk.own_end = min(walk.own_at + pl.own_run, pl.total_own);
+        // the last lane whose sequences begin at or before the first own tile; next() walks on from there
+        const unsigned starts = __ballot_sync(0xffffffffu, pl.lane_begin <= walk.own_at);
+        const int src = 31 - __clz(starts);
+        walk.b = src * pl.chunk;
+        walk.begin = __shfl_sync(0xffffffffu, pl.lane_begin, src);
+        if (blockIdx.x == 0 && warp == 2) {  // for the merge kernel
+            if (lane == 0) {
+                p.plan[0] = pl.run;
+                p.plan[1] = pl.own_run;
+            }
+            int first = pl.lane_begin;
+            for (int b = min(lane * pl.chunk, p.B); b < min((lane + 1) * pl.chunk, p.B); b++) {
+                p.plan[8 + b] = first;
+                first += p.Hkv * p.own_mtiles * own_tiles(p, b);
+            }
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    walk.b = s_scan[SP_THREADS / 32];  // used only when the CTA has own tiles (then some thread has set them)
-    walk.begin = s_scan[SP_THREADS / 32 + 1];
     const uint32_t tmem = *tmem_slot;
     // Bounded waits of a whole warp, on one barrier or on three at once (a wait that succeeds at once still costs a round
     // trip to shared memory, so the issuer asks for all it needs in one go).  The failure flag is looked at only after a
@@ -289,10 +325,13 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 gi++;
             }
         };
-        // The first requests wait for the query rows: those asked for behind every CTA's first 160 KiB came 6 us later.
-        ok = warp_wait(q_ready, 0);
+        // The first K rows are asked for beside the query rows, all others behind them: query rows asked for behind every
+        // CTA's first 160 KiB came 6 us later.
+        bool first = true;
         while (ok && walk.next(p)) {
             load_k(walk, walk.t0);
+            if (first && ok) ok = warp_wait(q_ready, 0);
+            first = false;
             for (int j = 0; j < walk.nt && ok; j++) {
                 if (j + 1 < walk.nt) load_k(walk, walk.t0 + j + 1);
                 load_v(walk, walk.t0 + j);
@@ -404,8 +443,10 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         };
         unsigned n = 0;
         bool more = walk.next(p);
-        request_q(walk);  // (a CTA without a tile has left)
-        q_landed();
+        if (more) {
+            request_q(walk);
+            q_landed();
+        }
         while (more) {
             const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
             // columns of the unit this row sees
@@ -571,115 +612,166 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
 }
 
 // Joins the partials of the query rows by log-sum-exp, in a fixed order, and applies the gate.  CTA = 32 consecutive
-// query rows of a kv head (lane = row) x 32 dims; warp w takes the partials w, w + 8, ... of every row (the prefix
-// unit's first, then the own unit's), and the warps' results are joined through shared memory.
+// query rows of a kv head (lane = row).  Few partials per row: warp w takes the dims [32 w, 32 w + 32) of all partials
+// (the prefix unit's first, then the own unit's).  Many (FEW false; a long prefix cut for a small batch): the CTA takes 32
+// dims, warp w the partials w, w + 8, ..., and the warps' results are joined through shared memory.
 constexpr int MG_WARPS = 8;
 constexpr int MG_DIMS = 32;
-__global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const SharedAttnParams p) {
-    __shared__ float s_m[MG_WARPS][32], s_l[MG_WARPS][32];
-    __shared__ float4 s_o[MG_WARPS][MG_DIMS / 4][33];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows_hk = p.B * p.T * p.group;
-    const int blocks_hk = (rows_hk + 31) / 32;
-    const int hk = blockIdx.x / blocks_hk, idx = (blockIdx.x - hk * blocks_hk) * 32 + lane;
-    const int d0 = blockIdx.y * MG_DIMS;
-    const int own_run = p.plan[0], run = (p.Hkv * p.prefix_mtiles * p.prefix_tiles + p.grid - 1) / p.grid;
-    // prefix: partials [0, np); own: partials [np, np + no)
-    int np = 0, no = 0, b = 0, t = 0, hg = 0, pr = 0, orow = 0;
-    size_t p0 = 0, o0 = 0;  // first row of the first slot
-    if (idx < rows_hk) {
-        const int bt = idx / p.group;
-        hg = idx - bt * p.group;
-        b = bt / p.T;
-        t = bt - b * p.T;
-        if (p.prefix_tiles > 0) {
-            const int mt = idx / SP_M, unit = hk * p.prefix_mtiles + mt;
-            const int first = unit * p.prefix_tiles / run, last = ((unit + 1) * p.prefix_tiles - 1) / run;
-            np = last - first + 1;
-            p0 = ((size_t)unit + first) * SP_M;
-            pr = idx - mt * SP_M;
-        }
-        const int nt = own_tiles(p, b);
-        if (nt > 0) {
-            const int i = t * p.group + hg, mt = i / SP_M, u = hk * p.own_mtiles + mt;
-            const int begin = p.plan[8 + b] + u * nt;
-            const int first = begin / own_run, last = (begin + nt - 1) / own_run;
-            no = last - first + 1;
-            o0 = ((size_t)p.Hkv * p.prefix_mtiles + p.grid) * SP_M + ((size_t)b * p.Hkv * p.own_mtiles + u + first) * p.own_rows;
-            orow = i - mt * SP_M;
-        }
+constexpr int MG_FEW = 12, MG_FEW_BLOCKS = 128;
+
+struct RowParts {
+    int np, no;      // partials of the prefix unit and of the own unit
+    int pr, orow;    // the row within their slots
+    size_t p0, o0;   // first row of the first slot of each
+};
+// Partials of query row idx of kv head hk.
+__device__ __forceinline__ RowParts row_parts(const SharedAttnParams &p, int hk, int idx) {
+    RowParts r = {0, 0, 0, 0, 0, 0};
+    const int bt = idx / p.group, b = bt / p.T;
+    const int run = p.plan[0], own_run = p.plan[1], nt = own_tiles(p, b);
+    if (p.prefix_tiles > 0) {
+        const int mt = idx / SP_M, unit = hk * p.prefix_mtiles + mt;
+        const int first = unit * p.prefix_tiles / run, last = ((unit + 1) * p.prefix_tiles - 1) / run;
+        r.np = last - first + 1;
+        r.p0 = ((size_t)unit + first) * SP_M;
+        r.pr = idx - mt * SP_M;
     }
-    float M = -INFINITY, L = 0.0f;
+    if (nt > 0) {
+        const int i = idx - b * p.T * p.group, mt = i / SP_M, u = hk * p.own_mtiles + mt;
+        const int begin = p.plan[8 + b] + u * nt;
+        const int first = begin / own_run, last = (begin + nt - 1) / own_run;
+        r.no = last - first + 1;
+        r.o0 = ((size_t)p.Hkv * p.prefix_mtiles + p.grid) * SP_M + ((size_t)b * p.Hkv * p.own_mtiles + u + first) * p.own_rows;
+        r.orow = i - mt * SP_M;
+    }
+    return r;
+}
+struct Joined {
+    float M, L;
     float4 acc[MG_DIMS / 4];
+};
+// Partials from, from + step, ... of a row, MG_DIMS dims from d0 on.
+__device__ __forceinline__ void join_parts(const SharedAttnParams &p, const RowParts &r, int from, int step, int d0, Joined &j) {
+    j.M = -INFINITY;
+    j.L = 0.0f;
 #pragma unroll
-    for (int i = 0; i < MG_DIMS / 4; i++) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c = warp; c < np + no; c += MG_WARPS) {
-        const bool pre = c < np;
-        const int srows = pre ? SP_M : p.own_rows, r = pre ? pr : orow;
-        const size_t row0 = pre ? p0 + (size_t)c * SP_M : o0 + (size_t)(c - np) * p.own_rows;
-        const float4 *src = reinterpret_cast<const float4 *>(p.part_o + row0 * HEAD_DIM) + r;
+    for (int i = 0; i < MG_DIMS / 4; i++) j.acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = from; c < r.np + r.no; c += step) {
+        const bool pre = c < r.np;
+        const int srows = pre ? SP_M : p.own_rows, row = pre ? r.pr : r.orow;
+        const size_t row0 = pre ? r.p0 + (size_t)c * SP_M : r.o0 + (size_t)(c - r.np) * p.own_rows;
+        const float4 *src = reinterpret_cast<const float4 *>(p.part_o + row0 * HEAD_DIM) + row;
         float4 o[MG_DIMS / 4];
 #pragma unroll
         for (int i = 0; i < MG_DIMS / 4; i++) o[i] = src[(size_t)(d0 / 4 + i) * srows];
-        const float m = p.part_m[row0 + r], l = p.part_l[row0 + r];
+        const float m = p.part_m[row0 + row], l = p.part_l[row0 + row];
         if (m == -INFINITY) continue;  // no weight: contributes nothing, whatever it holds
-        const float mn = fmaxf(M, m);
-        const float wa = M == -INFINITY ? 0.0f : ex2_approx(M - mn), wb = ex2_approx(m - mn);
-        M = mn;
-        L = L * wa + l * wb;
+        const float mn = fmaxf(j.M, m);
+        const float wa = j.M == -INFINITY ? 0.0f : ex2_approx(j.M - mn), wb = ex2_approx(m - mn);
+        j.M = mn;
+        j.L = j.L * wa + l * wb;
 #pragma unroll
         for (int i = 0; i < MG_DIMS / 4; i++) {
-            acc[i].x = fmaf(wb, o[i].x, acc[i].x * wa);
-            acc[i].y = fmaf(wb, o[i].y, acc[i].y * wa);
-            acc[i].z = fmaf(wb, o[i].z, acc[i].z * wa);
-            acc[i].w = fmaf(wb, o[i].w, acc[i].w * wa);
+            j.acc[i].x = fmaf(wb, o[i].x, j.acc[i].x * wa);
+            j.acc[i].y = fmaf(wb, o[i].y, j.acc[i].y * wa);
+            j.acc[i].z = fmaf(wb, o[i].z, j.acc[i].z * wa);
+            j.acc[i].w = fmaf(wb, o[i].w, j.acc[i].w * wa);
         }
     }
-    s_m[warp][lane] = M;
-    s_l[warp][lane] = L;
+}
+__device__ __forceinline__ float2 gate2(uint32_t bits) {
+    return make_float2(1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(bits & 0xffffu)))),
+                       1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(bits >> 16)))));
+}
+
+template <bool FEW>
+__global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const SharedAttnParams p) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows_hk = p.B * p.T * p.group;
+    const int blocks_hk = (rows_hk + 31) / 32;
+    const int hk = blockIdx.x / blocks_hk, idx0 = (blockIdx.x - hk * blocks_hk) * 32;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan and the partials are written by the kernel before
+    RowParts parts = {0, 0, 0, 0, 0, 0};
+    if (idx0 + lane < rows_hk) parts = row_parts(p, hk, idx0 + lane);
+    if (FEW) {
+        const int idx = idx0 + lane, d0 = warp * MG_DIMS;
+        if (idx >= rows_hk) return;
+        const int bt = idx / p.group, h = hk * p.group + (idx - bt * p.group);
+        uint4 g[MG_DIMS / 8];
+        if (p.gate) {
+            const int b = bt / p.T, t = bt - b * p.T;
+            const uint4 *gp = reinterpret_cast<const uint4 *>(p.gate + (int64_t)b * p.g_seq + (int64_t)t * p.g_token + (int64_t)h * p.g_head + d0);
 #pragma unroll
-    for (int i = 0; i < MG_DIMS / 4; i++) s_o[warp][i][lane] = acc[i];
-    __syncthreads();
-    // thread = (row of the 32, four dims): eight threads write 64 consecutive bytes of a row
-    const int row = threadIdx.x >> 3, q4 = threadIdx.x & 7;
-    const int idx2 = (blockIdx.x - hk * blocks_hk) * 32 + row;
-    if (idx2 >= rows_hk) return;
-    M = -INFINITY;
+            for (int i = 0; i < MG_DIMS / 8; i++) g[i] = gp[i];
+        }
+        Joined j;
+        join_parts(p, parts, 0, 1, d0, j);
+        const bool none = j.M == -INFINITY;
+        const float inv = none ? 0.0f : 1.0f / j.L;
+        const size_t orw = (size_t)bt * p.H + h;
+        uint4 *dst = reinterpret_cast<uint4 *>(p.out + orw * HEAD_DIM + d0);
 #pragma unroll
-    for (int w = 0; w < MG_WARPS; w++) M = fmaxf(M, s_m[w][row]);
-    L = 0.0f;
-    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i = 0; i < MG_DIMS / 8; i++) {
+            const float4 a = j.acc[2 * i], c = j.acc[2 * i + 1];
+            float2 x0 = make_float2(a.x * inv, a.y * inv), x1 = make_float2(a.z * inv, a.w * inv);
+            float2 x2 = make_float2(c.x * inv, c.y * inv), x3 = make_float2(c.z * inv, c.w * inv);
+            if (p.gate) {
+                const float2 s0 = gate2(g[i].x), s1 = gate2(g[i].y), s2 = gate2(g[i].z), s3 = gate2(g[i].w);
+                x0 = make_float2(x0.x * s0.x, x0.y * s0.y);
+                x1 = make_float2(x1.x * s1.x, x1.y * s1.y);
+                x2 = make_float2(x2.x * s2.x, x2.y * s2.y);
+                x3 = make_float2(x3.x * s3.x, x3.y * s3.y);
+            }
+            dst[i] = make_uint4(pack_bf16x2(x0.x, x0.y), pack_bf16x2(x1.x, x1.y), pack_bf16x2(x2.x, x2.y), pack_bf16x2(x3.x, x3.y));
+        }
+        if (p.lse && warp == 0) p.lse[orw] = none ? -INFINITY : (j.M + log2f(j.L)) * 0.6931471805599453f;
+    } else {
+        __shared__ float s_m[MG_WARPS][32], s_l[MG_WARPS][32];
+        __shared__ float4 s_o[MG_WARPS][MG_DIMS / 4][33];
+        const int d0 = blockIdx.y * MG_DIMS;
+        Joined j;
+        join_parts(p, parts, warp, MG_WARPS, d0, j);
+        s_m[warp][lane] = j.M;
+        s_l[warp][lane] = j.L;
 #pragma unroll
-    for (int w = 0; w < MG_WARPS; w++) {
-        const float m = s_m[w][row];
-        if (m == -INFINITY) continue;
-        const float wt = ex2_approx(m - M);
-        const float4 o = s_o[w][q4][row];
-        L += wt * s_l[w][row];
-        a.x = fmaf(wt, o.x, a.x);
-        a.y = fmaf(wt, o.y, a.y);
-        a.z = fmaf(wt, o.z, a.z);
-        a.w = fmaf(wt, o.w, a.w);
+        for (int i = 0; i < MG_DIMS / 4; i++) s_o[warp][i][lane] = j.acc[i];
+        __syncthreads();
+        // thread = (row of the 32, four dims): eight threads write 64 consecutive bytes of a row
+        const int row = threadIdx.x >> 3, q4 = threadIdx.x & 7;
+        const int idx = idx0 + row;
+        if (idx >= rows_hk) return;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < MG_WARPS; w++) M = fmaxf(M, s_m[w][row]);
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < MG_WARPS; w++) {
+            const float m = s_m[w][row];
+            if (m == -INFINITY) continue;
+            const float wt = ex2_approx(m - M);
+            const float4 o = s_o[w][q4][row];
+            L += wt * s_l[w][row];
+            a.x = fmaf(wt, o.x, a.x);
+            a.y = fmaf(wt, o.y, a.y);
+            a.z = fmaf(wt, o.z, a.z);
+            a.w = fmaf(wt, o.w, a.w);
+        }
+        const bool none = M == -INFINITY;
+        const float inv = none ? 0.0f : 1.0f / L;
+        float2 x0 = make_float2(a.x * inv, a.y * inv), x1 = make_float2(a.z * inv, a.w * inv);
+        const int bt = idx / p.group, h = hk * p.group + (idx - bt * p.group);
+        const int d = d0 + 4 * q4;
+        if (p.gate) {
+            const int b = bt / p.T, t = bt - b * p.T;
+            const uint2 g = *reinterpret_cast<const uint2 *>(p.gate + (int64_t)b * p.g_seq + (int64_t)t * p.g_token + (int64_t)h * p.g_head + d);
+            const float2 s0 = gate2(g.x), s1 = gate2(g.y);
+            x0 = make_float2(x0.x * s0.x, x0.y * s0.y);
+            x1 = make_float2(x1.x * s1.x, x1.y * s1.y);
+        }
+        const size_t orw = (size_t)bt * p.H + h;
+        *reinterpret_cast<uint2 *>(p.out + orw * HEAD_DIM + d) = make_uint2(pack_bf16x2(x0.x, x0.y), pack_bf16x2(x1.x, x1.y));
+        if (p.lse && d == 0) p.lse[orw] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
-    const bool none = M == -INFINITY;
-    const float inv = none ? 0.0f : 1.0f / L;
-    a.x *= inv;
-    a.y *= inv;
-    a.z *= inv;
-    a.w *= inv;
-    const int bt = idx2 / p.group, h = hk * p.group + (idx2 - bt * p.group);
-    const int d = d0 + 4 * q4;
-    if (p.gate) {
-        const int bb = bt / p.T, tt = bt - bb * p.T;
-        const uint2 gb = *reinterpret_cast<const uint2 *>(p.gate + (int64_t)bb * p.g_seq + (int64_t)tt * p.g_token + (int64_t)h * p.g_head + d);
-        a.x *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.x & 0xffffu))));
-        a.y *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.x >> 16))));
-        a.z *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.y & 0xffffu))));
-        a.w *= 1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(gb.y >> 16))));
-    }
-    const size_t orw = (size_t)bt * p.H + h;
-    *reinterpret_cast<uint2 *>(p.out + orw * HEAD_DIM + d) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-    if (p.lse && d == 0) p.lse[orw] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace
@@ -694,9 +786,22 @@ cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &
     shared_prefix_attn_kernel<<<p.grid, SP_THREADS, SP_SMEM, stream>>>(pk, pv, ok, ov, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const unsigned blocks = (unsigned)(p.Hkv * ((p.B * p.T * p.group + 31) / 32));
-    shared_attn_merge_kernel<<<dim3(blocks, HEAD_DIM / MG_DIMS), 32 * MG_WARPS, 0, stream>>>(p);
-    return cudaGetLastError();
+    // partials a row has at most, about: the CTAs a unit is spread over, of the prefix and of the own rows
+    const int64_t units_p = (int64_t)p.Hkv * p.prefix_mtiles, units_o = (int64_t)p.B * p.Hkv * p.own_mtiles;
+    const int64_t own_t = (p.own_cap + SP_N - 1) / SP_N, np = p.grid / units_p + 2, no = p.grid / units_o + 2;
+    // (with few rows the other form spreads them over more SMs: 64 rows of five partials take 6 us less)
+    const int64_t blocks = (int64_t)p.Hkv * ((p.B * p.T * p.group + 31) / 32);
+    const bool few = (np < p.prefix_tiles ? np : p.prefix_tiles) + (no < own_t ? no : own_t) <= MG_FEW && blocks >= MG_FEW_BLOCKS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks, few ? 1 : HEAD_DIM / MG_DIMS);
+    cfg.blockDim = dim3(32 * MG_WARPS);
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return few ? cudaLaunchKernelEx(&cfg, shared_attn_merge_kernel<true>, p) : cudaLaunchKernelEx(&cfg, shared_attn_merge_kernel<false>, p);
 }
 
 }  // namespace mfc
