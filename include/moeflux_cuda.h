@@ -402,7 +402,8 @@ int mfc_sdpa_static_status(void *stream);
  * side.  head_dim is 256.  Strides are in elements.  Return 0 on success, -1
  * on a refused argument (nothing was launched).  Lengths read from device
  * memory are checked by the kernels: a sequence whose length lies outside
- * [0, capacity] is treated as empty and reported by mfc_synchronize.
+ * [0, capacity] is treated as empty and reported by mfc_synchronize.  The tunings
+ * gqa_wait_spins and gqa_inject_lost_load apply to the two attention calls.
  * ---------------------------------------------------------------------- */
 
 /* Where a full-attention layer's rows of one sequence live: *k and *v point at

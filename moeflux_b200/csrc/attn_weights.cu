@@ -32,7 +32,6 @@ constexpr uint32_t AW_GRAN_BYTES = 32768;
 constexpr int AW_MAX_GRAN = 6;
 constexpr uint32_t AW_CTRL = 1024;         // barriers and flags
 constexpr uint32_t AW_SMEM_MAX = 232448;
-constexpr unsigned AW_SPINS = 1u << 22;
 constexpr float LOG2E_AW = 1.4426950408889634f;
 
 // Shared memory: ring of granules | query buffers | their lse and limits | control
@@ -160,7 +159,7 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     auto warp_wait = [&](uint64_t *bar, unsigned parity) -> bool {
-        for (unsigned i = 0; i < AW_SPINS; i++) {
+        for (unsigned i = 0; i < p.wait_spins; i++) {
             if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
             if (*s_fail) return false;
         }
@@ -197,7 +196,8 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     if (gi >= (unsigned)lay.gran && !(ok = warp_wait(&empty[gst], gph ^ 1u))) break;
                     if (elect_one()) {
                         mbar_expect_tx(&full[gst], AW_GRAN_BYTES);
-                        tma_load_5d(smem + gst * AW_GRAN_BYTES, &k_map, 0, (walk.t0 + j) * AW_TILE, 2 * d, walk.hk, walk.b, &full[gst]);
+                        if (!(p.inject_lost_load && blockIdx.x == 0 && gi == 0))
+                            tma_load_5d(smem + gst * AW_GRAN_BYTES, &k_map, 0, (walk.t0 + j) * AW_TILE, 2 * d, walk.hk, walk.b, &full[gst]);
                     }
                     advance();
                 }
@@ -342,7 +342,7 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 ph ^= 1u;
             }
             st--;
-            mbar_wait_bounded(&full[st], ph);
+            mbar_wait_bounded(&full[st], ph, p.wait_spins);
         }
     }
     if (warp == 0) tmem_dealloc(tmem, cols);

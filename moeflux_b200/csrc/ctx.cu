@@ -1615,6 +1615,8 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
     p.plan = c->serve_plan;
     p.status = c->status;
     p.scale = a->softmax_scale;
+    p.wait_spins = c->gqa_wait_spins ? c->gqa_wait_spins : 1u << 22;
+    p.inject_lost_load = c->gqa_inject_lost_load;
     CUtensorMap m[4];
     memset(m, 0, sizeof(m));
     if (has_prefix && (!make_rows_map(c, &m[0], a->prefix_k, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 2, 128) ||
@@ -1679,6 +1681,8 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *c, const mfc_attn_weights *a) try {
     p.cap = a->cap;
     p.scale = a->softmax_scale;
     p.decay = a->decay;
+    p.wait_spins = c->gqa_wait_spins ? c->gqa_wait_spins : 1u << 22;
+    p.inject_lost_load = c->gqa_inject_lost_load;
     if ((int64_t)p.B * p.Hkv * ((p.cap + 127) / 128) >= ((int64_t)1 << 30)) {
         fail(c, "too many rows in one call");
         return -1;

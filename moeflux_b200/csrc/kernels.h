@@ -325,6 +325,8 @@ struct AttnWeightsParams {
     unsigned *status;
     int B, T, H, Hkv, group, cap;
     float scale, decay;
+    unsigned wait_spins;   // poll limit of the bounded waits
+    int inject_lost_load;  // test hook: CTA 0 arms its first granule and requests nothing for it
 };
 cudaError_t attn_weights_configure();
 // k_map: over the cached K rows as for the attention call (boxes of two fourths x 128 rows)
@@ -350,6 +352,8 @@ struct SharedAttnParams {
     int own_rows;                     // rows of an own slot: min(128, T * group)
     int grid;
     float scale;
+    unsigned wait_spins;              // poll limit of the bounded waits
+    int inject_lost_load;             // test hook: CTA 0 arms its first granule and requests nothing for it
 };
 cudaError_t shared_prefix_attn_configure();
 // Maps (64 dims, row, fourth of the dims, kv head, sequence) over the prefix and own rows; boxes of two fourths x 128

@@ -48,7 +48,6 @@ constexpr uint32_t SP_OFF_XM = SP_OFF_RING + SP_GRAN * GRAN_BYTES;  // row-maxim
 constexpr uint32_t SP_OFF_BAR = SP_OFF_XM + 1024;
 constexpr uint32_t SP_SMEM = SP_OFF_BAR + 512 + 1024;      // + alignment slack
 static_assert(SP_SMEM <= 232448, "shared memory of an SM");
-constexpr unsigned SP_SPINS = 1u << 22;                     // polls of a bounded wait, each a hardware-defined short time
 constexpr float LOG2E_SP = 1.4426950408889634f;
 
 constexpr uint32_t SP_TMEM_COLS = 512;
@@ -275,14 +274,14 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     // trip to shared memory, so the issuer asks for all it needs in one go).  The failure flag is looked at only after a
     // poll that found nothing.
     auto warp_wait = [&](uint64_t *bar, unsigned parity) -> bool {
-        for (unsigned i = 0; i < SP_SPINS; i++) {
+        for (unsigned i = 0; i < p.wait_spins; i++) {
             if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
             if (*s_fail) return false;
         }
         return false;
     };
     auto warp_wait3 = [&](uint64_t *b0, unsigned p0, uint64_t *b1, unsigned p1, uint64_t *b2, unsigned p2) -> bool {
-        for (unsigned i = 0; i < SP_SPINS; i++) {
+        for (unsigned i = 0; i < p.wait_spins; i++) {
             const bool r0 = mbar_try_wait(b0, p0), r1 = mbar_try_wait(b1, p1), r2 = mbar_try_wait(b2, p2);
             if (__all_sync(0xffffffffu, r0 && r1 && r2)) return true;
             if (*s_fail) return false;
@@ -306,7 +305,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 const unsigned st = gi % SP_GRAN;
                 if (elect_one()) {
                     mbar_expect_tx(&full[st], GRAN_BYTES);
-                    tma_load_5d(smem + SP_OFF_RING + st * GRAN_BYTES, s.own ? &ok_map : &pk_map, 0, tile * SP_N, 2 * d, s.hk, s.own ? s.b : 0,
+                    if (!(p.inject_lost_load && blockIdx.x == 0 && gi == 0))
+                        tma_load_5d(smem + SP_OFF_RING + st * GRAN_BYTES, s.own ? &ok_map : &pk_map, 0, tile * SP_N, 2 * d, s.hk, s.own ? s.b : 0,
                                 &full[st]);
                 }
                 gi++;
@@ -607,7 +607,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     if (tid == 0 && *s_fail) atomicOr(p.status, STATUS_TMA_TIMEOUT);
     // on the ordinary path every granule has been used; after a failure the copies in flight land before the CTA leaves
     if (warp == SP_SOFT + 1 && lane == 0 && *s_fail)
-        for (unsigned k = gi > SP_GRAN ? gi - SP_GRAN : 0; k < gi; k++) mbar_wait_bounded(&full[k % SP_GRAN], (k / SP_GRAN) & 1u);
+        for (unsigned k = gi > SP_GRAN ? gi - SP_GRAN : 0; k < gi; k++) mbar_wait_bounded(&full[k % SP_GRAN], (k / SP_GRAN) & 1u, p.wait_spins);
     if (warp == 0) tmem_dealloc(tmem, SP_TMEM_COLS);
 }
 

@@ -491,3 +491,158 @@ def test_verify_drafts_edges(ctx):
     n, tok = call_verify(ctx, p, None, x, None, ua, us)
     assert n.tolist() == [1, 0, 0, 0, 0, 0]
     assert tok.tolist() == [[5, 5], [7, -1], [9, -1], [-1, -1], [199, -1], [12, -1]]
+
+
+# ---------------------------------------------------------------------------------------------------- together
+
+
+class _Rows:
+    """Device memory the context owns, as a torch tensor (for reading cached rows back)."""
+
+    def __init__(self, ptr, shape, strides):
+        self.__cuda_array_interface__ = dict(shape=tuple(shape), strides=tuple(2 * s for s in strides), typestr="<i2",
+                                             data=(ptr, False), version=3)
+
+
+def test_a_server_s_steps(M):
+    """A prompt is prefilled into a context once; a batch then decodes behind it with drafted tokens: attention over the
+    shared rows and each sequence's own, the rows' weights, verification, the lengths cut to what was accepted, and an
+    eviction when a sequence passes its budget.  Every call against its 64-bit form on the state the calls before left."""
+    g = gen(21)
+    layer, P, B, T, H, Hkv, cap, budget, V = 3, 300, 5, 3, 32, 2, 80, 40, 500
+    c = M.Ctx(num_layers=4, max_seq=512, n_seqs=2, kv_dtype=M.KV_BF16)
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    x = [rn(g, P, n, D) for n in (H, H, Hkv, Hkv)]
+    scratch = torch.empty(P, H, D, device="cuda", dtype=torch.bfloat16)
+    c.full_attn_prefill_dev(layer, 1, 0, P, x[0].data_ptr(), x[1].data_ptr(), x[2].data_ptr(), x[3].data_ptr(), scratch.data_ptr())
+    kp, vp, seq_stride, head_stride, rows = c.kv_cache_view(layer, 1)
+    assert rows == P and seq_stride == Hkv * head_stride
+    pk, pv = (torch.as_tensor(_Rows(a, (Hkv, P, D), (head_stride, D, 1)), device="cuda").view(torch.bfloat16) for a in (kp, vp))
+    c.synchronize()
+    assert torch.equal(pv, x[3].transpose(0, 1))  # V goes into the cache as it is
+
+    ok, ov = torch.zeros(B, Hkv, cap, D, device="cuda", dtype=torch.bfloat16), torch.zeros(B, Hkv, cap, D, device="cuda", dtype=torch.bfloat16)
+    ok.fill_(float("nan"))
+    ov.fill_(float("nan"))
+    w = torch.zeros(B, Hkv, cap, device="cuda")
+    pos = torch.zeros(B, Hkv, cap, device="cuda", dtype=torch.int32)
+    lens = torch.zeros(B, device="cuda", dtype=torch.int32)
+    nxt = torch.full((B,), P, device="cuda", dtype=torch.int32)
+    out, lse = torch.empty(B, T, H, D, device="cuda", dtype=torch.bfloat16), torch.empty(B, T, H, device="cuda")
+    evictions = 0
+    for step in range(24):
+        # the step's rows: the last accepted token and T - 1 drafts, appended by the caller
+        for b in range(B):
+            n = int(lens[b])
+            ok[b, :, n : n + T], ov[b, :, n : n + T] = rn(g, Hkv, T, D), rn(g, Hkv, T, D)
+            w[b, :, n : n + T] = 0.0
+            pos[b, :, n : n + T] = nxt[b] + torch.arange(T, device="cuda", dtype=torch.int32)
+        lens += T
+        q, gate = rn(g, B, T, H, D, scale=1.5), rn(g, B, T, H, D)
+        c.shared_prefix_attn_dev(**attn_args(q, gate, pk, pv, ok, ov, lens, out, lse))
+        w_before = w.clone()
+        c.attn_weights_accumulate_dev(**weights_args(q, ok, lens, lse, w))
+        p = torch.softmax(torch.randn(B, T, V, generator=g, device="cuda"), -1)
+        qd = torch.softmax(torch.log(p[:, : T - 1]) + 0.3 * torch.randn(B, T - 1, V, generator=g, device="cuda"), -1)
+        drafts = torch.multinomial(qd.view(-1, V), 1, generator=g).view(B, T - 1).to(torch.int32)
+        ua, us = torch.rand(B, T - 1, generator=g, device="cuda"), torch.rand(B, generator=g, device="cuda")
+        n_acc, tok = call_verify(c, p, qd, drafts, None, ua, us)
+        ro, rl, bo, bl = attn_ref(q, gate, pk, pv, ok, ov, lens)
+        assert ((out.double() - ro).abs() <= bo).all() and ((lse.double() - rl).abs() <= bl).all(), step
+        ref, tol = weights_ref(q, ok, lens, lse, w_before, 1.0)
+        used = (torch.arange(cap, device="cuda").view(1, 1, cap) < lens.view(B, 1, 1)).expand_as(w)
+        assert ((w.double() - ref).abs() <= tol)[used].all(), step
+        rn_, rt = verify_ref(p, qd, drafts, torch.full((B,), T - 1), ua, us)
+        assert torch.equal(n_acc, rn_) and torch.equal(tok, rt)
+        # rows of refused drafts are dropped; the drawn token's row is the next step's first
+        lens -= (T - 1 - n_acc.cuda())
+        nxt += 1 + n_acc.cuda()
+        if int(lens.max()) + T > cap or step % 8 == 7:
+            src = evict_ref(ok, ov, w, pos, lens, nxt, budget, P + 2, 6)
+            before = [t.clone() for t in (ok, ov, w, pos, lens)]
+            new = torch.empty_like(lens)
+            c.kv_evict_dev(n_seqs=B, num_kv_heads=Hkv, kv_dtype=M.KV_BF16, cap=cap, k=ok.data_ptr(), v=ov.data_ptr(),
+                           seq_stride=ok.stride(0), head_stride=ok.stride(1), row_stride=D, budget=budget, n_sink=P + 2, n_recent=6,
+                           lens=lens.data_ptr(), next_pos=nxt.data_ptr(), weights=w.data_ptr(), positions=pos.data_ptr(),
+                           map_seq_stride=w.stride(0), map_head_stride=w.stride(1), weights_out=w.data_ptr(),
+                           positions_out=pos.data_ptr(), lens_out=new.data_ptr())
+            c.synchronize()
+            evictions += int((before[4] > budget).sum())
+            for (b, h), rows_ in src.items():
+                ix = torch.tensor(rows_, device="cuda", dtype=torch.long)
+                n = len(rows_)
+                for now, was in zip((ok, ov, w, pos), before):
+                    assert torch.equal(now[b, h, :n], was[b, h, ix])
+                    assert torch.equal(now[b, h, n:].nan_to_num(7), was[b, h, n:].nan_to_num(7))
+            assert torch.equal(new, before[4].clamp(max=budget))
+            lens = new
+    assert evictions > B
+    assert torch.equal(pv, x[3].transpose(0, 1)) and c.kv_cache_view(layer, 1)[4] == P  # the shared rows are as they were
+    with pytest.raises(M.MfcError):
+        c.kv_cache_view(0, 0)  # not a full-attention layer
+    with pytest.raises(M.MfcError):
+        c.kv_cache_view(layer, 2)
+    c.check_guards()
+    c.close()
+
+
+@pytest.mark.parametrize("call", ["attn", "weights"])
+def test_a_lost_load_is_reported_and_the_context_survives(ctx, M, call):
+    """A barrier armed with no load issued for it: the wait runs out, every role leaves, the status names it, and the next
+    call is right."""
+    g = gen(31)
+    B, T, H, Hkv, cap = 3, 2, 32, 2, 300
+    q, ok, ov = rn(g, B, T, H, D), rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    pk, pv = rn(g, Hkv, 700, D), rn(g, Hkv, 700, D)
+    lens = torch.tensor([300, 130, 5], device="cuda", dtype=torch.int32)
+    out, lse = torch.zeros(B, T, H, D, device="cuda", dtype=torch.bfloat16), torch.zeros(B, T, H, device="cuda")
+    w = torch.zeros(B, Hkv, cap, device="cuda")
+    run = (lambda: ctx.shared_prefix_attn_dev(**attn_args(q, None, pk, pv, ok, ov, lens, out, lse))) if call == "attn" else (
+        lambda: ctx.attn_weights_accumulate_dev(**weights_args(q, ok, lens, lse, w)))
+    ctx.set_tuning("gqa_wait_spins", 2000)
+    ctx.set_tuning("gqa_inject_lost_load", 1)
+    try:
+        run()
+        with pytest.raises(M.MfcError, match="did not arrive"):
+            ctx.synchronize()
+    finally:
+        ctx.set_tuning("gqa_inject_lost_load", 0)
+        ctx.set_tuning("gqa_wait_spins", 0)
+    w.zero_()
+    run()
+    ctx.synchronize()
+    check_attn(ctx, q, None, pk, pv, ok, ov, lens)
+
+
+def test_refusals(ctx, M):
+    """One refused call per entry point and check; nothing is launched.  (All checks run without a GPU as well, on the
+    host code alone.)"""
+    t = torch.zeros(64 * 256, device="cuda", dtype=torch.bfloat16)
+    i = torch.zeros(64, device="cuda", dtype=torch.int32)
+    f = torch.zeros(64 * 256, device="cuda")
+    P, I, F = t.data_ptr(), i.data_ptr(), f.data_ptr()
+    attn = dict(n_seqs=1, n_tokens=1, num_attn_heads=2, num_kv_heads=1, softmax_scale=SCALE, q=P, q_seq_stride=512, q_token_stride=512,
+                q_head_stride=256, own_k=P, own_v=P, own_seq_stride=1024, own_head_stride=1024, own_row_stride=256, own_cap=4, own_lens=I, out=P)
+    wts = dict(n_seqs=1, n_tokens=1, num_attn_heads=2, num_kv_heads=1, softmax_scale=SCALE, decay=1.0, q=P, q_seq_stride=512,
+               q_token_stride=512, q_head_stride=256, k=P, k_seq_stride=1024, k_head_stride=1024, k_row_stride=256, cap=4, lens=I, lse=F, weights=F)
+    ev = dict(n_seqs=1, num_kv_heads=1, kv_dtype=M.KV_BF16, cap=4, k=P, v=P + 8192, seq_stride=1024, head_stride=1024, row_stride=256, budget=2,
+              lens=I, next_pos=I, weights=F, positions=I, map_seq_stride=4, map_head_stride=4, weights_out=F, positions_out=I, lens_out=I + 128)
+    vf = dict(n_seqs=1, max_drafts=2, vocab=8, target_probs=F, target_seq_stride=24, target_row_stride=8, draft_tokens=I, u_accept=F,
+              u_sample=F, n_accepted=I, tokens=I)
+    before = ctx.launch_count
+    for fn, base, bad in [
+        (ctx.shared_prefix_attn_dev, attn, [dict(n_tokens=0), dict(n_tokens=17), dict(num_attn_heads=17), dict(softmax_scale=0.0), dict(q=None),
+                                            dict(out=P + 2), dict(q_head_stride=4), dict(own_row_stride=128), dict(prefix_len=3), dict(n_seqs=4097),
+                                            dict(own_head_stride=-1024, num_attn_heads=4, num_kv_heads=2), dict(prefix_len=-1)]),
+        (ctx.attn_weights_accumulate_dev, wts, [dict(k=P + 8), dict(k_row_stride=12), dict(lse=None), dict(cap=-1), dict(num_kv_heads=0)]),
+        (ctx.kv_evict_dev, ev, [dict(budget=0), dict(kv_dtype=7), dict(v=P), dict(lens_out=I), dict(cap=300000), dict(row_stride=100), dict(weights=None)]),
+        (ctx.verify_drafts_dev, vf, [dict(max_drafts=33), dict(vocab=0), dict(tokens=None), dict(u_accept=None), dict(target_probs=F + 2)])]:
+        for change in bad:
+            with pytest.raises(M.MfcError):
+                fn(**{**base, **change})
+        with pytest.raises(TypeError):
+            fn(**{**base, "no_such_field": 1})
+    for fn, base in [(ctx.shared_prefix_attn_dev, attn), (ctx.attn_weights_accumulate_dev, wts), (ctx.kv_evict_dev, ev), (ctx.verify_drafts_dev, vf)]:
+        fn(**{**base, "n_seqs": 0})  # an empty batch is no error and no launch
+    assert ctx.launch_count == before
+    ctx.synchronize()
