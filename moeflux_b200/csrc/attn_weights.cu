@@ -100,6 +100,7 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     const AwLayout lay = aw_layout(nq);
     const uint32_t np = (uint32_t)lay.np;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + lay.off_ctrl);
+    // arrivals a phase: bars[0 .. 13] one, s_free 4, q_full 2, q_empty 9
     uint64_t *full = bars;            // [6] TMA: granule landed
     uint64_t *empty = bars + 6;       // [6] tcgen05.commit: the products that read the granule are done
     uint64_t *s_ready = bars + 12;    // [2] tcgen05.commit: scores of a tile are in tensor memory
@@ -116,17 +117,15 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         tmem_alloc(tmem_slot, cols);
         tmem_relinquish();
     }
-    if (tid == 32) {
-        for (int i = 0; i < 12; i++) mbar_init(&bars[i], 1);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&s_ready[i], 1);
-            mbar_init(&s_free[i], 4);
-            mbar_init(&q_full[i], 2);
-            mbar_init(&q_empty[i], 9);
-        }
-        *s_fail = 0;
+    if (warp == 1) {
+        if (lane < 20) mbar_init(&bars[lane], lane < 14 ? 1 : (lane < 16 ? 4 : (lane < 18 ? 2 : 9)));
+        if (lane == 20) *s_fail = 0;
         mbar_fence_init();
     }
+    if (tid == 64) prefetch_tmap(&k_map);
+    __syncwarp();
+    dependency_wait();
+    dependency_allow();
     // ---- every warp by itself: scan over the lengths, this CTA's run, its first sequence ----
     AwWalk walk;
     {
@@ -358,8 +357,7 @@ cudaError_t launch_attn_weights(const CUtensorMap &k_map, const AttnWeightsParam
     if (p.B <= 0 || p.cap <= 0) return cudaSuccess;
     const int64_t most = (int64_t)p.B * p.Hkv * ((p.cap + AW_TILE - 1) / AW_TILE);
     const int grid = most < n_sms ? (int)most : n_sms;
-    attn_weights_kernel<<<(unsigned)grid, AW_THREADS, aw_layout(p.T * p.group).total, stream>>>(k_map, p);
-    return cudaGetLastError();
+    return launch_dependent(attn_weights_kernel, dim3((unsigned)grid), AW_THREADS, aw_layout(p.T * p.group).total, stream, 1u, k_map, p);
 }
 
 }  // namespace mfc

@@ -90,6 +90,13 @@ __device__ __forceinline__ void fence_proxy_async() {
     asm volatile("fence.proxy.async;" ::: "memory");
 }
 
+// ---- programmatic dependent launch ----------------------------------------
+// A kernel launched with programmatic stream serialization may start while the kernel ahead of it drains; it calls
+// dependency_wait() before it touches any argument's memory, in every thread block, so that completion stays transitive.
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next such kernel start preparing itself; it waits for this one by itself.
+__device__ __forceinline__ void dependency_allow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- ldmatrix / mma.sync ----------------------------------------------
 __device__ __forceinline__ void ldmatrix_x4(uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3,
                                             uint32_t addr) {

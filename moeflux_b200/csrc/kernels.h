@@ -283,6 +283,29 @@ cudaError_t launch_dequant_matvec_4bit(MatvecBatch mb, const float *x, int in_di
                                        cudaStream_t stream, const MatvecMaps *maps = nullptr, int *grid_out = nullptr);
 
 // ---------------------------------------------------------------- serving a batch from cached rows
+// Launch of a kernel that waits for its predecessor by itself (dependency_wait); cluster > 1: that many CTAs per cluster.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                                    unsigned cluster, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster > 1) {
+        at[1].id = cudaLaunchAttributeClusterDimension;
+        at[1].val.clusterDim.x = cluster;
+        at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    cfg.attrs = at;
+    return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 struct VerifyParams {
     const float *p, *q;            // target and draft probabilities; q may be nullptr
     int64_t p_seq, p_row, q_seq, q_row;

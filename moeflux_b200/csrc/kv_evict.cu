@@ -108,6 +108,8 @@ __global__ void __launch_bounds__(EV_THREADS, 1) kv_evict_select_kernel(const Ev
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     for (int i = tid; i < 3 * EV_BINS / 4; i += EV_THREADS) (&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+    dependency_wait();
+    dependency_allow();
     int n = p.lens[b];
     const long long recent = (long long)p.next_pos[b] - p.n_recent;
     if (n < 0 || n > p.cap) {
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(EC_THREADS) kv_evict_copy_kernel(const EvictPa
     extern __shared__ int first[];  // [units + 1] first move of every unit
     __shared__ int s_warp[EC_THREADS / 32];
     const int units = p.B * p.Hkv, tid = threadIdx.x, lane = tid & 31;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the lists are written by the kernel before
+    dependency_wait();  // the lists are written by the kernel before
     const int per = (units + EC_THREADS - 1) / EC_THREADS;
     const int u0 = min(tid * per, units), u1 = min(u0 + per, units);
     int sum = 0, total;
@@ -369,32 +371,11 @@ cudaError_t launch_kv_evict(EvictParams p, int n_sms, cudaStream_t stream, int *
     while (cs < EV_MAX_CLUSTER && ((int64_t)units * cs * 2 <= n_sms || p.cap > cs * EV_MAX_ROWS_PER_CTA) && p.cap > cs * EV_MIN_ROWS) cs *= 2;
     p.fused = cs == 1 && p.cap <= EV_FUSED_ROWS;
     const int rows_cap = (p.cap + cs - 1) / cs;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * cs));
-    cfg.blockDim = dim3(EV_THREADS);
-    cfg.dynamicSmemBytes = (size_t)rows_cap * 4;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)cs;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kv_evict_select_kernel, p);
+    cudaError_t e = launch_dependent(kv_evict_select_kernel, dim3((unsigned)(units * cs)), EV_THREADS, (size_t)rows_cap * 4, stream, (unsigned)cs, p);
     if (e != cudaSuccess) return e;
     *launches = 1;
     if (p.fused) return cudaSuccess;
-    cudaLaunchConfig_t cc = {};
-    cc.gridDim = dim3((unsigned)(n_sms * 4));
-    cc.blockDim = dim3(EC_THREADS);
-    cc.dynamicSmemBytes = (size_t)(units + 1) * 4;
-    cc.stream = stream;
-    cudaLaunchAttribute pd[1];
-    pd[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    pd[0].val.programmaticStreamSerializationAllowed = 1;
-    cc.attrs = pd;
-    cc.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cc, kv_evict_copy_kernel, p);
+    e = launch_dependent(kv_evict_copy_kernel, dim3((unsigned)(n_sms * 4)), EC_THREADS, (size_t)(units + 1) * 4, stream, 1u, p);
     if (e == cudaSuccess) *launches = 2;
     return e;
 }

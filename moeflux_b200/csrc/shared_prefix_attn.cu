@@ -226,17 +226,24 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge kernel may prepare itself
-    if (warp == 0) {
+    if (warp == SP_SOFT) {
         tmem_alloc(tmem_slot, SP_TMEM_COLS);
         tmem_relinquish();
     }
-    if (warp == 1) {
+    if (warp == SP_SOFT + 1) {
+        if (lane == 20) {
+            prefetch_tmap(&pk_map);
+            prefetch_tmap(&pv_map);
+            prefetch_tmap(&ok_map);
+            prefetch_tmap(&ov_map);
+        }
         if (lane < 17) mbar_init(&bars[lane], (lane >= 11 && lane <= 13) || lane == 16 ? SP_SOFT : 1);
         if (lane == 17) *s_fail = 0;
         mbar_fence_init();
     }
     __syncwarp();
+    dependency_wait();
+    dependency_allow();
     // ---- every warp by itself: the plan, this CTA's runs, its first sequence ----
     const int own_cta = (int)gridDim.x - 1 - (int)blockIdx.x;
     Walk walk;
@@ -265,6 +272,34 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 first += p.Hkv * p.own_mtiles * own_tiles(p, b);
             }
         }
+    }
+    // Q of a segment: softmax warp w copies 16 rows, one 512-byte row per instruction, without registers in between; rows
+    // without a query are zero.  The copies are complete, for this thread, after q_landed().
+    const int tg = p.T * p.group;
+    auto request_q = [&](const Walk &w) {
+        const int rows = w.own ? min(SP_M, tg - w.mt * SP_M) : min(SP_M, p.B * tg - w.mt * SP_M);
+        int64_t off = 0;  // lane i: offset of row 16 * warp + i
+        const int r = 16 * warp + (lane & 15);
+        if (r < rows) {
+            const int idx = w.mt * SP_M + r;
+            const int bt = idx / p.group, hg = idx - bt * p.group;
+            const int b = w.own ? w.b : bt / p.T, t = w.own ? bt : bt - b * p.T;
+            off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(w.hk * p.group + hg) * p.q_head;
+        }
+        const uint32_t qb = smem_u32(smem + (lane >> 3) * SP_Q_BOX + 16 * warp * 128);
+#pragma unroll 4
+        for (int i = 0; i < 16; i++) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, i);
+            const uint32_t bytes = 16 * warp + i < rows ? 16u : 0u;  // 0: the 16 bytes are filled with zeros
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(qb + i * 128 + (((lane & 7) ^ (i & 7)) << 4)),
+                         "l"(p.q + o + 8 * lane), "r"(bytes)
+                         : "memory");
+        }
+    };
+    bool more = false;
+    if (warp < SP_SOFT) {  // the first segment's queries are on their way while the CTA sets itself up
+        more = walk.next(p);
+        if (more) request_q(walk);
     }
     tc_fence_before();
     __syncthreads();
@@ -406,7 +441,6 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         const uint32_t lane_base = tmem + ((uint32_t)(32 * quad) << 16);
         float *xm = reinterpret_cast<float *>(smem + SP_OFF_XM);  // [2 halves][128 rows] row maxima, row sums
         const float sl2 = p.scale * LOG2E_SP;
-        const int tg = p.T * p.group;
         auto warp_arrive = [&](uint64_t *bar) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
@@ -414,39 +448,13 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         auto give_up = [&]() {
             if (lane == 0) *s_fail = 1;
         };
-        // Q of a segment: this warp copies 16 rows, one 512-byte row per instruction, without registers in between; rows
-        // without a query are zero.  The copies are complete, for this thread, after q_landed().
-        auto request_q = [&](const Walk &w) {
-            const int rows = w.own ? min(SP_M, tg - w.mt * SP_M) : min(SP_M, p.B * tg - w.mt * SP_M);
-            int64_t off = 0;  // lane i: offset of row 16 * warp + i
-            const int r = 16 * warp + (lane & 15);
-            if (r < rows) {
-                const int idx = w.mt * SP_M + r;
-                const int bt = idx / p.group, hg = idx - bt * p.group;
-                const int b = w.own ? w.b : bt / p.T, t = w.own ? bt : bt - b * p.T;
-                off = (int64_t)b * p.q_seq + (int64_t)t * p.q_token + (int64_t)(w.hk * p.group + hg) * p.q_head;
-            }
-            const uint32_t qb = smem_u32(smem + (lane >> 3) * SP_Q_BOX + 16 * warp * 128);
-#pragma unroll 4
-            for (int i = 0; i < 16; i++) {
-                const int64_t o = __shfl_sync(0xffffffffu, off, i);
-                const uint32_t bytes = 16 * warp + i < rows ? 16u : 0u;  // 0: the 16 bytes are filled with zeros
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(qb + i * 128 + (((lane & 7) ^ (i & 7)) << 4)),
-                             "l"(p.q + o + 8 * lane), "r"(bytes)
-                             : "memory");
-            }
-        };
         auto q_landed = [&]() {
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async_smem();
             warp_arrive(q_ready);
         };
         unsigned n = 0;
-        bool more = walk.next(p);
-        if (more) {
-            request_q(walk);
-            q_landed();
-        }
+        if (more) q_landed();
         while (more) {
             const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
             // columns of the unit this row sees
@@ -608,7 +616,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     // on the ordinary path every granule has been used; after a failure the copies in flight land before the CTA leaves
     if (warp == SP_SOFT + 1 && lane == 0 && *s_fail)
         for (unsigned k = gi > SP_GRAN ? gi - SP_GRAN : 0; k < gi; k++) mbar_wait_bounded(&full[k % SP_GRAN], (k / SP_GRAN) & 1u, p.wait_spins);
-    if (warp == 0) tmem_dealloc(tmem, SP_TMEM_COLS);
+    if (warp == SP_SOFT) tmem_dealloc(tmem, SP_TMEM_COLS);
 }
 
 // Joins the partials of the query rows by log-sum-exp, in a fixed order, and applies the gate.  CTA = 32 consecutive
@@ -690,7 +698,7 @@ __global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const 
     const int rows_hk = p.B * p.T * p.group;
     const int blocks_hk = (rows_hk + 31) / 32;
     const int hk = blockIdx.x / blocks_hk, idx0 = (blockIdx.x - hk * blocks_hk) * 32;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan and the partials are written by the kernel before
+    dependency_wait();  // the plan and the partials are written by the kernel before
     RowParts parts = {0, 0, 0, 0, 0, 0};
     if (idx0 + lane < rows_hk) parts = row_parts(p, hk, idx0 + lane);
     if (FEW) {
@@ -783,8 +791,7 @@ cudaError_t shared_prefix_attn_configure() {
 cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &pv, const CUtensorMap &ok,
                                       const CUtensorMap &ov, const SharedAttnParams &p, cudaStream_t stream) {
     if (p.B <= 0) return cudaSuccess;
-    shared_prefix_attn_kernel<<<p.grid, SP_THREADS, SP_SMEM, stream>>>(pk, pv, ok, ov, p);
-    cudaError_t e = cudaGetLastError();
+    cudaError_t e = launch_dependent(shared_prefix_attn_kernel, dim3((unsigned)p.grid), SP_THREADS, SP_SMEM, stream, 1u, pk, pv, ok, ov, p);
     if (e != cudaSuccess) return e;
     // partials a row has at most, about: the CTAs a unit is spread over, of the prefix and of the own rows
     const int64_t units_p = (int64_t)p.Hkv * p.prefix_mtiles, units_o = (int64_t)p.B * p.Hkv * p.own_mtiles;
@@ -792,16 +799,9 @@ cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &
     // (with few rows the other form spreads them over more SMs: 64 rows of five partials take 6 us less)
     const int64_t blocks = (int64_t)p.Hkv * ((p.B * p.T * p.group + 31) / 32);
     const bool few = (np < p.prefix_tiles ? np : p.prefix_tiles) + (no < own_t ? no : own_t) <= MG_FEW && blocks >= MG_FEW_BLOCKS;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks, few ? 1 : HEAD_DIM / MG_DIMS);
-    cfg.blockDim = dim3(32 * MG_WARPS);
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return few ? cudaLaunchKernelEx(&cfg, shared_attn_merge_kernel<true>, p) : cudaLaunchKernelEx(&cfg, shared_attn_merge_kernel<false>, p);
+    const dim3 grid((unsigned)blocks, few ? 1 : HEAD_DIM / MG_DIMS);
+    return few ? launch_dependent(shared_attn_merge_kernel<true>, grid, 32 * MG_WARPS, 0, stream, 1u, p)
+               : launch_dependent(shared_attn_merge_kernel<false>, grid, 32 * MG_WARPS, 0, stream, 1u, p);
 }
 
 }  // namespace mfc

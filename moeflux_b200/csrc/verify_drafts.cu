@@ -12,6 +12,8 @@
 // the one that owns it re-reads the 1024 entries of that segment (from L2).  Order of all sums fixed by the sizes.
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -112,6 +114,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
     __shared__ double s_tot[2];  // this CTA's total, for the first pass and for the pass over p alone
     __shared__ int s_n;
 
+    dependency_wait();
+    dependency_allow();
+    const float u = p.u_sample[b];  // needed at the end: asked for now
     const int len = p.draft_lens ? min(p.draft_lens[b], p.K) : p.K;
     if (warp == 0) {
         bool refused = false;
@@ -171,8 +176,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
         qrow = nullptr;  // the residual is zero everywhere: draw from p
         x = -1;
     }
+    auto read = cluster.barrier_arrive();  // this CTA has read what it needs of its peers' memory
     // a uniform outside [0, 1) counts as the nearest end, so that the border lies in exactly one run
-    const double target = fmin(fmax((double)p.u_sample[b], 0.0), 1.0 - 1.0 / (1ll << 50)) * total;
+    const double target = fmin(fmax((double)u, 0.0), 1.0 - 1.0 / (1ll << 50)) * total;
     int *tok = p.tokens + (size_t)b * (p.K + 1) + n;
     if (warp == 0 && s1 > s0 && total > 0.0) {
         // the border lies in this CTA's run when the sum before the run does not exceed the target and the sum behind
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
             if (lane == 0) *tok = first != 0x7fffffff ? first : fin;
         }
     }
-    cluster.sync();  // a CTA's shared memory stays until its peers have read it
+    cluster.barrier_wait(std::move(read));  // a CTA's shared memory stays until its peers have read it
 }
 
 }  // namespace
@@ -271,17 +277,7 @@ cudaError_t launch_verify_drafts(const VerifyParams &p, int n_sms, cudaStream_t 
     while (cs < VD_MAX_CLUSTER && (int64_t)p.B * cs * 2 <= 7 * n_sms && (int64_t)p.V > (int64_t)cs * 2 * VD_SEG) cs *= 2;
     int64_t seg = VD_SEG;  // longer segments where a run would not fit the table of sums
     while ((p.V + seg - 1) / seg > (int64_t)cs * VD_MAX_SEGS) seg *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.B * cs));
-    cfg.blockDim = dim3(VD_THREADS);
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)cs;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, verify_drafts_kernel, p, (int)seg);
+    return launch_dependent(verify_drafts_kernel, dim3((unsigned)(p.B * cs)), VD_THREADS, 0, stream, (unsigned)cs, p, (int)seg);
 }
 
 }  // namespace mfc
