@@ -7,7 +7,7 @@
 // entries is about 10^-5 of the total; fp32 prefix sums would move the border by a hundredth of a step).
 //
 // HBM-bound: of the K+1 rows of a sequence only the refused one of p and q is read, once.  A cluster of CTAs owns a
-// sequence, each a run of `segments` of 1024 entries; a warp sums a segment and keeps the sum in shared memory; the CTAs
+// sequence, each a run of segments of 128 to 1024 entries; a warp sums a segment and keeps the sum in shared memory; the CTAs
 // exchange their totals through distributed shared memory, every CTA finds out whether the border lies in its run, and
 // the one that owns it re-reads the 1024 entries of that segment (from L2).  Order of all sums fixed by the sizes.
 #include <cooperative_groups.h>
@@ -23,11 +23,10 @@ namespace mfc {
 
 namespace {
 
-constexpr int VD_THREADS = 128;
-constexpr int VD_WARPS = VD_THREADS / 32;
-constexpr int VD_SEG = 1024;     // entries of a segment
+constexpr int VD_MAX_THREADS = 512;
+constexpr int VD_MIN_SEG = 128, VD_SEG = 1024;  // entries of a segment: at least, and at most unless the row is very long
 constexpr int VD_MAX_SEGS = 512;  // segments of a CTA's run kept in shared memory; longer runs use longer segments
-constexpr int VD_MAX_CLUSTER = 16;
+constexpr int VD_MAX_CLUSTER = 8;
 
 __device__ __forceinline__ double weight(float p, float q) {
     const double w = (double)p - (double)q;
@@ -41,14 +40,34 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 }
 
 // inclusive prefix sum over the lanes
-__device__ __forceinline__ double warp_scan_f64(double v) {
+__device__ __noinline__ double warp_scan_f64(double v) {
     const int lane = threadIdx.x & 31;
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
         const double up = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += up;
     }
     return v;
+}
+
+// Where the cumulative sum of the lanes' values, from c on, first exceeds the target: the lane (else the last lane with a
+// positive value, else -1), whether it exceeds there, the sum ahead of that lane and the sum behind all of them.  One copy
+// of this code serves the three levels of the search: it runs once per sequence, so what it takes is the fetching of its
+// instructions (unrolled, with 128 entries a step, the search took 8.5 thousand cycles).
+struct Found {
+    int lane;
+    bool over;
+    double ahead, behind;
+};
+__device__ __noinline__ Found locate(double v, double c, double target) {
+    const double run = warp_scan_f64(v);
+    const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && c + run > target), any = __ballot_sync(0xffffffffu, v > 0.0);
+    Found f;
+    f.lane = over ? __ffs(over) - 1 : (any ? 31 - __clz(any) : -1);
+    f.over = over != 0;
+    f.ahead = c + __shfl_sync(0xffffffffu, run - v, f.lane < 0 ? 0 : f.lane);
+    f.behind = c + __shfl_sync(0xffffffffu, run, 31);
+    return f;
 }
 
 // entries [v, v + 4) of the row's weights; x: the drafted token whose q is 1 when there are no draft probabilities
@@ -77,24 +96,36 @@ __device__ __forceinline__ void load_w4(const float *p, const float *q, int x, i
 template <bool VEC>
 __device__ __forceinline__ void sum_segments(const float *p, const float *q, int x, int V, int seg, int s0, int s1, double *s_sum) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int s = s0 + warp; s < s1; s += VD_WARPS) {
+    for (int s = s0 + warp; s < s1; s += (int)blockDim.x / 32) {
         const int v1 = min((s + 1) * seg, V);
         double acc = 0.0;
         int v0 = s * seg;
-        if (VEC && x < 0) {  // whole steps of 512 entries: eight loads of a lane in flight
-            for (; v0 + 512 <= v1; v0 += 512) {
+        // whole steps of 512 entries that do not hold the drafted token: a lane's loads of a step are in flight together
+        for (; v0 + 512 <= v1 && (x < v0 || x >= v0 + 512); v0 += 512) {
+            double t[4];
+            if (VEC) {
                 float4 a[4], b[4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) a[u] = *reinterpret_cast<const float4 *>(p + v0 + 4 * lane + 128 * u);
 #pragma unroll
                 for (int u = 0; u < 4; u++) b[u] = q ? *reinterpret_cast<const float4 *>(q + v0 + 4 * lane + 128 * u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                double t[4];
 #pragma unroll
                 for (int u = 0; u < 4; u++)
                     t[u] = (weight(a[u].x, b[u].x) + weight(a[u].y, b[u].y)) + (weight(a[u].z, b[u].z) + weight(a[u].w, b[u].w));
-                acc += (t[0] + t[1]) + (t[2] + t[3]);
+            } else {  // rows that start anywhere: 32 consecutive entries a load
+                float a[16], b[16];
+#pragma unroll
+                for (int u = 0; u < 16; u++) a[u] = p[v0 + 32 * u + lane];
+#pragma unroll
+                for (int u = 0; u < 16; u++) b[u] = q ? q[v0 + 32 * u + lane] : 0.0f;
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    t[u] = (weight(a[4 * u], b[4 * u]) + weight(a[4 * u + 1], b[4 * u + 1])) +
+                           (weight(a[4 * u + 2], b[4 * u + 2]) + weight(a[4 * u + 3], b[4 * u + 3]));
             }
+            acc += (t[0] + t[1]) + (t[2] + t[3]);
         }
+#pragma unroll 4
         for (int v = v0 + 4 * lane; v < v1; v += 128) {
             double w[4];
             load_w4<VEC>(p, q, x, v, V, w);
@@ -105,13 +136,14 @@ __device__ __forceinline__ void sum_segments(const float *p, const float *q, int
     }
 }
 
-__global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyParams p, int seg) {
+__global__ void __launch_bounds__(VD_MAX_THREADS) verify_drafts_kernel(const VerifyParams p, int seg) {
     cg::cluster_group cluster = cg::this_cluster();
     const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int b = (int)blockIdx.x / cs;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     __shared__ double s_sum[VD_MAX_SEGS];
     __shared__ double s_tot[2];  // this CTA's total, for the first pass and for the pass over p alone
+    __shared__ double s_part[VD_MAX_THREADS / 32];
     __shared__ int s_n;
 
     dependency_wait();
@@ -151,7 +183,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
     const int n_segs = (p.V + seg - 1) / seg, per = (n_segs + cs - 1) / cs;
     const int s0 = min(rank * per, n_segs), s1 = min(s0 + per, n_segs);
 
-    double total = 0.0, before = 0.0, mine = 0.0;
+    double total = 0.0, before = 0.0, behind = 0.0;
     for (int pass = 0; pass < 2; pass++) {
         if (vec) sum_segments<true>(prow, qrow, x, p.V, seg, s0, s1, s_sum);
         else sum_segments<false>(prow, qrow, x, p.V, seg, s0, s1, s_sum);
@@ -163,15 +195,12 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
             if (lane == 0) s_tot[pass] = t;
         }
         cluster.sync();
-        total = before = 0.0;
-        for (int r = 0; r < cs; r++) {
-            const double t = *cluster.map_shared_rank(&s_tot[pass], r);
-            if (r == rank) {
-                before = total;
-                mine = t;
-            }
-            total += t;
-        }
+        // every warp by itself, in the same order: the sum before this CTA's run, behind it, and behind all runs
+        const double t = lane < cs ? *cluster.map_shared_rank(&s_tot[pass], lane) : 0.0;
+        const double run = warp_scan_f64(t);
+        behind = __shfl_sync(0xffffffffu, run, rank);
+        before = rank > 0 ? __shfl_sync(0xffffffffu, run, rank - 1) : 0.0;
+        total = __shfl_sync(0xffffffffu, run, 31);
         if (total > 0.0 || (!qrow && x < 0)) break;
         qrow = nullptr;  // the residual is zero everywhere: draw from p
         x = -1;
@@ -180,84 +209,61 @@ __global__ void __launch_bounds__(VD_THREADS) verify_drafts_kernel(const VerifyP
     // a uniform outside [0, 1) counts as the nearest end, so that the border lies in exactly one run
     const double target = fmin(fmax((double)u, 0.0), 1.0 - 1.0 / (1ll << 50)) * total;
     int *tok = p.tokens + (size_t)b * (p.K + 1) + n;
-    if (warp == 0 && s1 > s0 && total > 0.0) {
-        // the border lies in this CTA's run when the sum before the run does not exceed the target and the sum behind
-        // it does; the additions are those every CTA makes, so exactly one run qualifies
-        const bool here = before <= target && before + mine > target;
-        if (here) {
-            // Three levels, each a sum over lanes: the segment, the step of 128 entries in it, the entry.  Sums of the same
-            // entries in two orders may differ in the last bit; where a level then finds no place, its last one counts.
-            // (Entries without weight are never the last one.)
+    if (s1 > s0 && total > 0.0) {
+        // the border lies in this CTA's run when the sum before the run does not exceed the target and the sum behind it
+        // does; all CTAs compare the same sums, so exactly one run qualifies
+        if (before <= target && behind > target) {
+            // Four levels: the segment, a warp's part of it, a lane's, the entry.  Sums of the same entries in two orders may
+            // differ in the last bit; where a level then finds no place, its last entry of any weight counts.  The first
+            // two levels run in every warp alike.
             double c = before, c_last = before;
             int s = -1, s_last = s0;
+#pragma unroll 1
             for (int k0 = s0; k0 < s1 && s < 0; k0 += 32) {
-                const double v = k0 + lane < s1 ? s_sum[k0 + lane - s0] : 0.0;
-                const double run = warp_scan_f64(v);
-                const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && c + run > target), any = __ballot_sync(0xffffffffu, v > 0.0);
-                const int l = over ? __ffs(over) - 1 : (any ? 31 - __clz(any) : -1);
-                if (l >= 0) {
-                    const double ahead = c + __shfl_sync(0xffffffffu, run - v, l);
-                    if (over) {
-                        s = k0 + l;
-                        c = ahead;
-                        break;
-                    }
-                    s_last = k0 + l;
-                    c_last = ahead;
+                const Found f = locate(k0 + lane < s1 ? s_sum[k0 + lane - s0] : 0.0, c, target);
+                if (f.lane >= 0) {
+                    s_last = k0 + f.lane;
+                    c_last = f.ahead;
+                    if (f.over) s = s_last;
                 }
-                c += __shfl_sync(0xffffffffu, run, 31);
+                c = f.behind;
             }
-            if (s < 0) {
-                s = s_last;
-                c = c_last;
-            }
-            auto load4 = [&](int v, double (&w)[4]) {
-                if (vec) load_w4<true>(prow, qrow, x, v, p.V, w);
-                else load_w4<false>(prow, qrow, x, v, p.V, w);
-            };
-            const int v1 = min((s + 1) * seg, p.V);
-            int step = -1, step_last = s * seg;
-            c_last = c;
-            for (int v0 = s * seg; v0 < v1 && step < 0; v0 += 8 * 128) {
-                double part[8];
-#pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    double w[4] = {0.0, 0.0, 0.0, 0.0};
-                    if (v0 + 128 * u < v1) load4(v0 + 128 * u + 4 * lane, w);
-                    part[u] = (w[0] + w[1]) + (w[2] + w[3]);
+            // warps that share the segment (a short one is left to the first), a lane's entries
+            const int parts = seg <= 512 ? 1 : min((int)blockDim.x / 32, seg / 128), per = seg / (32 * parts);
+            const int v0 = s_last * seg + (warp * 32 + lane) * per;
+            double mine = 0.0;
+            if (warp < parts)
+#pragma unroll 2
+                for (int k = 0; k < per; k += 4) {
+                    double w[4];
+                    if (vec) load_w4<true>(prow, qrow, x, v0 + k, p.V, w);
+                    else load_w4<false>(prow, qrow, x, v0 + k, p.V, w);
+                    mine += (w[0] + w[1]) + (w[2] + w[3]);
                 }
-#pragma unroll
-                for (int u = 0; u < 8; u++) part[u] = warp_sum_f64(part[u]);
-#pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    if (step >= 0 || !(part[u] > 0.0)) continue;
-                    if (c + part[u] > target) {
-                        step = v0 + 128 * u;
-                    } else {
-                        step_last = v0 + 128 * u;
-                        c_last = c;
-                        c += part[u];
-                    }
+            int owner = 0;
+            if (parts > 1) {
+                const double sum = warp_sum_f64(mine);
+                if (lane == 0) s_part[warp] = sum;
+                __syncthreads();
+                const Found wf = locate(lane < parts ? s_part[lane] : 0.0, c_last, target);
+                owner = max(wf.lane, 0);
+                c_last = wf.ahead;
+            }
+            if (warp == owner) {
+                const Found lf = locate(mine, c_last, target);
+                const int from = __shfl_sync(0xffffffffu, v0, max(lf.lane, 0));
+                int found = -1;
+                c = lf.ahead;
+#pragma unroll 1
+                for (int k = 0; k < per; k += 32) {
+                    const int v = from + k + lane;
+                    const Found f = locate(k + lane < per && v < p.V && v != x ? weight(prow[v], qrow ? qrow[v] : 0.0f) : 0.0, c, target);
+                    if (f.lane >= 0) found = from + k + f.lane;
+                    if (f.over) break;
+                    c = f.behind;
                 }
+                if (lane == 0) *tok = found;
             }
-            if (step < 0) {
-                step = step_last;
-                c = c_last;
-            }
-            double w[4];
-            load4(step + 4 * lane, w);
-            const double i0 = w[0], i1 = i0 + w[1], i2 = i1 + w[2], i3 = i2 + w[3];
-            const double lead = c + (warp_scan_f64(i3) - i3);
-            int at = 0x7fffffff, end = -1;
-            if (w[3] > 0.0 && lead + i3 > target) at = step + 4 * lane + 3;
-            if (w[2] > 0.0 && lead + i2 > target) at = step + 4 * lane + 2;
-            if (w[1] > 0.0 && lead + i1 > target) at = step + 4 * lane + 1;
-            if (w[0] > 0.0 && lead + i0 > target) at = step + 4 * lane;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (w[e] > 0.0) end = step + 4 * lane + e;
-            const int first = __reduce_min_sync(0xffffffffu, at), fin = __reduce_max_sync(0xffffffffu, end);
-            if (lane == 0) *tok = first != 0x7fffffff ? first : fin;
         }
     }
     cluster.barrier_wait(std::move(read));  // a CTA's shared memory stays until its peers have read it
@@ -271,13 +277,17 @@ cudaError_t verify_drafts_configure() {
 
 cudaError_t launch_verify_drafts(const VerifyParams &p, int n_sms, cudaStream_t stream) {
     if (p.B <= 0) return cudaSuccess;
-    // As many CTAs per sequence as are resident at once (seven a SM), but at least two segments each.  128 sequences of
-    // 131072 entries: 134, 74, 46, 32, 38 us with 1, 2, 4, 8, 16.
+    // Up to eight CTAs per sequence, of 512, 256 or 128 threads: about a thousand threads per SM in one wave (128 sequences
+    // of 131072 entries, 128 threads: 134, 74, 46, 32, 38 us with 1, 2, 4, 8, 16 CTAs).  A segment per warp where that
+    // makes segments of at most VD_SEG entries.
     int cs = 1;
-    while (cs < VD_MAX_CLUSTER && (int64_t)p.B * cs * 2 <= 7 * n_sms && (int64_t)p.V > (int64_t)cs * 2 * VD_SEG) cs *= 2;
-    int64_t seg = VD_SEG;  // longer segments where a run would not fit the table of sums
+    while (cs < VD_MAX_CLUSTER && (int64_t)p.B * cs * 2 <= 7 * n_sms && (int64_t)p.V > (int64_t)cs * 8 * VD_MIN_SEG) cs *= 2;
+    int threads = VD_MAX_THREADS;
+    while (threads > 128 && ((int64_t)p.B * cs * threads > (int64_t)n_sms * 1024 || (int64_t)cs * threads * 4 > p.V)) threads /= 2;
+    int64_t seg = VD_MIN_SEG;
+    while (seg < VD_SEG && (int64_t)cs * (threads / 32) * seg < p.V) seg *= 2;
     while ((p.V + seg - 1) / seg > (int64_t)cs * VD_MAX_SEGS) seg *= 2;
-    return launch_dependent(verify_drafts_kernel, dim3((unsigned)(p.B * cs)), VD_THREADS, 0, stream, (unsigned)cs, p, (int)seg);
+    return launch_dependent(verify_drafts_kernel, dim3((unsigned)(p.B * cs)), (unsigned)threads, 0, stream, (unsigned)cs, p, (int)seg);
 }
 
 }  // namespace mfc

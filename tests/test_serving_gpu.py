@@ -446,7 +446,8 @@ def call_verify(ctx, p, q, x, lens, ua, us):
 
 @pytest.mark.parametrize("B,K,V,sampled,pad", [
     (1, 1, 1, True, 0), (1, 0, 10, True, 0), (3, 4, 7, True, 0), (2, 4, 1000, False, 0), (9, 8, 4099, True, 1), (64, 3, 1025, True, 3),
-    (1, 5, 131072, True, 0), (200, 2, 2048, False, 0), (2, 32, 50001, True, 0), (1, 1, 1200003, True, 0)])
+    (1, 5, 131072, True, 0), (200, 2, 2048, False, 0), (2, 32, 50001, True, 0), (1, 1, 1200003, True, 0), (24, 4, 40007, False, 0),
+    (44, 8, 20011, True, 0), (3, 2, 300, False, 2), (150, 1, 7000, True, 0)])
 def test_verify_drafts(ctx, B, K, V, sampled, pad):
     g = gen(B + K + V)
     logits = torch.randn(B, K + 1, V + pad, generator=g, device="cuda") * 2
