@@ -664,27 +664,41 @@ __device__ __forceinline__ void join_parts(const SharedAttnParams &p, const RowP
     j.L = 0.0f;
 #pragma unroll
     for (int i = 0; i < MG_DIMS / 4; i++) j.acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c = from; c < r.np + r.no; c += step) {
+    struct Part {
+        float4 o[MG_DIMS / 4];
+        float m, l;
+    };
+    auto load = [&](int c, Part &q) {
         const bool pre = c < r.np;
         const int srows = pre ? SP_M : p.own_rows, row = pre ? r.pr : r.orow;
         const size_t row0 = pre ? r.p0 + (size_t)c * SP_M : r.o0 + (size_t)(c - r.np) * p.own_rows;
         const float4 *src = reinterpret_cast<const float4 *>(p.part_o + row0 * HEAD_DIM) + row;
-        float4 o[MG_DIMS / 4];
 #pragma unroll
-        for (int i = 0; i < MG_DIMS / 4; i++) o[i] = src[(size_t)(d0 / 4 + i) * srows];
-        const float m = p.part_m[row0 + row], l = p.part_l[row0 + row];
-        if (m == -INFINITY) continue;  // no weight: contributes nothing, whatever it holds
-        const float mn = fmaxf(j.M, m);
-        const float wa = j.M == -INFINITY ? 0.0f : ex2_approx(j.M - mn), wb = ex2_approx(m - mn);
+        for (int i = 0; i < MG_DIMS / 4; i++) q.o[i] = src[(size_t)(d0 / 4 + i) * srows];
+        q.m = p.part_m[row0 + row];
+        q.l = p.part_l[row0 + row];
+    };
+    auto fold = [&](const Part &q) {
+        if (q.m == -INFINITY) return;  // no weight: contributes nothing, whatever it holds
+        const float mn = fmaxf(j.M, q.m);
+        const float wa = j.M == -INFINITY ? 0.0f : ex2_approx(j.M - mn), wb = ex2_approx(q.m - mn);
         j.M = mn;
-        j.L = j.L * wa + l * wb;
+        j.L = j.L * wa + q.l * wb;
 #pragma unroll
         for (int i = 0; i < MG_DIMS / 4; i++) {
-            j.acc[i].x = fmaf(wb, o[i].x, j.acc[i].x * wa);
-            j.acc[i].y = fmaf(wb, o[i].y, j.acc[i].y * wa);
-            j.acc[i].z = fmaf(wb, o[i].z, j.acc[i].z * wa);
-            j.acc[i].w = fmaf(wb, o[i].w, j.acc[i].w * wa);
+            j.acc[i].x = fmaf(wb, q.o[i].x, j.acc[i].x * wa);
+            j.acc[i].y = fmaf(wb, q.o[i].y, j.acc[i].y * wa);
+            j.acc[i].z = fmaf(wb, q.o[i].z, j.acc[i].z * wa);
+            j.acc[i].w = fmaf(wb, q.o[i].w, j.acc[i].w * wa);
         }
+    };
+    const int n = r.np + r.no;
+    for (int c = from; c < n; c += 2 * step) {  // two partials in flight
+        Part a, b;
+        load(c, a);
+        if (c + step < n) load(c + step, b);
+        fold(a);
+        if (c + step < n) fold(b);
     }
 }
 __device__ __forceinline__ float2 gate2(uint32_t bits) {
