@@ -1571,33 +1571,15 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
     }
     SharedAttnParams p;
     memset(&p, 0, sizeof(p));
-    p.B = a->n_seqs;
     p.T = a->n_tokens;
     p.H = a->num_attn_heads;
     p.Hkv = a->num_kv_heads;
     p.group = p.H / p.Hkv;
     p.prefix_len = a->prefix_len;
     p.own_cap = a->own_cap;
-    p.prefix_tiles = (a->prefix_len + SHARED_ATTN_N - 1) / SHARED_ATTN_N;
-    p.prefix_mtiles = (int)(((int64_t)p.B * p.T * p.group + SHARED_ATTN_M - 1) / SHARED_ATTN_M);
+    p.prefix_tiles = (int)(((int64_t)a->prefix_len + SHARED_ATTN_N - 1) / SHARED_ATTN_N);
     p.own_mtiles = (p.T * p.group + SHARED_ATTN_M - 1) / SHARED_ATTN_M;
     p.own_rows = p.T * p.group < SHARED_ATTN_M ? p.T * p.group : SHARED_ATTN_M;
-    const int64_t own_units = (int64_t)p.B * p.Hkv * p.own_mtiles;
-    const int64_t own_tiles = own_units * ((a->own_cap + SHARED_ATTN_N - 1) / SHARED_ATTN_N);
-    const int64_t tiles = (int64_t)p.Hkv * p.prefix_mtiles * p.prefix_tiles + own_tiles;
-    if (tiles >= ((int64_t)1 << 30)) {
-        fail(c, "too many rows and queries in one call");
-        return -1;
-    }
-    p.grid = tiles < c->n_sms ? (int)tiles : c->n_sms;
-    if (p.grid < 1) p.grid = 1;
-    // one slot per (unit, CTA) pair at most: units + CTAs of each kind
-    const int64_t need = ((int64_t)p.Hkv * p.prefix_mtiles + p.grid) * SHARED_ATTN_M + (own_units + p.grid) * p.own_rows;
-    if (need > (int64_t)c->max_parts * 16) {
-        fail(c, "n_seqs * n_tokens * num_attn_heads needs " + std::to_string(need) + " partial rows, the scratch reserved at open holds " +
-                    std::to_string((int64_t)c->max_parts * 16));
-        return -1;
-    }
     p.q = (const __nv_bfloat16 *)a->q;
     p.q_seq = a->q_seq_stride;
     p.q_token = a->q_token_stride;
@@ -1617,17 +1599,48 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
     p.scale = a->softmax_scale;
     p.wait_spins = c->gqa_wait_spins ? c->gqa_wait_spins : 1u << 22;
     p.inject_lost_load = c->gqa_inject_lost_load;
+    // sequences per launch: as many as the scratch holds partials for, one slot per (unit, CTA) pair at most
+    auto plan = [&](int n) -> bool {
+        p.B = n;
+        p.prefix_mtiles = (int)(((int64_t)n * p.T * p.group + SHARED_ATTN_M - 1) / SHARED_ATTN_M);
+        const int64_t own_units = (int64_t)n * p.Hkv * p.own_mtiles;
+        const int64_t tiles = (int64_t)p.Hkv * p.prefix_mtiles * p.prefix_tiles +
+                              own_units * (((int64_t)a->own_cap + SHARED_ATTN_N - 1) / SHARED_ATTN_N);
+        p.grid = tiles < 1 ? 1 : (tiles < c->n_sms ? (int)tiles : c->n_sms);
+        const int64_t need = ((int64_t)p.Hkv * p.prefix_mtiles + p.grid) * SHARED_ATTN_M + (own_units + p.grid) * p.own_rows;
+        return need <= (int64_t)c->max_parts * 16 && tiles < ((int64_t)1 << 30);
+    };
+    int per_launch = a->n_seqs;
+    while (!plan(per_launch)) {
+        if (per_launch == 1) {
+            fail(c, "too many rows and heads: the partials of one sequence exceed the scratch reserved at open, or its tiles 2^30");
+            return -1;
+        }
+        per_launch = (per_launch + 1) / 2;
+    }
     CUtensorMap m[4];
     memset(m, 0, sizeof(m));
     if (has_prefix && (!make_rows_map(c, &m[0], a->prefix_k, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 2, 128) ||
                        !make_rows_map(c, &m[1], a->prefix_v, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 4, 64)))
         return -1;
-    if (has_own && (!make_rows_map(c, &m[2], a->own_k, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 2, 128) ||
-                    !make_rows_map(c, &m[3], a->own_v, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, p.B, a->own_seq_stride, 4, 64)))
-        return -1;
     DeviceScope dev(c->cfg.device);
-    CK(launch_shared_prefix_attn(m[0], m[1], m[2], m[3], p, c->stream));
-    c->launches += 2;
+    const int64_t rows = (int64_t)p.T * p.H;
+    for (int b0 = 0; b0 < a->n_seqs; b0 += per_launch) {
+        const int n = a->n_seqs - b0 < per_launch ? a->n_seqs - b0 : per_launch;
+        const int64_t off = (int64_t)b0 * a->own_seq_stride * 2;  // bytes
+        if (has_own && (!make_rows_map(c, &m[2], (const uint8_t *)a->own_k + off, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, n, a->own_seq_stride, 2, 128) ||
+                        !make_rows_map(c, &m[3], (const uint8_t *)a->own_v + off, a->own_cap, a->own_row_stride, p.Hkv, a->own_head_stride, n, a->own_seq_stride, 4, 64)))
+            return -1;
+        plan(n);
+        SharedAttnParams q = p;
+        q.q += (int64_t)b0 * p.q_seq;
+        if (q.gate) q.gate += (int64_t)b0 * p.g_seq;
+        q.lens += b0;
+        q.out += (int64_t)b0 * rows * HEAD_DIM;
+        if (q.lse) q.lse += (int64_t)b0 * rows;
+        CK(launch_shared_prefix_attn(m[0], m[1], m[2], m[3], q, c->stream));
+        c->launches += 2;
+    }
     return 0;
 } catch (...) {
     return -1;

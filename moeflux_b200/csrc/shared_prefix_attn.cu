@@ -459,7 +459,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             const int rows = walk.own ? min(SP_M, tg - walk.mt * SP_M) : min(SP_M, p.B * tg - walk.mt * SP_M);
             // columns of the unit this row sees
             int lim = walk.len;
-            if (walk.own) lim = walk.len - (p.T - 1 - (walk.mt * SP_M + row) / p.group);
+            if (walk.own) lim = row < rows ? walk.len - (p.T - 1 - (walk.mt * SP_M + row) / p.group) : 0;
             const int safe = walk.own ? walk.len - (p.T - 1) : walk.len;  // columns that every row sees
             const bool live = 32 * quad < rows;                           // some row of this quadrant carries a query
             float m_run = -INFINITY, l_run = 0.0f;  // m_run: reference of the row's exponents; l_run: this thread's half

@@ -169,7 +169,10 @@ def test_shared_prefix_attn_ignores_what_lies_behind_the_lengths(ctx):
         ok[b, :, n:] = float("nan")
         ov[b, :, n:] = float("nan")
         ov[b, :, n : n + 3] = float("inf")
-    check_attn(ctx, q, None, pk, pv, ok, ov, lens)
+    out, lse = check_attn(ctx, q, None, pk, pv, ok, ov, lens)
+    used = torch.arange(cap, device="cuda").view(1, 1, cap, 1) < lens.view(B, 1, 1, 1)
+    out0, lse0 = check_attn(ctx, q, None, pk, pv, torch.where(used, ok, 0.0), torch.where(used, ov, 0.0), lens)
+    assert torch.equal(out, out0) and torch.equal(lse, lse0)  # not even in the last bit
 
 
 def test_shared_prefix_attn_strided(ctx):
@@ -647,3 +650,157 @@ def test_refusals(ctx, M):
         fn(**{**base, "n_seqs": 0})  # an empty batch is no error and no launch
     assert ctx.launch_count == before
     ctx.synchronize()
+
+
+def test_a_captured_step_of_all_four(ctx, M):
+    """One graph of the four calls, replayed on changed inputs, against the same calls made directly."""
+    g = gen(41)
+    B, T, H, Hkv, P, cap, budget, V = 6, 3, 32, 2, 400, 200, 90, 3001
+    q, gate = rn(g, B, T, H, D), rn(g, B, T, H, D)
+    pk, pv, ok, ov = rn(g, Hkv, P, D), rn(g, Hkv, P, D), rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    w, pos = torch.rand(B, Hkv, cap, generator=g, device="cuda"), torch.arange(cap, device="cuda", dtype=torch.int32).expand(B, Hkv, cap).contiguous()
+    lens = lens_for(g, B, T, cap)
+    nxt, new = lens.clone(), torch.zeros_like(lens)
+    p = torch.softmax(torch.randn(B, T, V, generator=g, device="cuda"), -1)
+    qd = torch.softmax(torch.randn(B, T - 1, V, generator=g, device="cuda"), -1)
+    x = torch.randint(0, V, (B, T - 1), generator=g, device="cuda", dtype=torch.int32)
+    ua, us = torch.rand(B, T - 1, generator=g, device="cuda"), torch.rand(B, generator=g, device="cuda")
+    out, lse = torch.zeros(B, T, H, D, device="cuda", dtype=torch.bfloat16), torch.zeros(B, T, H, device="cuda")
+    n, tok = torch.zeros(B, device="cuda", dtype=torch.int32), torch.zeros(B, T, device="cuda", dtype=torch.int32)
+    state = [ok, ov, w, pos]
+    start = [t.clone() for t in state]
+
+    def step():
+        ctx.shared_prefix_attn_dev(**attn_args(q, gate, pk, pv, ok, ov, lens, out, lse))
+        ctx.attn_weights_accumulate_dev(**weights_args(q, ok, lens, lse, w, 0.9))
+        ctx.verify_drafts_dev(n_seqs=B, max_drafts=T - 1, vocab=V, target_probs=p.data_ptr(), target_seq_stride=p.stride(0),
+                              target_row_stride=V, draft_probs=qd.data_ptr(), draft_seq_stride=qd.stride(0), draft_row_stride=V,
+                              draft_tokens=x.data_ptr(), u_accept=ua.data_ptr(), u_sample=us.data_ptr(), n_accepted=n.data_ptr(),
+                              tokens=tok.data_ptr())
+        ctx.kv_evict_dev(n_seqs=B, num_kv_heads=Hkv, kv_dtype=M.KV_BF16, cap=cap, k=ok.data_ptr(), v=ov.data_ptr(), seq_stride=ok.stride(0),
+                         head_stride=ok.stride(1), row_stride=D, budget=budget, n_sink=2, n_recent=5, lens=lens.data_ptr(),
+                         next_pos=nxt.data_ptr(), weights=w.data_ptr(), positions=pos.data_ptr(), map_seq_stride=w.stride(0),
+                         map_head_stride=w.stride(1), weights_out=w.data_ptr(), positions_out=pos.data_ptr(), lens_out=new.data_ptr())
+
+    home, side = torch.cuda.current_stream().cuda_stream, torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ctx.set_stream(side.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+        step()  # (the second finds nothing to evict where the lengths still say so: it runs all the same)
+    ctx.set_stream(home)
+    for turn in range(3):
+        q.copy_(rn(g, B, T, H, D))
+        us.copy_(torch.rand(B, generator=g, device="cuda"))
+        results = []
+        for way in ("direct", "graph"):
+            for t, s in zip(state, start):
+                t.copy_(s)
+            torch.cuda.synchronize()
+            if way == "direct":
+                step()
+                step()
+                ctx.synchronize()
+            else:
+                graph.replay()
+                torch.cuda.synchronize()
+            results.append([t.clone() for t in (*state, out, lse, n, tok, new)])
+        for a, b in zip(*results):
+            assert torch.equal(a, b), turn
+
+
+def test_offsets_beyond_32_bits(ctx, M):
+    """A cache of more than 2^31 elements, its rows in use in the last place only: every call reaches them."""
+    g = gen(43)
+    B, Hkv, cap, H, T = 36, 2, 131072, 16, 1
+    ok, ov = (torch.zeros(B, Hkv, cap, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    assert ok.numel() > 2 ** 31
+    ok[-1], ov[-1] = rn(g, Hkv, cap, D), rn(g, Hkv, cap, D)
+    lens = torch.zeros(B, device="cuda", dtype=torch.int32)
+    lens[-1], lens[0] = cap, 3
+    q = rn(g, B, T, H, D, scale=1.5)
+    out, lse = torch.zeros(B, T, H, D, device="cuda", dtype=torch.bfloat16), torch.zeros(B, T, H, device="cuda")
+    ctx.shared_prefix_attn_dev(**attn_args(q, None, None, None, ok, ov, lens, out, lse))
+    ctx.synchronize()
+    ro, rl, bo, bl = attn_ref(q[-1:], None, None, None, ok[-1:], ov[-1:], lens[-1:])
+    assert ((out[-1:].double() - ro).abs() <= bo).all() and ((lse[-1:].double() - rl).abs() <= bl).all()
+    assert (out[1:-1] == 0).all() and torch.isneginf(lse[1:-1]).all() and (out[0] == 0).all()
+    w = torch.zeros(B, Hkv, cap, device="cuda")
+    ctx.attn_weights_accumulate_dev(**weights_args(q, ok, lens, lse, w))
+    ctx.synchronize()
+    ref, tol = weights_ref(q[-1:], ok[-1:], lens[-1:], lse[-1:], torch.zeros_like(w[-1:]), 1.0)
+    assert ((w[-1:].double() - ref).abs() <= tol).all() and (w[1:-1] == 0).all()
+    pos = torch.arange(cap, device="cuda", dtype=torch.int32).expand(B, Hkv, cap).contiguous()
+    budget, new = 60001, torch.zeros_like(lens)
+    src = evict_ref(ok[-1:], ov[-1:], w[-1:], pos[-1:], lens[-1:], lens[-1:], budget, 4, 100)
+    k0, v0 = ok[-1].clone(), ov[-1].clone()
+    ctx.kv_evict_dev(n_seqs=B, num_kv_heads=Hkv, kv_dtype=M.KV_BF16, cap=cap, k=ok.data_ptr(), v=ov.data_ptr(), seq_stride=ok.stride(0),
+                     head_stride=ok.stride(1), row_stride=D, budget=budget, n_sink=4, n_recent=100, lens=lens.data_ptr(), next_pos=lens.data_ptr(),
+                     weights=w.data_ptr(), positions=pos.data_ptr(), map_seq_stride=w.stride(0), map_head_stride=w.stride(1),
+                     weights_out=w.data_ptr(), positions_out=pos.data_ptr(), lens_out=new.data_ptr())
+    ctx.synchronize()
+    for (_, h), rows in src.items():
+        ix = torch.tensor(rows, device="cuda", dtype=torch.long)
+        assert torch.equal(ok[-1, h, :budget], k0[h, ix]) and torch.equal(ov[-1, h, :budget], v0[h, ix])
+        assert torch.equal(pos[-1, h, :budget].long(), ix)
+    assert new.tolist() == [3] + [0] * (B - 2) + [budget]
+
+
+def test_largest_evicted_cache(ctx, M):
+    """262,144 rows, the most a call takes: clusters of sixteen CTAs."""
+    g = gen(44)
+    cap, budget = 262144, 100001
+    k, v = rn(g, 1, 1, cap, D), rn(g, 1, 1, cap, D)
+    w = torch.randint(0, 50000, (1, 1, cap), generator=g, device="cuda").float()
+    pos = torch.randperm(cap, generator=g, device="cuda").to(torch.int32).view(1, 1, cap)
+    lens = torch.tensor([cap], device="cuda", dtype=torch.int32)
+    new, k0, v0 = torch.zeros_like(lens), k.clone(), v.clone()
+    rows = evict_ref(k, v, w, pos, lens, lens, budget, 4, 1000)[0, 0]
+    wo, po = torch.zeros_like(w), torch.zeros_like(pos)
+    ctx.kv_evict_dev(n_seqs=1, num_kv_heads=1, kv_dtype=M.KV_BF16, cap=cap, k=k.data_ptr(), v=v.data_ptr(), seq_stride=k.stride(0),
+                     head_stride=k.stride(1), row_stride=D, budget=budget, n_sink=4, n_recent=1000, lens=lens.data_ptr(), next_pos=lens.data_ptr(),
+                     weights=w.data_ptr(), positions=pos.data_ptr(), map_seq_stride=cap, map_head_stride=cap, weights_out=wo.data_ptr(),
+                     positions_out=po.data_ptr(), lens_out=new.data_ptr())
+    ctx.synchronize()
+    ix = torch.tensor(rows, device="cuda", dtype=torch.long)
+    assert torch.equal(k[0, 0, :budget], k0[0, 0, ix]) and torch.equal(v[0, 0, :budget], v0[0, 0, ix])
+    assert torch.equal(wo[0, 0, :budget], w[0, 0, ix]) and torch.equal(po[0, 0, :budget], pos[0, 0, ix]) and new.tolist() == [budget]
+
+
+def test_batches_that_take_several_launches(ctx, M):
+    """More query rows, and more moves, than the context's scratch holds at once."""
+    g = gen(45)
+    B, T, H, Hkv, P, cap = 2400, 2, 32, 2, 150, 20
+    q, pk, pv = rn(g, B, T, H, D), rn(g, Hkv, P, D), rn(g, Hkv, P, D)
+    ok, ov = rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    lens = lens_for(g, B, T, cap)
+    out, lse = torch.zeros(B, T, H, D, device="cuda", dtype=torch.bfloat16), torch.zeros(B, T, H, device="cuda")
+    before = ctx.launch_count
+    ctx.shared_prefix_attn_dev(**attn_args(q, q, pk, pv, ok, ov, lens, out, lse))
+    ctx.synchronize()
+    assert ctx.launch_count > before + 2
+    some = torch.tensor([0, 1, 2, 599, 600, 601, 1199, 1200, 1201, 1800, B - 1], device="cuda")
+    ro, rl, bo, bl = attn_ref(q[some], q[some], pk, pv, ok[some], ov[some], lens[some])
+    assert ((out[some].double() - ro).abs() <= bo).all() and ((lse[some].double() - rl).abs() <= bl).all()
+    # every sequence differs from its neighbours, so a slip of the offsets would show above; none is left out
+    assert torch.isfinite(lse).all() and (out.float().abs().amax((1, 2, 3)) > 0).all()
+    B, Hkv, cap, budget = 4000, 4, 60, 30
+    k, v = rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    w = torch.rand(B, Hkv, cap, generator=g, device="cuda")
+    pos = torch.arange(cap, device="cuda", dtype=torch.int32).expand(B, Hkv, cap).contiguous()
+    lens = torch.randint(0, cap + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    new, k0, v0, w0 = torch.zeros_like(lens), k.clone(), v.clone(), w.clone()
+    src = evict_ref(k, v, w, pos, lens, lens, budget, 1, 2)
+    ctx.kv_evict_dev(n_seqs=B, num_kv_heads=Hkv, kv_dtype=M.KV_BF16, cap=cap, k=k.data_ptr(), v=v.data_ptr(), seq_stride=k.stride(0),
+                     head_stride=k.stride(1), row_stride=D, budget=budget, n_sink=1, n_recent=2, lens=lens.data_ptr(), next_pos=lens.data_ptr(),
+                     weights=w.data_ptr(), positions=pos.data_ptr(), map_seq_stride=w.stride(0), map_head_stride=w.stride(1),
+                     weights_out=w.data_ptr(), positions_out=pos.data_ptr(), lens_out=new.data_ptr())
+    ctx.synchronize()
+    ix = torch.arange(cap).expand(B, Hkv, cap).clone()
+    for (b, h), rows in src.items():
+        ix[b, h, : len(rows)] = torch.tensor(rows, dtype=torch.long)
+    ix = ix.cuda()
+    at = ix.unsqueeze(-1).expand(B, Hkv, cap, D)
+    assert torch.equal(k, k0.gather(2, at)) and torch.equal(v, v0.gather(2, at)) and torch.equal(w, w0.gather(2, ix))
+    assert torch.equal(pos.long(), ix) and torch.equal(new, lens.clamp(max=budget))
