@@ -365,7 +365,7 @@ struct SharedAttnParams {
     const int32_t *lens;
     __nv_bfloat16 *out;
     float *lse;
-    int *plan;                        // [0], [1]: prefix and own tiles per CTA, [8 + b]: first own tile of sequence b
+    int *plan;                        // [0], [1]: prefix and own tiles per CTA, [2]: tiles a unit occupies, [8 + b]: first own tile of sequence b
     float *part_o, *part_m, *part_l;  // partials: prefix slots of 128 rows, then own slots of own_rows rows
     unsigned *status;
     int B, T, H, Hkv, group;

@@ -98,23 +98,25 @@ __device__ __forceinline__ int own_len(const SharedAttnParams &p, int b) {
 __device__ __forceinline__ int own_tiles(const SharedAttnParams &p, int b) { return (own_len(p, b) + SP_N - 1) / SP_N; }
 
 // How a call's tiles are dealt to CTAs: the prefix tiles in runs of `run` to the CTAs 0, 1, ..., the own tiles in runs of
-// `own_run` to the CTAs grid - 1, grid - 2, ....  Either every CTA takes a run of both, or (a call with few tiles per CTA,
-// where a second segment's start and end cost more than its tiles) the first `prefix_ctas` take prefix tiles only and the
-// others own tiles only.  The choice minimises the longest CTA, a segment counted as SP_SEG_COST tiles on top of its own
-// (measured: 5.4 thousand cycles to write a partial of 128 rows, about 4 thousand to fill and drain, against 2.3 thousand
-// per tile) and an own tile, whose rows come from HBM and not from L2, as a quarter more; the split has to win by a tenth
-// (64 sequences x 4 tokens over 32768 rows, where the two estimates meet: 284 us dealt to all, 302 us split).  Every warp
-// computes the plan by itself from the lengths; 32 splits, one a lane, are looked at.
+// `own_run` to the CTAs grid - 1, grid - 2, ....  Either every CTA takes a run of both, or the first CTAs take prefix tiles
+// only and the others own tiles only.  Prefix runs are cut within the units where that is shorter (a unit's place in the
+// sequence is then `unit_place` tiles, whole runs, and no CTA takes parts of two units: 37 x 3 tokens over 10007 rows 49 ->
+// 44 us).  The choice minimises the longest CTA, counted in prefix tiles (2.3 thousand cycles): an own tile, whose rows come
+// from HBM and not from L2, is a quarter more; a further prefix segment 3 (writing the partial of 128 rows takes 4.3
+// thousand cycles), a further own segment 1 and its share of the same.  A split has to win by a fifteenth (64 x 4 tokens
+// over 32768 rows, where the estimates meet: 275 us dealt to all, 282 us split).  Every warp computes the plan by itself from
+// the lengths, 31 splits, one a lane.
 struct Plan {
-    int run, own_run;
+    int run, unit_place, own_run;
     int total_own;
     int chunk, lane_begin;  // lane l covers sequences [l * chunk, ...): its first own tile
 };
-constexpr float SP_SEG_COST = 4.0f, SP_OWN_TILE_COST = 1.25f, SP_SPLIT_GAIN = 0.9f;
+constexpr float SP_SEG_COST = 3.0f, SP_OWN_TILE_COST = 1.25f, SP_BOTH_BIAS = 0.93f;
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + (unsigned)b - 1u) / (unsigned)b); }
 
 __device__ __forceinline__ Plan make_plan(const SharedAttnParams &p, bool *bad) {
     const int lane = threadIdx.x & 31;
-    const int per = p.Hkv * p.own_mtiles, total_p = p.Hkv * p.prefix_mtiles * p.prefix_tiles;
+    const int per = p.Hkv * p.own_mtiles, units_p = p.Hkv * p.prefix_mtiles;
     Plan pl;
     pl.chunk = (p.B + 31) / 32;
     const int b_lo = min(lane * pl.chunk, p.B), b_hi = min(b_lo + pl.chunk, p.B);
@@ -135,36 +137,53 @@ __device__ __forceinline__ Plan make_plan(const SharedAttnParams &p, bool *bad) 
     }
     pl.lane_begin = inc - mine;
     pl.total_own = __shfl_sync(0xffffffffu, inc, 31);
-    const float units_p = (float)(p.Hkv * p.prefix_mtiles), units_o = (float)(per * (int)__reduce_add_sync(0xffffffffu, some));
-    auto cost = [&](int tiles, float units, int ctas, float tile_cost) {
-        const float inv = __frcp_rn((float)ctas), run = ceilf((float)tiles * inv);
-        return tile_cost * run + SP_SEG_COST * fminf(run, 1.0f + units * inv);
-    };
-    int ctas = p.grid;  // for the prefix; grid: both kinds on every CTA
-    if (total_p > 0 && pl.total_own > 0) {
-        float best = SP_SPLIT_GAIN * (cost(total_p, units_p, p.grid, 1.0f) + cost(pl.total_own, units_o, p.grid, SP_OWN_TILE_COST));
-        int at = p.grid;
-        const int c = (lane + 1) * p.grid / 33;  // a split: c CTAs for the prefix
-        if (c >= 1) {
-            const float t = fmaxf(cost(total_p, units_p, c, 1.0f), cost(pl.total_own, units_o, p.grid - c, SP_OWN_TILE_COST));
-            if (t < best) {
-                best = t;
-                at = c;
+    const int units_o = per * (int)__reduce_add_sync(0xffffffffu, some);
+    // the prefix on at most c CTAs: cost of the longest, run length, tiles a unit occupies, CTAs used
+    auto prefix_cost = [&](int c, int &run, int &place, int &used) {
+        run = ceil_div(units_p * p.prefix_tiles, c);
+        place = p.prefix_tiles;
+        used = c;
+        float t = (float)run + SP_SEG_COST * (float)min(run - 1, ceil_div(units_p, c));
+        if (c >= units_p) {
+            const int r = ceil_div(p.prefix_tiles, (int)((unsigned)c / (unsigned)units_p));
+            if ((float)r <= t) {
+                const int parts = ceil_div(p.prefix_tiles, r);
+                t = (float)r;
+                run = r;
+                place = parts * r;
+                used = parts * units_p;
             }
         }
-        // the least cost of all lanes, the smallest split among equals
-        const unsigned least = __reduce_min_sync(0xffffffffu, __float_as_uint(best));
-        ctas = (int)__reduce_min_sync(0xffffffffu, __float_as_uint(best) == least ? (unsigned)at : 0xffffffffu);
+        return t;
+    };
+    const float own_seg = 1.0f + SP_SEG_COST * (float)p.own_rows / (float)SP_M;
+    auto own_cost = [&](int c, int &run) {
+        run = max(1, ceil_div(pl.total_own, c));
+        return SP_OWN_TILE_COST * (float)run + own_seg * (float)min(run - 1, ceil_div(units_o, c));
+    };
+    // lane 31: every CTA takes both kinds; the others: c CTAs for the prefix, the rest for the own rows.  (A call with one
+    // kind only is decided by lane 31 alone.)
+    const bool both = lane == 31;
+    const int c = both ? p.grid : (lane + 1) * p.grid / 32;
+    int run = 1, place = p.prefix_tiles, used = 0, own_run = 1;
+    float t = INFINITY;
+    if (both || (c >= 1 && c < p.grid && p.prefix_tiles > 0 && pl.total_own > 0)) {
+        const float tp = p.prefix_tiles > 0 ? prefix_cost(c, run, place, used) : 0.0f;
+        const float to = own_cost(both ? p.grid : p.grid - used, own_run);
+        t = both ? SP_BOTH_BIAS * (tp + to + own_seg) : fmaxf(tp, to);
     }
-    const int own_ctas = ctas == p.grid ? p.grid : p.grid - ctas;
-    pl.run = (total_p + ctas - 1) / ctas;
-    pl.own_run = max(1, (pl.total_own + own_ctas - 1) / own_ctas);
+    // the least cost, the smallest split among equals
+    const unsigned least = __reduce_min_sync(0xffffffffu, __float_as_uint(t));
+    const int src = __ffs(__ballot_sync(0xffffffffu, __float_as_uint(t) == least)) - 1;
+    pl.run = __shfl_sync(0xffffffffu, run, src);
+    pl.unit_place = __shfl_sync(0xffffffffu, place, src);
+    pl.own_run = __shfl_sync(0xffffffffu, own_run, src);
     return pl;
 }
 // A segment: the tiles [t0, t0 + nt) of one unit.  Every role of a CTA walks the same segments by itself: first its run
 // of the prefix tiles, then its run of the own tiles.
 struct Walk {
-    int at, end;          // prefix tiles left to this CTA
+    int at, end, place;   // prefix tiles left to this CTA, tiles that a unit occupies
     int own_at, own_end;  // own tiles left to it
     int b, begin;         // sequence at hand and its first own tile
     // the segment at hand
@@ -176,13 +195,13 @@ struct Walk {
     __device__ __forceinline__ bool next(const SharedAttnParams &p) {
         if (at < end) {
             own = false;
-            unit = at / p.prefix_tiles;
+            unit = at / place;
             hk = unit / p.prefix_mtiles;
             mt = unit - hk * p.prefix_mtiles;
-            t0 = at - unit * p.prefix_tiles;
+            t0 = at - unit * place;
             nt = min(p.prefix_tiles - t0, end - at);
             len = p.prefix_len;
-            at += nt;
+            at = t0 + nt == p.prefix_tiles ? (unit + 1) * place : at + nt;
             return true;
         }
         if (own_at >= own_end) return false;
@@ -251,7 +270,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         bool bad;
         const Plan pl = make_plan(p, &bad);
         if (bad && blockIdx.x == 0 && warp == 0) atomicOr(p.status, STATUS_BAD_ITEM);
-        const int total_p = p.Hkv * p.prefix_mtiles * p.prefix_tiles;
+        const int total_p = p.Hkv * p.prefix_mtiles * pl.unit_place;
+        walk.place = pl.unit_place;
         walk.at = min((int)blockIdx.x * pl.run, total_p);
         walk.end = min(walk.at + pl.run, total_p);
         walk.own_at = (int)min((long long)own_cta * pl.own_run, (long long)pl.total_own);
@@ -265,6 +285,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
             if (lane == 0) {
                 p.plan[0] = pl.run;
                 p.plan[1] = pl.own_run;
+                p.plan[2] = pl.unit_place;
             }
             int first = pl.lane_begin;
             for (int b = min(lane * pl.chunk, p.B); b < min((lane + 1) * pl.chunk, p.B); b++) {
@@ -639,7 +660,7 @@ __device__ __forceinline__ RowParts row_parts(const SharedAttnParams &p, int hk,
     const int run = p.plan[0], own_run = p.plan[1], nt = own_tiles(p, b);
     if (p.prefix_tiles > 0) {
         const int mt = idx / SP_M, unit = hk * p.prefix_mtiles + mt;
-        const int first = unit * p.prefix_tiles / run, last = ((unit + 1) * p.prefix_tiles - 1) / run;
+        const int place = p.plan[2], first = unit * place / run, last = (unit * place + p.prefix_tiles - 1) / run;
         r.np = last - first + 1;
         r.p0 = ((size_t)unit + first) * SP_M;
         r.pr = idx - mt * SP_M;
