@@ -523,8 +523,9 @@ int mfc_kv_evict_dev(mfc_ctx *ctx, const mfc_kv_evict *args);
  *   target_probs: fp32 [n_seqs][max_drafts + 1][vocab], draft_probs: fp32
  *     [n_seqs][max_drafts][vocab] by their strides;
  *   draft_tokens int32, u_accept fp32: [n_seqs][max_drafts];  u_sample [n_seqs];
- *   draft_lens: int32 [n_seqs], drafts in use, or NULL = max_drafts; a negative
- *     length marks an idle place (n_accepted 0, tokens -1);
+ *   draft_lens: int32 [n_seqs], drafts in use (at most max_drafts count), or
+ *     NULL = max_drafts; a negative length marks an idle place (n_accepted 0,
+ *     tokens -1);  a u_sample outside [0, 1) counts as the nearest end;
  *   tokens: int32 [n_seqs][max_drafts + 1]: the accepted drafts, the drawn token,
  *     then -1.
  * 0 <= max_drafts <= 32. */

@@ -21,8 +21,8 @@
 // reference that a row's exponents are taken against is the maximum of its first tile and moves, with a rescaling of O,
 // only when some score exceeds it by more than 2^32 (fp32 and bf16 have the exponents to spare, and no digits are lost):
 // so no maximum stands before the exponentials of a tile; its rows' maxima are taken along with them, and the two halves
-// of a row ask one another with one barrier reduction whether either must move, which redoes the tile.  P is rounded to bf16 (the type of V: both operands of one
-// instruction have the same type); the row sums l are taken before that rounding.
+// of a row ask one another with one barrier reduction whether either must move, which redoes the tile.  P is rounded to
+// bf16 (the type of V: both operands of one instruction have the same type); the row sums l are taken before that rounding.
 // Every mbarrier wait is bounded.  When one runs out the CTA sets a flag that ends all its waits; the softmax warps still
 // walk their tiles, without work, so that the block barriers among them stay paired; then a status bit is set, the CTA
 // waits for its copies in flight, frees its tensor memory and leaves.
