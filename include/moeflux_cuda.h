@@ -433,7 +433,7 @@ int mfc_kv_cache_view(mfc_ctx *ctx, int32_t layer, int32_t seq_id, void **k, voi
  *     ln sum exp of the scaled scores, or NULL.
  * A query that sees no row at all gets out = 0 and lse = -inf.  Strides are
  * multiples of 8, pointers 16-byte aligned.  1 <= n_tokens <= 16, n_seqs <= 4096,
- * at most 16 query heads per kv head. */
+ * at most 16 query heads per kv head, prefix_len and own_cap at most 2^30. */
 typedef struct mfc_shared_prefix_attn {
     int32_t n_seqs, n_tokens, num_attn_heads, num_kv_heads;
     float softmax_scale;
@@ -462,7 +462,9 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *ctx, const mfc_shared_prefix_attn *args)
  * j < lens[b] - (n_tokens - 1 - t)); other rows of `weights` are left as they
  * were.  lse is what mfc_shared_prefix_attn_dev returned, so weights taken with a
  * shared prefix are shares of the whole softmax.  q, k bf16, lse and weights
- * fp32.  Strides of q and k are multiples of 8, their pointers 16-byte aligned. */
+ * fp32.  decay = 0 starts the sums afresh: what `weights` holds is then not read.
+ * Strides of q and k are multiples of 8, their pointers 16-byte aligned; cap is at
+ * most 2^30. */
 typedef struct mfc_attn_weights {
     int32_t n_seqs, n_tokens, num_attn_heads, num_kv_heads;
     float softmax_scale, decay;
@@ -481,12 +483,12 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *ctx, const mfc_attn_weights *args);
 /* Eviction: every (sequence, kv head) with lens[b] > budget rows keeps the
  * `budget` rows of the largest weight, in place.  Rows whose position is below
  * n_sink or at least next_pos[b] - n_recent are protected and rank before all
- * others; a NaN weight ranks last; ties go to the lowest row.  The result's row r < min(lens[b], budget) is the old row r if it was kept, else
- * the next kept row from beyond the budget: the j-th evicted row below the
- * budget receives the j-th kept row at or above it (attention does not depend on
- * the order of rows whose keys are already rotated; `positions` says which
- * position a row holds).  K and V rows outside the evicted places are not
- * written.
+ * others; a NaN weight ranks last; ties go to the lowest row.  The result's row
+ * r < min(lens[b], budget) is the old row r if it was kept, else the next kept
+ * row from beyond the budget: the j-th evicted row below the budget receives
+ * the j-th kept row at or above it (attention does not depend on the order of rows
+ * whose keys are already rotated; `positions` says which position a row holds).
+ * K and V rows outside the evicted places are not written.
  *   k, v: [seq][kv head][cap][256] of kv_dtype by the three strides;
  *   weights, positions (int32): element (b, hk, row) at b*map_seq + hk*map_head + row;
  *   weights_out, positions_out: same strides, may be weights and positions
@@ -518,7 +520,7 @@ int mfc_kv_evict_dev(mfc_ctx *ctx, const mfc_kv_evict *args);
  * was refused: the lowest v whose cumulative weight exceeds u_sample[b] times the
  * total, sums in 64 bits.  If that residual is zero everywhere the token is drawn
  * from p; if p is zero too it is -1.  Entries that are negative or NaN count as
- * zero.  draft_probs NULL: the drafts were not sampled (q is 1 at x_i).  A drafted
+ * zero; an infinite total leaves -1.  draft_probs NULL: the drafts were not sampled (q is 1 at x_i).  A drafted
  * token outside [0, vocab) is refused.
  *   target_probs: fp32 [n_seqs][max_drafts + 1][vocab], draft_probs: fp32
  *     [n_seqs][max_drafts][vocab] by their strides;

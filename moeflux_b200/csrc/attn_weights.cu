@@ -109,23 +109,24 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     uint64_t *q_empty = bars + 18;    // [2] tcgen05.commit and the summing warps: the unit is done with them
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 20);
     volatile int *s_fail = reinterpret_cast<volatile int *>(bars + 21);
+    uint64_t *drained = bars + 22;    // tcgen05.commit, after a failure: the products in flight are done
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // tensor memory: two buffers of np columns
     const uint32_t cols = np <= 16 ? 32 : (np <= 32 ? 64 : (np <= 64 ? 128 : (np <= 128 ? 256 : 512)));
-    if (warp == 0) {
+    if (warp == 8) {
         tmem_alloc(tmem_slot, cols);
         tmem_relinquish();
     }
     if (warp == 1) {
         if (lane < 20) mbar_init(&bars[lane], lane < 14 ? 1 : (lane < 16 ? 4 : (lane < 18 ? 2 : 9)));
         if (lane == 20) *s_fail = 0;
+        if (lane == 22) mbar_init(drained, 1);
         mbar_fence_init();
     }
     if (tid == 64) prefetch_tmap(&k_map);
     __syncwarp();
     dependency_wait();
-    dependency_allow();
     // ---- every warp by itself: scan over the lengths, this CTA's run, its first sequence ----
     AwWalk walk;
     {
@@ -156,6 +157,8 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // (only now: a CTA of the next kernel may take tensor memory and then wait for this one, which so has its own already)
+    dependency_allow();
     const uint32_t tmem = *tmem_slot;
     auto warp_wait = [&](uint64_t *bar, unsigned parity) -> bool {
         for (unsigned i = 0; i < p.wait_spins; i++) {
@@ -283,7 +286,7 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 const unsigned tile = n + j;
                 const int r0 = (walk.t0 + j) * AW_TILE, r = r0 + row;
                 const bool in = r < walk.len;
-                const float old = in ? wbase[r] : 0.0f;
+                const float old = in && p.decay != 0.0f ? wbase[r] : 0.0f;  // decay 0 starts afresh, whatever is there
                 ok = warp_wait(&s_ready[grp], (tile >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
@@ -344,7 +347,14 @@ attn_weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             mbar_wait_bounded(&full[st], ph, p.wait_spins);
         }
     }
-    if (warp == 0) tmem_dealloc(tmem, cols);
+    if (warp == 8) {
+        if (*s_fail) {  // and so do the products in flight
+            if (elect_one()) tc_commit(drained);
+            mbar_wait_bounded(drained, 0, p.wait_spins);
+            __syncwarp();
+        }
+        tmem_dealloc(tmem, cols);
+    }
 }
 
 }  // namespace

@@ -1476,6 +1476,8 @@ struct DeviceScope {
     }
 };
 
+constexpr int32_t MAX_CACHED_ROWS = 1 << 30;  // of a head; the kernels add a tile to row numbers in 32 bits
+
 bool misaligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
 
 // head layout shared by the attention calls
@@ -1547,8 +1549,8 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
     }
     if (!check_heads(c, a->n_seqs, a->n_tokens, a->num_attn_heads, a->num_kv_heads, a->softmax_scale)) return -1;
     if (a->n_seqs == 0) return 0;
-    if (a->prefix_len < 0 || a->own_cap < 0) {
-        fail(c, "prefix_len and own_cap must not be negative");
+    if (a->prefix_len < 0 || a->own_cap < 0 || a->prefix_len > MAX_CACHED_ROWS || a->own_cap > MAX_CACHED_ROWS) {
+        fail(c, "prefix_len and own_cap must be in [0, 2^30]");
         return -1;
     }
     const bool has_prefix = a->prefix_len > 0, has_own = a->own_cap > 0;
@@ -1608,12 +1610,12 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
                               own_units * (((int64_t)a->own_cap + SHARED_ATTN_N - 1) / SHARED_ATTN_N);
         p.grid = tiles < 1 ? 1 : (tiles < c->n_sms ? (int)tiles : c->n_sms);
         const int64_t need = ((int64_t)p.Hkv * p.prefix_mtiles + p.grid) * SHARED_ATTN_M + (own_units + p.grid) * p.own_rows;
-        return need <= (int64_t)c->max_parts * 16 && tiles < ((int64_t)1 << 30);
+        return need <= (int64_t)c->max_parts * 16 && tiles < ((int64_t)1 << 26);
     };
     int per_launch = a->n_seqs;
     while (!plan(per_launch)) {
         if (per_launch == 1) {
-            fail(c, "too many rows and heads: the partials of one sequence exceed the scratch reserved at open, or its tiles 2^30");
+            fail(c, "too many rows and heads: the partials of one sequence exceed the scratch reserved at open, or its tiles 2^26");
             return -1;
         }
         per_launch = (per_launch + 1) / 2;
@@ -1653,8 +1655,8 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *c, const mfc_attn_weights *a) try {
         return -1;
     }
     if (!check_heads(c, a->n_seqs, a->n_tokens, a->num_attn_heads, a->num_kv_heads, a->softmax_scale)) return -1;
-    if (a->cap < 0) {
-        fail(c, "cap must not be negative");
+    if (a->cap < 0 || a->cap > MAX_CACHED_ROWS) {
+        fail(c, "cap must be in [0, 2^30]");
         return -1;
     }
     if (a->n_seqs == 0 || a->cap == 0) return 0;

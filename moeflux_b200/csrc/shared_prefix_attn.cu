@@ -78,8 +78,8 @@ __device__ __forceinline__ bool quad_any(int quad, bool v) {
     return r != 0;
 }
 // One lane of a converged warp, always the same.  The warps that issue TMA and tensor-core instructions run their loops
-// as whole warps and let this lane issue: addresses and descriptors are then uniform values for the compiler, where a
-// lane-0 branch around the whole loop cost 75 cycles per issued instruction.
+// as whole warps and let this lane issue: addresses and descriptors are then uniform values for the compiler (with a lane-0
+// branch around the whole loop the largest case took 364 us where this took 342).
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;
     asm volatile(
@@ -242,6 +242,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     uint64_t *q_ready = bars + 16;          // softmax warps: the segment's Q is in shared memory
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
     volatile int *s_fail = reinterpret_cast<volatile int *>(bars + 18);
+    uint64_t *drained = bars + 19;          // tcgen05.commit, after a failure: the products in flight are done
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -258,11 +259,11 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         }
         if (lane < 17) mbar_init(&bars[lane], (lane >= 11 && lane <= 13) || lane == 16 ? SP_SOFT : 1);
         if (lane == 17) *s_fail = 0;
+        if (lane == 19) mbar_init(drained, 1);
         mbar_fence_init();
     }
     __syncwarp();
     dependency_wait();
-    dependency_allow();
     // ---- every warp by itself: the plan, this CTA's runs, its first sequence ----
     const int own_cta = (int)gridDim.x - 1 - (int)blockIdx.x;
     Walk walk;
@@ -272,7 +273,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
         if (bad && blockIdx.x == 0 && warp == 0) atomicOr(p.status, STATUS_BAD_ITEM);
         const int total_p = p.Hkv * p.prefix_mtiles * pl.unit_place;
         walk.place = pl.unit_place;
-        walk.at = min((int)blockIdx.x * pl.run, total_p);
+        walk.at = (int)min((long long)blockIdx.x * pl.run, (long long)total_p);
         walk.end = min(walk.at + pl.run, total_p);
         walk.own_at = (int)min((long long)own_cta * pl.own_run, (long long)pl.total_own);
         walk.own_end = min(walk.own_at + pl.own_run, pl.total_own);
@@ -325,6 +326,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // (only now: a CTA of the next kernel may take tensor memory and then wait for this one, which so has its own already)
+    dependency_allow();
     const uint32_t tmem = *tmem_slot;
     // Bounded waits of a whole warp, on one barrier or on three at once (a wait that succeeds at once still costs a round
     // trip to shared memory, so the issuer asks for all it needs in one go).  The failure flag is looked at only after a
@@ -612,7 +615,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
                 const size_t row0 = seg.own ? ((size_t)p.Hkv * p.prefix_mtiles + gridDim.x) * SP_M + slot * p.own_rows : slot * SP_M;
                 const bool valid = ok && row < rows;
                 if (valid && hf == 0) {
-                    p.part_m[row0 + row] = m_run == -INFINITY ? -INFINITY : m_run * sl2;
+                    // (a sum that is NaN with no reference found: every score was NaN, which the merge must not leave out)
+                    p.part_m[row0 + row] = m_run != -INFINITY ? m_run * sl2 : (l_run == l_run ? -INFINITY : 0.0f);
                     p.part_l[row0 + row] = l_run;
                 }
                 float4 *dst = reinterpret_cast<float4 *>(p.part_o + row0 * HEAD_DIM) + row;
@@ -637,7 +641,14 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
     // on the ordinary path every granule has been used; after a failure the copies in flight land before the CTA leaves
     if (warp == SP_SOFT + 1 && lane == 0 && *s_fail)
         for (unsigned k = gi > SP_GRAN ? gi - SP_GRAN : 0; k < gi; k++) mbar_wait_bounded(&full[k % SP_GRAN], (k / SP_GRAN) & 1u, p.wait_spins);
-    if (warp == SP_SOFT) tmem_dealloc(tmem, SP_TMEM_COLS);
+    if (warp == SP_SOFT) {
+        if (*s_fail) {  // and so do the products in flight
+            if (elect_one()) tc_commit(drained);
+            mbar_wait_bounded(drained, 0, p.wait_spins);
+            __syncwarp();
+        }
+        tmem_dealloc(tmem, SP_TMEM_COLS);
+    }
 }
 
 // Joins the partials of the query rows by log-sum-exp, in a fixed order, and applies the gate.  CTA = 32 consecutive

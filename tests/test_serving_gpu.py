@@ -189,6 +189,26 @@ def test_shared_prefix_attn_strided(ctx):
     check_attn(ctx, q, gate, pk, pv, ok, ov, lens_for(g, B, T, cap))
 
 
+@pytest.mark.parametrize("P,cap", [(700, 90), (0, 300), (260, 0)])
+def test_shared_prefix_attn_of_a_query_that_is_nan(ctx, P, cap):
+    """A NaN among the queries shows in its own output and lse, and in no other."""
+    g = gen(6 + P)
+    B, T, H, Hkv = 5, 2, 32, 2
+    q = rn(g, B, T, H, D)
+    pk, pv = (rn(g, Hkv, P, D), rn(g, Hkv, P, D)) if P else (None, None)
+    ok, ov = (rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)) if cap else (None, None)
+    lens = torch.full((B,), cap, device="cuda", dtype=torch.int32)
+    ro, rl, bo, bl = attn_ref(q, None, pk, pv, ok, ov, lens)
+    bad = torch.zeros(B, T, H, dtype=torch.bool, device="cuda")
+    bad[1, 0, 3] = bad[1, 1, 20] = bad[4, 1, 31] = True
+    q[..., 17].masked_fill_(bad, float("nan"))
+    out, lse = torch.zeros_like(q), torch.zeros(B, T, H, device="cuda")
+    ctx.shared_prefix_attn_dev(**attn_args(q, None, pk, pv, ok, ov, lens, out, lse))
+    ctx.synchronize()
+    assert out[bad].isnan().all() and lse[bad].isnan().all()
+    assert ((out.double() - ro).abs() <= bo)[~bad].all() and ((lse.double() - rl).abs() <= bl)[~bad].all()
+
+
 def test_shared_prefix_attn_lengths_out_of_range_are_reported(ctx, M):
     g = gen(4)
     q, pk, pv = rn(g, 3, 1, 32, D), rn(g, 2, 200, D), rn(g, 2, 200, D)
@@ -283,6 +303,24 @@ def test_attn_weights(ctx, B, T, H, Hkv, cap, decay):
     assert ((w.double() - ref).abs() <= tol).all(), float(((w.double() - ref).abs() - tol).max())
     unused = torch.arange(cap, device="cuda").view(1, 1, cap) >= lens.view(B, 1, 1)
     assert torch.equal(w[unused.expand_as(w)], before[unused.expand_as(w)])
+
+
+def test_attn_weights_start_afresh(ctx):
+    """decay 0: what the sums held, NaN or infinite, is not read."""
+    g = gen(8)
+    B, T, H, Hkv, cap = 3, 2, 32, 2, 300
+    q, k = rn(g, B, T, H, D), rn(g, B, Hkv, cap, D)
+    lens = torch.tensor([300, 0, 129], device="cuda", dtype=torch.int32)
+    _, lse, _, _ = attn_ref(q, None, None, None, k, torch.zeros_like(k), lens)
+    lse = lse.float().contiguous()
+    ref, tol = weights_ref(q, k, lens, lse, torch.zeros(B, Hkv, cap, device="cuda"), 0.0)
+    w = torch.full((B, Hkv, cap), float("nan"), device="cuda")
+    w[..., ::2] = float("inf")
+    ctx.attn_weights_accumulate_dev(**weights_args(q, k, lens, lse, w, 0.0))
+    ctx.synchronize()
+    used = (torch.arange(cap, device="cuda").view(1, 1, cap) < lens.view(B, 1, 1)).expand_as(w)
+    assert ((w.double() - ref).abs() <= tol)[used].all()
+    assert not torch.isfinite(w[~used]).any()
 
 
 def test_attn_weights_strided_and_out_of_range(ctx, M):
@@ -650,6 +688,21 @@ def test_refusals(ctx, M):
         fn(**{**base, "n_seqs": 0})  # an empty batch is no error and no launch
     assert ctx.launch_count == before
     ctx.synchronize()
+
+
+def test_row_counts_that_pass_32_bits_are_refused(ctx, M):
+    t = torch.zeros(4096, device="cuda", dtype=torch.bfloat16)
+    P, many = t.data_ptr(), (1 << 30) + 1
+    q = dict(n_seqs=1, n_tokens=1, num_attn_heads=1, num_kv_heads=1, softmax_scale=SCALE, q=P, q_seq_stride=256, q_token_stride=256, q_head_stride=256)
+    before = ctx.launch_count
+    for rows in (many, (1 << 31) - 1):
+        with pytest.raises(M.MfcError, match="2\\^30"):
+            ctx.shared_prefix_attn_dev(**q, own_k=P, own_v=P, own_seq_stride=256, own_head_stride=256, own_row_stride=256, own_cap=rows, own_lens=P, out=P)
+        with pytest.raises(M.MfcError, match="2\\^30"):
+            ctx.shared_prefix_attn_dev(**q, prefix_k=P, prefix_v=P, prefix_head_stride=256, prefix_row_stride=256, prefix_len=rows, own_lens=P, out=P)
+        with pytest.raises(M.MfcError, match="2\\^30"):
+            ctx.attn_weights_accumulate_dev(**q, decay=1.0, k=P, k_seq_stride=256, k_head_stride=256, k_row_stride=256, cap=rows, lens=P, lse=P, weights=P)
+    assert ctx.launch_count == before
 
 
 def test_a_captured_step_of_all_four(ctx, M):
