@@ -857,3 +857,59 @@ def test_batches_that_take_several_launches(ctx, M):
     at = ix.unsqueeze(-1).expand(B, Hkv, cap, D)
     assert torch.equal(k, k0.gather(2, at)) and torch.equal(v, v0.gather(2, at)) and torch.equal(w, w0.gather(2, ix))
     assert torch.equal(pos.long(), ix) and torch.equal(new, lens.clamp(max=budget))
+
+
+def test_two_contexts_at_once(M):
+    """Two servers on one GPU, each with a context, a stream and inputs of its own: the same bits as one after the other."""
+    ways = []
+    for seed, (B, T, H, Hkv, P, cap) in [(51, (20, 3, 24, 2, 1700, 300)), (52, (7, 1, 32, 2, 900, 500))]:
+        g = gen(seed)
+        c, s = M.Ctx(num_layers=4, max_seq=64, n_seqs=1, kv_dtype=M.KV_BF16), torch.cuda.Stream()
+        c.set_stream(s.cuda_stream)
+        V = 20001
+        t = dict(q=rn(g, B, T, H, D), pk=rn(g, Hkv, P, D), pv=rn(g, Hkv, P, D), ok=rn(g, B, Hkv, cap, D), ov=rn(g, B, Hkv, cap, D),
+                 lens=lens_for(g, B, T, cap), p=torch.softmax(torch.randn(B, 3, V, generator=g, device="cuda"), -1),
+                 x=torch.randint(0, V, (B, 2), generator=g, device="cuda", dtype=torch.int32), ua=torch.rand(B, 2, generator=g, device="cuda"),
+                 us=torch.rand(B, generator=g, device="cuda"))
+        t.update(out=torch.zeros_like(t["q"]), lse=torch.zeros(B, T, H, device="cuda"), w=torch.zeros(B, Hkv, cap, device="cuda"),
+                 pos=torch.arange(cap, device="cuda", dtype=torch.int32).expand(B, Hkv, cap).contiguous(), new=torch.zeros_like(t["lens"]),
+                 n=torch.zeros(B, device="cuda", dtype=torch.int32), tok=torch.zeros(B, 3, device="cuda", dtype=torch.int32))
+        ways.append((c, t, (B, T, H, Hkv, cap, V)))
+
+    def step(c, t, sizes):
+        B, T, H, Hkv, cap, V = sizes
+        c.shared_prefix_attn_dev(**attn_args(t["q"], t["q"], t["pk"], t["pv"], t["ok"], t["ov"], t["lens"], t["out"], t["lse"]))
+        c.attn_weights_accumulate_dev(**weights_args(t["q"], t["ok"], t["lens"], t["lse"], t["w"], 0.5))
+        c.kv_evict_dev(n_seqs=B, num_kv_heads=Hkv, kv_dtype=M.KV_BF16, cap=cap, k=t["ok"].data_ptr(), v=t["ov"].data_ptr(),
+                       seq_stride=t["ok"].stride(0), head_stride=t["ok"].stride(1), row_stride=D, budget=100, n_sink=2, n_recent=5,
+                       lens=t["lens"].data_ptr(), next_pos=t["lens"].data_ptr(), weights=t["w"].data_ptr(), positions=t["pos"].data_ptr(),
+                       map_seq_stride=Hkv * cap, map_head_stride=cap, weights_out=t["w"].data_ptr(), positions_out=t["pos"].data_ptr(),
+                       lens_out=t["new"].data_ptr())
+        c.verify_drafts_dev(n_seqs=B, max_drafts=2, vocab=V, target_probs=t["p"].data_ptr(), target_seq_stride=3 * V, target_row_stride=V,
+                            draft_tokens=t["x"].data_ptr(), u_accept=t["ua"].data_ptr(), u_sample=t["us"].data_ptr(),
+                            n_accepted=t["n"].data_ptr(), tokens=t["tok"].data_ptr())
+
+    start = [{k: v.clone() for k, v in t.items()} for _, t, _ in ways]
+    results = []
+    for together in (False, True):
+        for (_, t, _), s in zip(ways, start):
+            for k, v in s.items():
+                t[k].copy_(v)
+        torch.cuda.synchronize()
+        if together:
+            for _ in range(8):
+                for way in ways:
+                    step(*way)
+        else:
+            for way in ways:
+                for _ in range(8):
+                    step(*way)
+                way[0].synchronize()
+        for c, _, _ in ways:
+            c.synchronize()
+        results.append([{k: v.clone() for k, v in t.items()} for _, t, _ in ways])
+    for a, b in zip(*results):
+        for k in a:
+            assert torch.equal(a[k], b[k]), k
+    for c, _, _ in ways:
+        c.close()
