@@ -9,9 +9,10 @@
 // beyond the budget and destinations below it, so the moves need no order among themselves.
 //
 // Two kernels.  The selection is bound by latency (8 bytes per row, then some ten dependent steps): a cluster of CTAs owns
-// a unit, each holds the keys of a contiguous run of rows in shared memory; the border key is found by a radix selection
-// (11 + 11 + 10 bits) whose histograms are summed through distributed shared memory; a warp walks its rows 32 at a time,
-// ballots give the ranks of ties, holes and movers, and the pairs (destination, source) go to a list in device memory.
+// a unit, each holds the keys of a contiguous run of rows in shared memory; the border (key, row) is found by a radix
+// selection (11 + 11 bits, histograms summed through distributed shared memory, then the few rows that share those 22 bits
+// are ranked one by one; many of them: 10 bits more, and the ties in the order of rows).  A warp walks its rows 32 at a
+// time, ballots give the ranks of holes and movers, and the pairs (destination, source) go to a list in device memory.
 // The copy is bound by HBM (4 KiB per moved row, bf16: 2 KiB): all moves of all units are dealt evenly over all SMs,
 // whatever the units' sizes (with the copies in the selecting CTAs, 8 sequences of 7 to 20 thousand rows took twice as
 // long).  A small call -- EV_FUSED_ROWS rows per unit at most -- copies in the selecting CTA and saves the second launch.
@@ -33,9 +34,10 @@ constexpr int EV_MAX_CLUSTER = 16;
 constexpr int EV_MAX_ROWS_PER_CTA = 16384;  // 4 bytes of shared memory each: 64 KiB
 constexpr int EV_MIN_ROWS = 2048;           // rows per CTA below which a cluster does not grow
 constexpr int EV_FUSED_ROWS = 2048;
-constexpr int EV_LISTS = EV_MAX_CLUSTER * EV_WARPS;  // warps of a unit
-static_assert(EV_LISTS <= EV_THREADS, "one thread per warp of a unit");
+constexpr int EV_CAND = 32;                 // rows that are ranked one by one, a lane each
 static_assert(EV_BINS / 4 <= EV_THREADS, "four bins per thread");
+static_assert(EV_MAX_ROWS_PER_CTA / EV_THREADS <= 32, "a warp's masks, one per 32 rows, are held by its lanes");
+static_assert(EV_FUSED_ROWS / 2 * sizeof(int2) <= EV_BINS * 4, "the moves of a small unit take the place of a histogram");
 
 __device__ __forceinline__ uint32_t weight_key(float w, bool safe) {
     if (safe) return 0xffffffffu;
@@ -90,12 +92,15 @@ __device__ __forceinline__ void copy_rows(const EvictParams &p, size_t base, int
 
 struct EvShared {
     uint4 hist[3][EV_BINS / 4];
-    uint4 sums[EV_BINS / 4];                    // of a pass, over the cluster's CTAs
-    int warp_sum[EV_WARPS];
+    uint4 sums[EV_BINS / 4];                // of a pass, over the cluster's CTAs
+    int warp_sum[3][EV_WARPS];
     int ties[EV_WARPS];
-    int holes[EV_WARPS], movers[EV_WARPS];      // of this CTA's warps, for its peers
-    int hole0[EV_LISTS], mover0[EV_LISTS];      // rank of the first hole / mover of every warp of the unit
-    int digit, above;                           // result of a selection pass
+    int holes[EV_WARPS], movers[EV_WARPS];
+    int2 cta_moves[EV_MAX_CLUSTER];         // the sums of both, of every CTA of the cluster
+    int digit[3], above[3], count[3];       // of a pass: the border's digit, the rows above it, those that share it
+    int last;                               // the last tie that is kept
+    unsigned n_cand;                        // of the first CTA: rows that share the border's first 22 bits
+    unsigned long long cand[EV_CAND];       // key, row (inverted: of equal keys the lower row ranks higher)
 };
 
 __global__ void __launch_bounds__(EV_THREADS, 1) kv_evict_select_kernel(const EvictParams p) {
@@ -108,6 +113,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) kv_evict_select_kernel(const Ev
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     for (int i = tid; i < 3 * EV_BINS / 4; i += EV_THREADS) (&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid == 0) sh.n_cand = 0u;
     dependency_wait();
     dependency_allow();
     int n = p.lens[b];
@@ -158,25 +164,20 @@ __global__ void __launch_bounds__(EV_THREADS, 1) kv_evict_select_kernel(const Ev
         }
     }
     if (all) return;
+    auto sync_unit = [&]() {
+        if (cs > 1) cluster.sync();
+        else __syncthreads();
+    };
 
-    // radix selection: after pass k the leading digits of the border key are known, and how many kept rows share them
+    // radix selection: after pass k the leading digits of the border key are known, how many of the rows that share them
+    // are kept, and how many there are
     uint32_t border = 0;
-    int need = kept_n;  // kept rows among those that share the known digits
-#pragma unroll
-    for (int ps = 0; ps < 3; ps++) {
-        const int shift = ps == 0 ? 21 : (ps == 1 ? 10 : 0);
-        const int bins = ps == 2 ? 1024 : 2048;
-        if (ps > 0) {
-            const int known = ps == 1 ? 21 : 10;
-            for (int i = tid; i < rows; i += EV_THREADS) {
-                const uint32_t k = keys[i];
-                if ((k >> known) == (border >> known)) atomicAdd(reinterpret_cast<unsigned *>(sh.hist[ps]) + ((k >> shift) & (bins - 1)), 1u);
-            }
-        }
+    int need = kept_n, sharing = 0;
+    auto select_digit = [&](int ps, int shift, int bins) {  // histogram ps is complete in every CTA's shared memory
+        sync_unit();
         if (cs > 1) {
             // every CTA sums its share of the bins over all CTAs and hands the sums to all (every CTA summing every bin
             // moves cs times as much through distributed shared memory: 6.5 thousand cycles a pass against 3.5 with eight)
-            cluster.sync();
             const int share = bins / 4 / cs;
             if (tid < share) {
                 uint4 c = make_uint4(0u, 0u, 0u, 0u);
@@ -192,103 +193,159 @@ __global__ void __launch_bounds__(EV_THREADS, 1) kv_evict_select_kernel(const Ev
                 for (int r = 0; r < cs; r++) *cluster.map_shared_rank(&sh.sums[rank * share + tid], r) = c;
             }
             cluster.sync();
-        } else {
-            __syncthreads();
         }
         // thread t owns the four bins below bins - 4t, from the largest down
         const int quad = bins / 4 - 1 - tid;
         uint4 c = make_uint4(0u, 0u, 0u, 0u);
         if (quad >= 0) c = cs > 1 ? sh.sums[quad] : sh.hist[ps][quad];
-        int total;
-        int above = block_scan((int)(c.x + c.y + c.z + c.w), sh.warp_sum, &total);
-        const int cnt[4] = {(int)c.w, (int)c.z, (int)c.y, (int)c.x};
+        const int mine = (int)(c.x + c.y + c.z + c.w), sum = __reduce_add_sync(0xffffffffu, mine);
+        if (lane == 0) sh.warp_sum[ps][warp] = sum;
+        __syncthreads();
+        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_sum[ps][lane] : 0);
+        if (before < need && before + sum >= need) {  // the border lies among this warp's bins
+            int inc = mine;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (above < need && above + cnt[e] >= need) {
-                sh.digit = quad * 4 + 3 - e;
-                sh.above = above;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += up;
             }
-            above += cnt[e];
-        }
-        __syncthreads();
-        border |= (uint32_t)sh.digit << shift;
-        need -= sh.above;
-        __syncthreads();
-    }
-    // rows whose key equals the border: the `need` lowest ones are kept; those of the CTAs before this one come first
-    int tie0 = 0;
-    for (int r = 0; r < rank; r++) tie0 += (int)*(cluster.map_shared_rank(reinterpret_cast<unsigned *>(sh.hist[2]), r) + (border & 1023u));
-
-    // warp w owns the rows [w0, w1) of the run
-    const int per = ((rows + EV_WARPS - 1) / EV_WARPS + 31) & ~31;
-    const int w0 = min(warp * per, rows), w1 = min(w0 + per, rows);
-    const unsigned below = (1u << lane) - 1u;
-    int ties = 0;
-    for (int i = w0 + lane; i < w1; i += 32) ties += keys[i] == border;
-    ties = __reduce_add_sync(0xffffffffu, ties);
-    if (lane == 0) sh.ties[warp] = ties;
-    __syncthreads();
-    tie0 += __reduce_add_sync(0xffffffffu, lane < warp ? sh.ties[lane] : 0);
-    // the 32 rows from i0 on: which are holes, which movers
-    auto classify = [&](int i0, int &tie, unsigned &holes, unsigned &movers) {
-        const int i = i0 + lane;
-        const bool in = i < w1;
-        const uint32_t k = in ? keys[i] : 0u;
-        const bool eq = in && k == border;
-        const unsigned eqs = __ballot_sync(0xffffffffu, eq);
-        const bool kept = in && (k > border || (eq && tie + __popc(eqs & below) < need));
-        holes = __ballot_sync(0xffffffffu, in && !kept && r0 + i < p.budget);
-        movers = __ballot_sync(0xffffffffu, kept && r0 + i >= p.budget);
-        tie += __popc(eqs);
-    };
-    int n_holes = 0, n_movers = 0, tie = tie0;
-    for (int i0 = w0; i0 < w1; i0 += 128) {  // (rows past the range classify as neither)
+            int above = before + inc - mine;
+            const int cnt[4] = {(int)c.w, (int)c.z, (int)c.y, (int)c.x};
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            unsigned hs, ms;
-            classify(i0 + 32 * u, tie, hs, ms);
-            n_holes += __popc(hs);
-            n_movers += __popc(ms);
+            for (int e = 0; e < 4; e++) {
+                if (above < need && above + cnt[e] >= need) {
+                    sh.digit[ps] = quad * 4 + 3 - e;
+                    sh.above[ps] = above;
+                    sh.count[ps] = cnt[e];
+                }
+                above += cnt[e];
+            }
+        }
+        __syncthreads();
+        border |= (uint32_t)sh.digit[ps] << shift;
+        need -= sh.above[ps];
+        sharing = sh.count[ps];
+    };
+    select_digit(0, 21, 2048);
+    for (int i = tid; i < rows; i += EV_THREADS) {
+        const uint32_t k = keys[i];
+        if (k >> 21 == border >> 21) atomicAdd(reinterpret_cast<unsigned *>(sh.hist[1]) + ((k >> 10) & 2047u), 1u);
+    }
+    select_digit(1, 10, 2048);
+    // kept: the rows whose key is above the border's, and of those that have it the rows up to `last`
+    const int per = ((rows + EV_WARPS - 1) / EV_WARPS + 31) & ~31;  // warp w owns the rows [w0, w1) of the run
+    const int w0 = min(warp * per, rows), w1 = min(w0 + per, rows);
+    int last;
+    if (sharing <= EV_CAND) {
+        EvShared *first = cs > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+        for (int i = tid; i < rows; i += EV_THREADS) {
+            const uint32_t k = keys[i];
+            if (k >> 10 == border >> 10) first->cand[atomicAdd(&first->n_cand, 1u)] = (unsigned long long)k << 32 | (uint32_t)~(r0 + i);
+        }
+        sync_unit();
+        const unsigned long long mine = lane < sharing ? first->cand[lane] : 0ull;
+        int ahead = 0;
+        for (int j = 0; j < sharing; j++) ahead += __shfl_sync(0xffffffffu, mine, j) > mine;
+        const unsigned at = __ballot_sync(0xffffffffu, lane < sharing && ahead == need - 1);
+        const unsigned long long edge = __shfl_sync(0xffffffffu, mine, __ffs(at) - 1);
+        border = (uint32_t)(edge >> 32);
+        last = (int)~(uint32_t)edge;
+    } else {
+        for (int i = tid; i < rows; i += EV_THREADS) {
+            const uint32_t k = keys[i];
+            if (k >> 10 == border >> 10) atomicAdd(reinterpret_cast<unsigned *>(sh.hist[2]) + (k & 1023u), 1u);
+        }
+        select_digit(2, 0, 1024);
+        // the `need` lowest of the rows that have the border's key are kept; those of the CTAs before this one come first
+        int here = 0;
+        for (int r = 0; r <= rank; r++) {
+            const int t = (int)*(cluster.map_shared_rank(reinterpret_cast<unsigned *>(sh.hist[2]), r) + (border & 1023u));
+            if (r < rank) need -= t;
+            else here = t;
+        }
+        last = need <= 0 ? -1 : n;
+        if (need > 0 && need < here) {  // (the same in all threads of the CTA)
+            int ties = 0;
+            for (int i = w0 + lane; i < w1; i += 32) ties += keys[i] == border;
+            ties = __reduce_add_sync(0xffffffffu, ties);
+            if (lane == 0) sh.ties[warp] = ties;
+            __syncthreads();
+            int left = need - __reduce_add_sync(0xffffffffu, lane < warp ? sh.ties[lane] : 0);
+            if (left > 0 && left <= ties)  // the last one that is kept is this warp's
+                for (int i0 = w0; i0 < w1; i0 += 32) {
+                    const unsigned eq = __ballot_sync(0xffffffffu, i0 + lane < w1 && keys[i0 + lane] == border);
+                    if (left > 0 && left <= __popc(eq)) {
+                        if (eq >> lane & 1u && __popc(eq & ((1u << lane) - 1u)) == left - 1) sh.last = r0 + i0 + lane;
+                    }
+                    left -= __popc(eq);
+                }
+            __syncthreads();
+            last = sh.last;
         }
     }
+    // Lane g holds the rows of the warp's g-th 32 that move (holes below the budget, movers beyond it).
+    const int w_rows = max(w1 - w0, 0);
+    unsigned hits = 0;
+#pragma unroll 4
+    for (int g = 0; g < (w_rows + 31) / 32; g++) {
+        const int i = w0 + 32 * g + lane;
+        const uint32_t k = i < w1 ? keys[i] : 0u;
+        const bool kept = k > border || (k == border && r0 + i <= last);
+        const unsigned m = __ballot_sync(0xffffffffu, i < w1 && kept != (r0 + i < p.budget));
+        if (lane == g) hits = m;
+    }
+    const int low = p.budget - (r0 + w0 + 32 * lane);  // rows of lane g's 32 that lie below the budget
+    const unsigned side = low >= 32 ? 0xffffffffu : (low <= 0 ? 0u : (1u << low) - 1u);
+    int hole = __popc(hits & side), mover = __popc(hits & ~side);
+    const int n_holes = __reduce_add_sync(0xffffffffu, hole), n_movers = __reduce_add_sync(0xffffffffu, mover);
     if (lane == 0) {
         sh.holes[warp] = n_holes;
         sh.movers[warp] = n_movers;
     }
-    if (cs > 1) cluster.sync();
-    else __syncthreads();
-    // ranks of every warp's first hole and mover within the unit
-    int moves;
-    {
-        const int lists = cs * EV_WARPS;
-        const int r = tid / EV_WARPS, k = tid % EV_WARPS;
-        const int nh = tid < lists ? *cluster.map_shared_rank(&sh.holes[k], r) : 0, nm = tid < lists ? *cluster.map_shared_rank(&sh.movers[k], r) : 0;
-        int same;  // holes and movers are equally many
-        const int h0 = block_scan(nh, sh.warp_sum, &moves), q0 = block_scan(nm, sh.warp_sum, &same);
-        if (tid < lists) {
-            sh.hole0[tid] = h0;
-            sh.mover0[tid] = q0;
-        }
+    if (cs > 1) {  // one warp hands the CTA's sums to all (all warps fetching them took 2.5 thousand cycles longer)
         __syncthreads();
-    }
-    int2 *list = p.moves + (size_t)unit * p.max_moves;
-    int hole = sh.hole0[rank * EV_WARPS + warp], mover = sh.mover0[rank * EV_WARPS + warp];
-    tie = tie0;
-    for (int i0 = w0; i0 < w1; i0 += 128) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int i = i0 + 32 * u;
-            unsigned hs, ms;
-            classify(i, tie, hs, ms);
-            if (hs >> lane & 1u) list[hole + __popc(hs & below)].x = r0 + i + lane;
-            if (ms >> lane & 1u) list[mover + __popc(ms & below)].y = r0 + i + lane;
-            hole += __popc(hs);
-            mover += __popc(ms);
+        if (warp == 0) {
+            const int2 sum = make_int2(__reduce_add_sync(0xffffffffu, sh.holes[lane]), __reduce_add_sync(0xffffffffu, sh.movers[lane]));
+            if (lane < cs) *cluster.map_shared_rank(&sh.cta_moves[rank], lane) = sum;
         }
+    }
+    // lane g: ranks of the first hole and mover of its 32 rows, within the warp and then within the unit
+    {
+        int ih = hole, im = mover;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int uh = __shfl_up_sync(0xffffffffu, ih, o), um = __shfl_up_sync(0xffffffffu, im, o);
+            if (lane >= o) {
+                ih += uh;
+                im += um;
+            }
+        }
+        hole = ih - hole;
+        mover = im - mover;
+    }
+    sync_unit();
+    const int wh = sh.holes[lane], wm = sh.movers[lane];
+    int moves = __reduce_add_sync(0xffffffffu, wh);  // holes and movers of a unit are equally many
+    hole += __reduce_add_sync(0xffffffffu, lane < warp ? wh : 0);
+    mover += __reduce_add_sync(0xffffffffu, lane < warp ? wm : 0);
+    if (cs > 1) {
+        const int2 of = lane < cs ? sh.cta_moves[lane] : make_int2(0, 0);
+        moves = __reduce_add_sync(0xffffffffu, of.x);
+        hole += __reduce_add_sync(0xffffffffu, lane < rank ? of.x : 0);
+        mover += __reduce_add_sync(0xffffffffu, lane < rank ? of.y : 0);
+    }
+    int2 *list = p.fused ? reinterpret_cast<int2 *>(sh.hist[0]) : p.moves + (size_t)unit * p.max_moves;
+    for (int g = 0; g < (w_rows + 31) / 32; g++) {
+        const unsigned m = __shfl_sync(0xffffffffu, hits, g), s = __shfl_sync(0xffffffffu, side, g);
+        const int h0 = __shfl_sync(0xffffffffu, hole, g), q0 = __shfl_sync(0xffffffffu, mover, g);
+        const unsigned below = (1u << lane) - 1u;
+        const int row = r0 + w0 + 32 * g + lane;
+        if (m & s & (1u << lane)) list[h0 + __popc(m & s & below)].x = row;
+        if (m & ~s & (1u << lane)) list[q0 + __popc(m & ~s & below)].y = row;
     }
     if (rank == 0 && tid == 0) p.counts[unit] = moves;
     if (cs > 1) {
-        cluster.sync();  // a CTA's counts stay until its peers have read them
+        cluster.sync();  // the histograms stay until the peers have read them
     } else if (p.fused) {
         __syncthreads();
         const size_t base = (size_t)b * p.seq_stride + (size_t)h * p.head_stride;
@@ -366,7 +423,7 @@ cudaError_t launch_kv_evict(EvictParams p, int n_sms, cudaStream_t stream, int *
     *launches = 0;
     if (units <= 0) return cudaSuccess;
     // As many CTAs per unit as there are SMs for, but at least EV_MIN_ROWS rows each: a small unit is over sooner without
-    // the exchanges through distributed shared memory (1088 rows: 14.7 us in one CTA, 18.9 in eight).
+    // the exchanges through distributed shared memory (4 x 1088 rows: 6.9 us in one CTA, 14.0 in eight).
     int cs = 1;
     while (cs < EV_MAX_CLUSTER && ((int64_t)units * cs * 2 <= n_sms || p.cap > cs * EV_MAX_ROWS_PER_CTA) && p.cap > cs * EV_MIN_ROWS) cs *= 2;
     p.fused = cs == 1 && p.cap <= EV_FUSED_ROWS;

@@ -411,6 +411,34 @@ def test_kv_evict(ctx, M, B, Hkv, cap, budget, dtype, kind):
             assert torch.equal(wo[b, h, n:].nan_to_num(-9.0), rest_w.nan_to_num(-9.0)) and torch.equal(po[b, h, n:], rest_p)
 
 
+@pytest.mark.parametrize("cap,budget", [(200, 90), (5000, 2400), (33000, 9000)])
+@pytest.mark.parametrize("crowd", [1, 2, 31, 32, 33, 70])
+@pytest.mark.parametrize("values", [1024, 5, 1])
+def test_kv_evict_with_a_crowd_at_the_border(ctx, M, cap, budget, crowd, values):
+    """`crowd` weights that differ in their last ten bits at most, of `values` different ones, and the border among them."""
+    g = gen(cap + crowd)
+    w = torch.rand(1, 2, cap, generator=g, device="cuda") + torch.where(torch.arange(cap, device="cuda") < budget - crowd // 2, 3.0, 0.0)
+    low = torch.randint(0, values, (2, crowd), generator=g, device="cuda", dtype=torch.int32)
+    w[0, :, budget - crowd // 2 : budget - crowd // 2 + crowd] = (low + 0x40000000).view(torch.float32)  # 2.0 and up
+    for h in range(2):
+        w[0, h] = w[0, h, torch.randperm(cap, generator=g, device="cuda")]
+    k, v = rn(g, 1, 2, cap, D), rn(g, 1, 2, cap, D)
+    pos = torch.arange(cap, device="cuda", dtype=torch.int32).expand(1, 2, cap).contiguous()
+    lens, new = torch.tensor([cap], device="cuda", dtype=torch.int32), torch.zeros(1, device="cuda", dtype=torch.int32)
+    src = evict_ref(k, v, w, pos, lens, lens, budget, 0, 0)
+    k0, v0, w0 = k.clone(), v.clone(), w.clone()
+    ctx.kv_evict_dev(n_seqs=1, num_kv_heads=2, kv_dtype=M.KV_BF16, cap=cap, k=k.data_ptr(), v=v.data_ptr(), seq_stride=k.stride(0),
+                     head_stride=k.stride(1), row_stride=D, budget=budget, n_sink=0, n_recent=0, lens=lens.data_ptr(),
+                     next_pos=lens.data_ptr(), weights=w.data_ptr(), positions=pos.data_ptr(), map_seq_stride=2 * cap, map_head_stride=cap,
+                     weights_out=w.data_ptr(), positions_out=pos.data_ptr(), lens_out=new.data_ptr())
+    ctx.synchronize()
+    assert int(new) == budget
+    for (b, h), rows in src.items():
+        ix = torch.tensor(rows, device="cuda")
+        assert torch.equal(pos[b, h, :budget].long(), ix) and torch.equal(w[b, h, :budget], w0[b, h, ix])
+        assert torch.equal(k[b, h, :budget], k0[b, h, ix]) and torch.equal(v[b, h, :budget], v0[b, h, ix])
+
+
 def test_kv_evict_strided_rows_and_out_of_range(ctx, M):
     g = gen(11)
     B, Hkv, cap, budget = 3, 2, 90, 50
