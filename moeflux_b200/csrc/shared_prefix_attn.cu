@@ -652,11 +652,12 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap pk_map, const __gr
 }
 
 // Joins the partials of the query rows by log-sum-exp, in a fixed order, and applies the gate.  CTA = 32 consecutive
-// query rows of a kv head (lane = row).  Few partials per row: warp w takes the dims [32 w, 32 w + 32) of all partials
-// (the prefix unit's first, then the own unit's).  Many (FEW false; a long prefix cut for a small batch): the CTA takes 32
-// dims, warp w the partials w, w + 8, ..., and the warps' results are joined through shared memory.
+// query rows of a kv head (lane = row) and 256 / GROUPS of their dims, a warp 32 dims of them.  One group: a warp takes all
+// partials (the prefix unit's first, then the own unit's).  Several (few rows, or a long prefix cut for a small batch): group
+// g takes the partials g, g + GROUPS, ..., and the groups' results are joined through shared memory.
 constexpr int MG_WARPS = 8;
 constexpr int MG_DIMS = 32;
+constexpr int MG_CTAS = 160;
 constexpr int MG_FEW = 12, MG_FEW_BLOCKS = 128;
 
 struct RowParts {
@@ -738,8 +739,8 @@ __device__ __forceinline__ float2 gate2(uint32_t bits) {
                        1.0f / (1.0f + expf(-bf16_bits_to_f32((uint16_t)(bits >> 16)))));
 }
 
-template <bool FEW>
-__global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const SharedAttnParams p) {
+template <int GROUPS>
+__global__ void __launch_bounds__(32 * MG_WARPS, GROUPS > 1 ? 2 : 1) shared_attn_merge_kernel(const SharedAttnParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows_hk = p.B * p.T * p.group;
     const int blocks_hk = (rows_hk + 31) / 32;
@@ -747,7 +748,7 @@ __global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const 
     dependency_wait();  // the plan and the partials are written by the kernel before
     RowParts parts = {0, 0, 0, 0, 0, 0};
     if (idx0 + lane < rows_hk) parts = row_parts(p, hk, idx0 + lane);
-    if (FEW) {
+    if (GROUPS == 1) {
         const int idx = idx0 + lane, d0 = warp * MG_DIMS;
         if (idx >= rows_hk) return;
         const int bt = idx / p.group, h = hk * p.group + (idx - bt * p.group);
@@ -782,9 +783,9 @@ __global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const 
     } else {
         __shared__ float s_m[MG_WARPS][32], s_l[MG_WARPS][32];
         __shared__ float4 s_o[MG_WARPS][MG_DIMS / 4][33];
-        const int d0 = blockIdx.y * MG_DIMS;
+        constexpr int CHUNKS = MG_WARPS / GROUPS;
         Joined j;
-        join_parts(p, parts, warp, MG_WARPS, d0, j);
+        join_parts(p, parts, warp % GROUPS, GROUPS, (blockIdx.y * CHUNKS + warp / GROUPS) * MG_DIMS, j);
         s_m[warp][lane] = j.M;
         s_l[warp][lane] = j.L;
 #pragma unroll
@@ -794,37 +795,40 @@ __global__ void __launch_bounds__(32 * MG_WARPS) shared_attn_merge_kernel(const 
         const int row = threadIdx.x >> 3, q4 = threadIdx.x & 7;
         const int idx = idx0 + row;
         if (idx >= rows_hk) return;
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < MG_WARPS; w++) M = fmaxf(M, s_m[w][row]);
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < MG_WARPS; w++) {
-            const float m = s_m[w][row];
-            if (m == -INFINITY) continue;
-            const float wt = ex2_approx(m - M);
-            const float4 o = s_o[w][q4][row];
-            L += wt * s_l[w][row];
-            a.x = fmaf(wt, o.x, a.x);
-            a.y = fmaf(wt, o.y, a.y);
-            a.z = fmaf(wt, o.z, a.z);
-            a.w = fmaf(wt, o.w, a.w);
-        }
-        const bool none = M == -INFINITY;
-        const float inv = none ? 0.0f : 1.0f / L;
-        float2 x0 = make_float2(a.x * inv, a.y * inv), x1 = make_float2(a.z * inv, a.w * inv);
         const int bt = idx / p.group, h = hk * p.group + (idx - bt * p.group);
-        const int d = d0 + 4 * q4;
-        if (p.gate) {
-            const int b = bt / p.T, t = bt - b * p.T;
-            const uint2 g = *reinterpret_cast<const uint2 *>(p.gate + (int64_t)b * p.g_seq + (int64_t)t * p.g_token + (int64_t)h * p.g_head + d);
-            const float2 s0 = gate2(g.x), s1 = gate2(g.y);
-            x0 = make_float2(x0.x * s0.x, x0.y * s0.y);
-            x1 = make_float2(x1.x * s1.x, x1.y * s1.y);
-        }
         const size_t orw = (size_t)bt * p.H + h;
-        *reinterpret_cast<uint2 *>(p.out + orw * HEAD_DIM + d) = make_uint2(pack_bf16x2(x0.x, x0.y), pack_bf16x2(x1.x, x1.y));
-        if (p.lse && d == 0) p.lse[orw] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+#pragma unroll
+        for (int chunk = 0; chunk < CHUNKS; chunk++) {
+            const int w0 = chunk * GROUPS, d = (blockIdx.y * CHUNKS + chunk) * MG_DIMS + 4 * q4;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = w0; w < w0 + GROUPS; w++) M = fmaxf(M, s_m[w][row]);
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = w0; w < w0 + GROUPS; w++) {
+                const float m = s_m[w][row];
+                if (m == -INFINITY) continue;
+                const float wt = ex2_approx(m - M);
+                const float4 o = s_o[w][q4][row];
+                L += wt * s_l[w][row];
+                a.x = fmaf(wt, o.x, a.x);
+                a.y = fmaf(wt, o.y, a.y);
+                a.z = fmaf(wt, o.z, a.z);
+                a.w = fmaf(wt, o.w, a.w);
+            }
+            const bool none = M == -INFINITY;
+            const float inv = none ? 0.0f : 1.0f / L;
+            float2 x0 = make_float2(a.x * inv, a.y * inv), x1 = make_float2(a.z * inv, a.w * inv);
+            if (p.gate) {
+                const int b = bt / p.T, t = bt - b * p.T;
+                const uint2 g = *reinterpret_cast<const uint2 *>(p.gate + (int64_t)b * p.g_seq + (int64_t)t * p.g_token + (int64_t)h * p.g_head + d);
+                const float2 s0 = gate2(g.x), s1 = gate2(g.y);
+                x0 = make_float2(x0.x * s0.x, x0.y * s0.y);
+                x1 = make_float2(x1.x * s1.x, x1.y * s1.y);
+            }
+            *reinterpret_cast<uint2 *>(p.out + orw * HEAD_DIM + d) = make_uint2(pack_bf16x2(x0.x, x0.y), pack_bf16x2(x1.x, x1.y));
+            if (p.lse && d == 0) p.lse[orw] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+        }
     }
 }
 
@@ -845,9 +849,15 @@ cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &
     // (with few rows the other form spreads them over more SMs: 64 rows of five partials take 6 us less)
     const int64_t blocks = (int64_t)p.Hkv * ((p.B * p.T * p.group + 31) / 32);
     const bool few = (np < p.prefix_tiles ? np : p.prefix_tiles) + (no < own_t ? no : own_t) <= MG_FEW && blocks >= MG_FEW_BLOCKS;
-    const dim3 grid((unsigned)blocks, few ? 1 : HEAD_DIM / MG_DIMS);
-    return few ? launch_dependent(shared_attn_merge_kernel<true>, grid, 32 * MG_WARPS, 0, stream, 1u, p)
-               : launch_dependent(shared_attn_merge_kernel<false>, grid, 32 * MG_WARPS, 0, stream, 1u, p);
+    // otherwise as few groups as give a CTA to every SM: fewer waves of CTAs, each with a chain of latencies of its own (1332
+    // rows of a head, eight partials: 42.5, 43.2, 43.9 us for the call with 2, 4, 8 groups)
+    int groups = few ? 1 : 8;
+    while (groups > 2 && blocks * (groups / 2) >= MG_CTAS) groups /= 2;
+    const dim3 grid((unsigned)blocks, (unsigned)groups);
+    if (groups == 1) return launch_dependent(shared_attn_merge_kernel<1>, grid, 32 * MG_WARPS, 0, stream, 1u, p);
+    if (groups == 2) return launch_dependent(shared_attn_merge_kernel<2>, grid, 32 * MG_WARPS, 0, stream, 1u, p);
+    if (groups == 4) return launch_dependent(shared_attn_merge_kernel<4>, grid, 32 * MG_WARPS, 0, stream, 1u, p);
+    return launch_dependent(shared_attn_merge_kernel<8>, grid, 32 * MG_WARPS, 0, stream, 1u, p);
 }
 
 }  // namespace mfc

@@ -137,6 +137,15 @@ def test_shared_prefix_attn(ctx, B, T, H, Hkv, P, cap):
     check_attn(ctx, q, gate, pk, pv, ok, ov, lens_for(g, B, T, cap))
 
 
+@pytest.mark.parametrize("B,T,H,Hkv,P,cap", [(64, 2, 32, 2, 400, 100), (37, 3, 24, 2, 1500, 90), (20, 2, 32, 2, 3000, 200), (4, 1, 32, 2, 20000, 30)])
+def test_shared_prefix_attn_with_many_and_few_rows_to_join(ctx, B, T, H, Hkv, P, cap):
+    """From 64 to 4096 query rows, from two to some seventy partials a row."""
+    g = gen(B + P)
+    q, pk, pv = rn(g, B, T, H, D), rn(g, Hkv, P, D), rn(g, Hkv, P, D)
+    ok, ov = rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    check_attn(ctx, q, q if B % 2 else None, pk, pv, ok, ov, lens_for(g, B, T, cap))
+
+
 def test_shared_prefix_attn_without_any_row(ctx):
     g = gen(1)
     q = rn(g, 3, 2, 32, D)
