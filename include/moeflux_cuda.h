@@ -519,9 +519,10 @@ int mfc_kv_evict_dev(mfc_ctx *ctx, const mfc_kv_evict *args);
  * max(p - q, 0) at the refused place, or from p behind the last draft when none
  * was refused: the lowest v whose cumulative weight exceeds u_sample[b] times the
  * total, sums in 64 bits.  If that residual is zero everywhere the token is drawn
- * from p; if p is zero too it is -1.  Entries that are negative or NaN count as
- * zero; an infinite total leaves -1.  draft_probs NULL: the drafts were not sampled (q is 1 at x_i).  A drafted
- * token outside [0, vocab) is refused.
+ * from p; if p is zero too it is -1.  Entries of p and of q that are negative or
+ * NaN count as zero, in the acceptance as in the residual; an infinite total
+ * leaves -1.  draft_probs NULL: the drafts were not sampled (q is 1 at x_i).  A
+ * drafted token outside [0, vocab) is refused.
  *   target_probs: fp32 [n_seqs][max_drafts + 1][vocab], draft_probs: fp32
  *     [n_seqs][max_drafts][vocab] by their strides;
  *   draft_tokens int32, u_accept fp32: [n_seqs][max_drafts];  u_sample [n_seqs];

@@ -28,9 +28,10 @@ constexpr int VD_MIN_SEG = 128, VD_SEG = 1024;  // entries of a segment: at leas
 constexpr int VD_MAX_SEGS = 512;  // segments of a CTA's run kept in shared memory; longer runs use longer segments
 constexpr int VD_MAX_CLUSTER = 8;
 
+// A negative or NaN probability counts as nothing, on either side of the difference (fmaxf takes the number beside a NaN).
 __device__ __forceinline__ double weight(float p, float q) {
-    const double w = (double)p - (double)q;
-    return w > 0.0 ? w : 0.0;  // negative and NaN count as nothing
+    const double w = (double)p - (double)fmaxf(q, 0.0f);
+    return w > 0.0 ? w : 0.0;  // false for a NaN p; a p that is not positive leaves nothing above any q
 }
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(VD_MAX_THREADS) verify_drafts_kernel(const Ver
             if (x >= 0 && x < p.V) {
                 const float px = p.p[(size_t)b * p.p_seq + (size_t)lane * p.p_row + x];
                 const float qx = p.q ? p.q[(size_t)b * p.q_seq + (size_t)lane * p.q_row + x] : 1.0f;
-                refused = !((double)p.u_accept[(size_t)b * p.K + lane] * (double)qx < (double)px);
+                refused = !((double)p.u_accept[(size_t)b * p.K + lane] * (double)fmaxf(qx, 0.0f) < (double)fmaxf(px, 0.0f));
             }
         }
         const unsigned m = __ballot_sync(0xffffffffu, refused);
