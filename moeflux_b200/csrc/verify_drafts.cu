@@ -196,9 +196,16 @@ __global__ void __launch_bounds__(VD_MAX_THREADS) verify_drafts_kernel(const Ver
             if (lane == 0) s_tot[pass] = t;
         }
         cluster.sync();
-        // every warp by itself, in the same order: the sum before this CTA's run, behind it, and behind all runs
+        // every warp by itself: the sum before this CTA's run, behind it, and behind all runs, added in the order of the
+        // runs, so that it never falls from one run to the next (a scan by doubling adds in another order for every lane:
+        // behind a run without weight its sum can be the smaller one in the last bit)
         const double t = lane < cs ? *cluster.map_shared_rank(&s_tot[pass], lane) : 0.0;
-        const double run = warp_scan_f64(t);
+        double run = 0.0;
+#pragma unroll
+        for (int r = 0; r < VD_MAX_CLUSTER; r++) {
+            const double of = __shfl_sync(0xffffffffu, t, r);
+            if (r <= lane) run += of;
+        }
         behind = __shfl_sync(0xffffffffu, run, rank);
         before = rank > 0 ? __shfl_sync(0xffffffffu, run, rank - 1) : 0.0;
         total = __shfl_sync(0xffffffffu, run, 31);
@@ -212,7 +219,7 @@ __global__ void __launch_bounds__(VD_MAX_THREADS) verify_drafts_kernel(const Ver
     int *tok = p.tokens + (size_t)b * (p.K + 1) + n;
     if (s1 > s0 && total > 0.0) {
         // the border lies in this CTA's run when the sum before the run does not exceed the target and the sum behind it
-        // does; all CTAs compare the same sums, so exactly one run qualifies
+        // does; all CTAs compare the same sums, which do not fall and end above the target, so exactly one run qualifies
         if (before <= target && behind > target) {
             // Four levels: the segment, a warp's part of it, a lane's, the entry.  Sums of the same entries in two orders may
             // differ in the last bit; where a level then finds no place, its last entry of any weight counts.  The first

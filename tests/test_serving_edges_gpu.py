@@ -42,3 +42,20 @@ def test_draft_probabilities_that_are_nan_or_negative_count_as_zero(ctx, V, pad)
     n, tok = call_verify(ctx, p, q, x, None, ua, torch.zeros(B, device="cuda"))
     assert n.tolist() == [r[4] for r in rows]
     assert tok.tolist() == [r[5] for r in rows]
+
+
+def test_a_border_on_the_last_bit_is_drawn_once(ctx):
+    """Weights whose sums differ in the last bit with the order of the additions, and a uniform that puts the border on that
+    bit, between two CTAs' runs of the row: either neighbour is right to rounding, but it is the same one every time."""
+    B, V = 64, 8192  # eight runs of 1024 entries
+    p = torch.zeros(B, 1, V, device="cuda")
+    for at, y in [(0, "0x1.577c720000000p+0"), (1024, "0x1.3d2b6a0000000p-35"), (2048, "0x1.d260f60000000p-30"),
+                  (3 * 1024 + 7, "0x1.7a01b20000000p-32"), (5120, "0x1.577c720000000p+0"), (5121, "0x1.1d655c0000000p-29")]:
+        p[:, 0, at] = float.fromhex(y)
+    x, ua, us = torch.zeros(B, 0, device="cuda", dtype=torch.int32), torch.zeros(B, 0, device="cuda"), torch.full((B,), 0.5, device="cuda")
+    seen = set()
+    for _ in range(50):
+        n, tok = call_verify(ctx, p, None, x, None, ua, us)
+        assert not n.any()
+        seen |= set(tok.flatten().tolist())
+    assert len(seen) == 1 and seen <= {3 * 1024 + 7, 5120}, seen
