@@ -409,9 +409,13 @@ int mfc_sdpa_static_status(void *stream);
 /* Where a full-attention layer's rows of one sequence live: *k and *v point at
  * row 0 of kv head 0; the next head starts *head_stride elements later, the
  * same layer's next sequence *seq_stride elements later, the next row 256
- * elements later; *len rows are in use (of the context's kv_dtype).  Rows up to
- * the layer's length may be read until the sequence is cleared, truncated or
- * reloaded. */
+ * elements later; *len rows are in use.  Rows up to the layer's length may be
+ * read until the sequence is cleared, truncated or reloaded.  The rows are of the
+ * context's kv_dtype (fp32 by default), the strides in elements of it: the two
+ * attention calls read bf16 and refuse the fp32 rows of their own context, and
+ * mfc_kv_evict_dev refuses its context's rows under another kv_dtype (rows of
+ * another context are not recognised).  With a KV split (kv_world > 1) these are
+ * the rows that this rank holds, in its own order. */
 int mfc_kv_cache_view(mfc_ctx *ctx, int32_t layer, int32_t seq_id, void **k, void **v,
                       int64_t *seq_stride, int64_t *head_stride, int32_t *len);
 

@@ -1489,6 +1489,18 @@ bool check_heads(mfc_ctx *c, int n_seqs, int n_tokens, int H, int Hkv, float sca
     if (!(scale > 0.0f) || !(scale < INFINITY)) return fail(c, "softmax_scale must be positive and finite");
     return true;
 }
+// Whether p points into the context's own cached rows (mfc_kv_cache_view), whose type is the context's.
+bool in_own_cache(const mfc_ctx *c, const void *p) {
+    const size_t bytes = (size_t)c->n_kv_slots * c->cfg.num_kv_heads * c->cap_rows * HEAD_DIM * c->kv_esize;
+    const uintptr_t at = (uintptr_t)p, k = (uintptr_t)c->k_cache, v = (uintptr_t)c->v_cache;
+    return (at >= k && at - k < bytes) || (at >= v && at - v < bytes);
+}
+// the attention calls read bf16 rows
+bool check_bf16_rows(mfc_ctx *c, const void *k, const void *v) {
+    if (c->cfg.kv_dtype == MFC_KV_F32 && (in_own_cache(c, k) || in_own_cache(c, v)))
+        return fail(c, "these are rows of the context's fp32 cache and the call reads bf16: open the context with MFC_KV_BF16");
+    return true;
+}
 bool strides8(int64_t a, int64_t b, int64_t d) { return a % 8 == 0 && b % 8 == 0 && d % 8 == 0; }
 
 // Map over cached bf16 rows, (64 dims, row, fourth of the 256 dims, kv head, sequence), boxes of `fourths` x box_rows rows:
@@ -1571,6 +1583,7 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
         fail(c, "strides must be multiples of 8 elements");
         return -1;
     }
+    if ((has_prefix && !check_bf16_rows(c, a->prefix_k, a->prefix_v)) || (has_own && !check_bf16_rows(c, a->own_k, a->own_v))) return -1;
     SharedAttnParams p;
     memset(&p, 0, sizeof(p));
     p.T = a->n_tokens;
@@ -1672,6 +1685,7 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *c, const mfc_attn_weights *a) try {
         fail(c, "the strides of q and k must be multiples of 8 elements");
         return -1;
     }
+    if (!check_bf16_rows(c, a->k, nullptr)) return -1;
     AttnWeightsParams p;
     memset(&p, 0, sizeof(p));
     p.q = (const __nv_bfloat16 *)a->q;
@@ -1748,6 +1762,10 @@ int mfc_kv_evict_dev(mfc_ctx *c, const mfc_kv_evict *a) try {
     }
     if (a->row_stride < HEAD_DIM) {
         fail(c, "rows must be at least 256 elements apart");
+        return -1;
+    }
+    if (a->kv_dtype != c->cfg.kv_dtype && (in_own_cache(c, a->k) || in_own_cache(c, a->v))) {
+        fail(c, "these are rows of the context's own cache, which are not of the call's kv_dtype");
         return -1;
     }
     EvictParams p;

@@ -59,3 +59,51 @@ def test_a_border_on_the_last_bit_is_drawn_once(ctx):
         assert not n.any()
         seen |= set(tok.flatten().tolist())
     assert len(seen) == 1 and seen <= {3 * 1024 + 7, 5120}, seen
+
+
+# ---------------------------------------------------------------------------------------------------- a context's own rows
+
+
+def test_rows_of_a_context_s_fp32_cache_are_refused_as_bf16(M):
+    """The view of a context that keeps fp32 rows (the default): the attention calls read bf16 and refuse it, eviction takes
+    it with its own type only; nothing is launched.  A bf16 context's rows stay open to all of them."""
+    g = gen(61)
+    q = rn(g, 1, 1, 32, D)
+    lens = torch.tensor([3], device="cuda", dtype=torch.int32)
+    rows = rn(g, 1, 2, 8, D)
+    out, lse = torch.zeros_like(q), torch.zeros(1, 1, 32, device="cuda")
+    w, pos = torch.zeros(1, 2, 64, device="cuda"), torch.zeros(1, 2, 64, device="cuda", dtype=torch.int32)
+    new = torch.zeros_like(lens)
+    for kv_dtype in (M.KV_F32, M.KV_BF16):
+        c = M.Ctx(num_layers=4, max_seq=64, n_seqs=2, kv_dtype=kv_dtype)
+        c.set_stream(torch.cuda.current_stream().cuda_stream)
+        k, v, seq_stride, head_stride, n = c.kv_cache_view(3, 1)
+        assert n == 0
+        attn = attn_args(q, None, None, None, rows, rows, lens, out, lse)
+        prefix = dict(prefix_head_stride=head_stride, prefix_row_stride=D, prefix_len=3)
+        own = dict(own_seq_stride=seq_stride, own_head_stride=head_stride, own_row_stride=D, own_cap=8)
+        wts = weights_args(q, rows, lens, lse, w)
+        ev = dict(n_seqs=1, num_kv_heads=2, cap=8, seq_stride=seq_stride, head_stride=head_stride, row_stride=D, budget=2, lens=lens.data_ptr(),
+                  next_pos=lens.data_ptr(), weights=w.data_ptr(), positions=pos.data_ptr(), map_seq_stride=128, map_head_stride=64,
+                  weights_out=w.data_ptr(), positions_out=pos.data_ptr(), lens_out=new.data_ptr())
+        r = rows.data_ptr()
+        calls = [lambda: c.shared_prefix_attn_dev(**attn, prefix_k=k, prefix_v=r, **prefix),
+                 lambda: c.shared_prefix_attn_dev(**attn, prefix_k=r, prefix_v=v, **prefix),
+                 lambda: c.shared_prefix_attn_dev(**{**attn, "own_k": k, **own}),
+                 lambda: c.shared_prefix_attn_dev(**{**attn, "own_v": v + 512, **own}),
+                 lambda: c.attn_weights_accumulate_dev(**{**wts, "k": k, "k_head_stride": head_stride, "cap": 8})]
+        before = c.launch_count
+        for call in calls:
+            if kv_dtype == M.KV_F32:
+                with pytest.raises(M.MfcError, match="fp32 cache"):
+                    call()
+            else:
+                call()
+        other = M.KV_BF16 if kv_dtype == M.KV_F32 else M.KV_F32
+        with pytest.raises(M.MfcError, match="kv_dtype"):
+            c.kv_evict_dev(**ev, k=k, v=v, kv_dtype=other)
+        assert c.launch_count == before + (0 if kv_dtype == M.KV_F32 else 9)
+        c.kv_evict_dev(**ev, k=k, v=v, kv_dtype=kv_dtype)
+        c.synchronize()
+        assert new.tolist() == [2]
+        c.close()
