@@ -107,3 +107,64 @@ def test_rows_of_a_context_s_fp32_cache_are_refused_as_bf16(M):
         c.synchronize()
         assert new.tolist() == [2]
         c.close()
+
+
+# ---------------------------------------------------------------------------------------------------- failures and captures
+
+
+@pytest.mark.parametrize("call", ["attn", "weights"])
+def test_a_call_after_a_lost_load_computes_what_it_should(ctx, M, call):
+    """The call that follows a failed one, the same entry point: its results against the 64-bit form."""
+    g = gen(62)
+    B, T, H, Hkv, P, cap = 3, 2, 32, 2, 700, 300
+    q, ok, ov = rn(g, B, T, H, D), rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    pk, pv = rn(g, Hkv, P, D), rn(g, Hkv, P, D)
+    lens = torch.tensor([300, 130, 5], device="cuda", dtype=torch.int32)
+    ro, rl, bo, bl = attn_ref(q, None, pk, pv, ok, ov, lens)
+    out, lse = torch.zeros(B, T, H, D, device="cuda", dtype=torch.bfloat16), torch.zeros(B, T, H, device="cuda")
+    given = rl.float().contiguous()
+    w = torch.zeros(B, Hkv, cap, device="cuda")
+    run = (lambda: ctx.shared_prefix_attn_dev(**attn_args(q, None, pk, pv, ok, ov, lens, out, lse))) if call == "attn" else (
+        lambda: ctx.attn_weights_accumulate_dev(**weights_args(q, ok, lens, given, w)))
+    ctx.set_tuning("gqa_wait_spins", 2000)
+    ctx.set_tuning("gqa_inject_lost_load", 1)
+    try:
+        run()
+        with pytest.raises(M.MfcError, match="did not arrive"):
+            ctx.synchronize()
+    finally:
+        ctx.set_tuning("gqa_inject_lost_load", 0)
+        ctx.set_tuning("gqa_wait_spins", 0)
+    for t in (out, lse):
+        t.fill_(float("nan"))
+    w.zero_()
+    run()
+    ctx.synchronize()
+    if call == "attn":
+        assert ((out.double() - ro).abs() <= bo).all() and ((lse.double() - rl).abs() <= bl).all()
+    else:
+        ref, tol = weights_ref(q, ok, lens, given, torch.zeros_like(w), 1.0)
+        assert ((w.double() - ref).abs() <= tol).all()
+
+
+def test_the_lse_of_a_replayed_call_follows_the_lengths(ctx):
+    g = gen(63)
+    B, T, H, Hkv, P, cap = 20, 3, 32, 2, 0, 300
+    q, ok, ov = rn(g, B, T, H, D), rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    lens = lens_for(g, B, T, cap)
+    out, lse = torch.zeros_like(q), torch.zeros(B, T, H, device="cuda")
+    s, home = torch.cuda.Stream(), torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    ctx.set_stream(s.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        ctx.shared_prefix_attn_dev(**attn_args(q, None, None, None, ok, ov, lens, out, lse))
+    ctx.set_stream(home)
+    for cut in (0, 5, 130):
+        lens.copy_((lens - cut).clamp(min=0))
+        graph.replay()
+        torch.cuda.synchronize()
+        ro, rl, bo, bl = attn_ref(q, None, None, None, ok, ov, lens)
+        none = torch.isinf(rl)
+        assert torch.equal(torch.isneginf(lse), none) and none.any()
+        assert ((lse.double() - rl).abs()[~none] <= bl[~none]).all() and ((out.double() - ro).abs() <= bo).all()
