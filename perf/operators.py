@@ -270,18 +270,19 @@ def _plain_verify(s):
 # ---------------------------------------------------------------------------------------------------- the calls
 
 
-_ctx = None
+_ctxs = {}
 
 
 def _handle():
-    """The context a user's program keeps open; its work goes to torch's current stream."""
-    global _ctx
-    if _ctx is None:
+    """The context that a user's program keeps open for the current device and stream: its work is ordered by that stream."""
+    device = torch.cuda.current_device()
+    at = (device, torch._C._cuda_getCurrentRawStream(device))  # (a torch.cuda.Stream object of it takes 3 us to make)
+    if at not in _ctxs:
         import moeflux_b200 as M
 
-        _ctx = M.Ctx(num_layers=4, max_seq=64, kv_dtype=M.KV_BF16)
-        _ctx.set_stream(torch.cuda.current_stream().cuda_stream)
-    return _ctx
+        _ctxs[at] = M.Ctx(num_layers=4, max_seq=64, kv_dtype=M.KV_BF16, device=device)
+        _ctxs[at].set_stream(at[1])
+    return _ctxs[at]
 
 
 def _own_run(s):
