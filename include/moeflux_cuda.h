@@ -423,21 +423,33 @@ int mfc_kv_cache_view(mfc_ctx *ctx, int32_t layer, int32_t seq_id, void **k, voi
  * sequence b attends to all prefix_len prefix rows and to the sequence's own
  * rows j < own_lens[b] - (n_tokens - 1 - t): the n_tokens newest rows are the
  * step's own tokens, causal among themselves (n_tokens > 1: drafted tokens that
- * are being verified).  The prefix rows are stored once and read once for all
- * sequences.
+ * are being verified).  The prefix rows are stored once and read once per 128
+ * query rows of a kv head (n_seqs * n_tokens * heads per kv head of them), not once
+ * per sequence; a batch whose partial results exceed the context's scratch takes
+ * several launches, and each reads the prefix again.
  *   q, gate: bf16, element (b, t, h, d) at b*seq + t*token + h*head + d; q is
  *     post-RoPE; gate NULL = no sigmoid gate.
  *   prefix_k/_v: bf16 [kv head][prefix_len][256] by the two strides.
  *   own_k/_v: bf16 [seq][kv head][own_cap][256] by the three strides; rows at
  *     and beyond own_lens[b] are never used, whatever they hold.  Every row
  *     below own_lens[b] enters the products of all n_tokens queries, with weight
- *     zero where a query does not see it: V must be finite there.
+ *     zero where a query does not see it: V must be finite there.  V of any row is
+ *     below 2^64 (weights are summed up to 2^32 times too large before they are
+ *     normalised).
  *   own_lens: int32 [n_seqs] in device memory, the new rows included.
  *   out: bf16 [n_seqs][n_tokens][heads][256];  lse: fp32 [n_seqs][n_tokens][heads],
  *     ln sum exp of the scaled scores, or NULL.
+ * Scores, their exponentials, the sums and the partial results are fp32; each
+ * exponential is rounded to bf16 on its way into the product with V (the sum it is
+ * divided by takes it unrounded), and `out` is rounded once more.
  * A query that sees no row at all gets out = 0 and lse = -inf.  Strides are
- * multiples of 8, pointers 16-byte aligned.  1 <= n_tokens <= 16, n_seqs <= 4096,
- * at most 16 query heads per kv head, prefix_len and own_cap at most 2^30. */
+ * multiples of 8, those of cached rows positive and below 2^39, rows at least 256
+ * elements apart; pointers are 16-byte aligned.  1 <= n_tokens <= 16, n_seqs <= 4096,
+ * at most 16 query heads per kv head, prefix_len and own_cap at most 2^30.  Refused
+ * as well: one sequence alone with 2^26 or more tiles of 128 query rows x 128 cached
+ * rows (prefix_len = 2^30 with 8 kv heads), or with more partial results than the
+ * scratch reserved at open holds (num_kv_heads * ceil(n_tokens * heads per kv head /
+ * 128) up to 360 always fit). */
 typedef struct mfc_shared_prefix_attn {
     int32_t n_seqs, n_tokens, num_attn_heads, num_kv_heads;
     float softmax_scale;
@@ -467,8 +479,12 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *ctx, const mfc_shared_prefix_attn *args)
  * were.  lse is what mfc_shared_prefix_attn_dev returned, so weights taken with a
  * shared prefix are shares of the whole softmax.  q, k bf16, lse and weights
  * fp32.  decay = 0 starts the sums afresh: what `weights` holds is then not read.
- * Strides of q and k are multiples of 8, their pointers 16-byte aligned; cap is at
- * most 2^30. */
+ * Strides of q and k are multiples of 8, their pointers 16-byte aligned, the strides
+ * of k positive and below 2^39, rows at least 256 elements apart.  The limits on
+ * n_seqs, n_tokens and heads are those of the attention call; cap is at most 2^30,
+ * and n_seqs * num_kv_heads * ceil(cap / 128) below 2^30.  Up to 64 queries per kv
+ * head of a sequence (n_tokens * heads per kv head) the call runs at the speed of
+ * memory; with 256 it takes 2.4 times as long. */
 typedef struct mfc_attn_weights {
     int32_t n_seqs, n_tokens, num_attn_heads, num_kv_heads;
     float softmax_scale, decay;
@@ -498,8 +514,12 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *ctx, const mfc_attn_weights *args);
  *   weights_out, positions_out: same strides, may be weights and positions
  *     themselves; rows [0, min(lens[b], budget)) are written;
  *   lens, next_pos: int32 [n_seqs]; lens_out[b] = min(lens[b], budget), not lens.
- * cap <= MFC_EVICT_MAX_ROWS, pointers 16-byte aligned, K and V strides multiples
- * of 16 bytes. */
+ * cap <= MFC_EVICT_MAX_ROWS, n_seqs <= 4096, num_kv_heads <= 1024; pointers of K and V
+ * 16-byte aligned, their strides multiples of 16 bytes, rows at least 256 elements
+ * apart.  The moves of one sequence have to fit the scratch reserved at open
+ * (num_kv_heads * min(budget, cap - budget) up to 2^24 always do); more sequences
+ * than fit take several launches.  Rows of a context's own sequences can be evicted,
+ * but the context's lengths do not follow. */
 #define MFC_EVICT_MAX_ROWS 262144
 typedef struct mfc_kv_evict {
     int32_t n_seqs, num_kv_heads, kv_dtype, cap;

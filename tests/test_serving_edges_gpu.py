@@ -168,3 +168,48 @@ def test_the_lse_of_a_replayed_call_follows_the_lengths(ctx):
         none = torch.isinf(rl)
         assert torch.equal(torch.isneginf(lse), none) and none.any()
         assert ((lse.double() - rl).abs()[~none] <= bl[~none]).all() and ((out.double() - ro).abs() <= bo).all()
+
+
+# ---------------------------------------------------------------------------------------------------- limits
+
+
+def test_limits_beside_the_field_ranges_are_refused(ctx, M):
+    """Sizes whose single fields are in range: tiles, partial results and lists of moves of one sequence.  Refused on the host,
+    before anything is read."""
+    t = torch.zeros(4096, device="cuda", dtype=torch.bfloat16)
+    P = t.data_ptr()
+    q = dict(softmax_scale=SCALE, q=P, q_seq_stride=256, q_token_stride=256, q_head_stride=256)
+    prefix = dict(prefix_k=P, prefix_v=P, prefix_head_stride=256, prefix_row_stride=256, own_lens=P, out=P)
+    before = ctx.launch_count
+    with pytest.raises(M.MfcError, match="2\\^26"):
+        ctx.shared_prefix_attn_dev(**q, **prefix, n_seqs=1, n_tokens=1, num_attn_heads=8, num_kv_heads=8, prefix_len=1 << 30)
+    with pytest.raises(M.MfcError, match="scratch"):
+        ctx.shared_prefix_attn_dev(**q, **prefix, n_seqs=1, n_tokens=16, num_attn_heads=8192, num_kv_heads=1024, prefix_len=200)
+    with pytest.raises(M.MfcError, match="too many rows"):
+        ctx.attn_weights_accumulate_dev(**q, n_seqs=128, n_tokens=1, num_attn_heads=1, num_kv_heads=1, decay=1.0, k=P, k_seq_stride=256,
+                                        k_head_stride=256, k_row_stride=256, cap=1 << 30, lens=P, lse=P, weights=P)
+    with pytest.raises(M.MfcError, match="scratch"):
+        ctx.kv_evict_dev(n_seqs=1, num_kv_heads=1024, kv_dtype=M.KV_BF16, cap=262144, k=P, v=P + 512, seq_stride=256, head_stride=256, row_stride=256,
+                         budget=131072, lens=P, next_pos=P, weights=P, positions=P, map_seq_stride=1, map_head_stride=1, weights_out=P,
+                         positions_out=P, lens_out=P + 512)
+    assert ctx.launch_count == before
+
+
+def test_as_many_kv_heads_as_always_fit(ctx):
+    """360 tiles of query rows in one sequence, the number that the header promises."""
+    g = gen(64)
+    for T, H, Hkv in [(1, 360, 360), (16, 16 * 180, 180)]:
+        q = rn(g, 1, T, H, D)
+        pk, pv = rn(g, Hkv, 300, D), rn(g, Hkv, 300, D)
+        ok, ov = rn(g, 1, Hkv, 40, D), rn(g, 1, Hkv, 40, D)
+        check_attn(ctx, q, None, pk, pv, ok, ov, torch.tensor([37], device="cuda", dtype=torch.int32))
+
+
+def test_large_values_under_a_growing_maximum(ctx):
+    """V near 2^62, and scores that pass each row's first maximum by up to 2^32 and by more: nothing overflows."""
+    g = gen(65)
+    B, T, H, Hkv, P, cap = 5, 2, 32, 2, 1400, 200
+    q, pk, pv = rn(g, B, T, H, D, scale=2.0), rn(g, Hkv, P, D), rn(g, Hkv, P, D, scale=2.0 ** 60)
+    pk *= torch.linspace(0.2, 4.0, P, device="cuda").view(1, P, 1).to(torch.bfloat16)
+    ok, ov = rn(g, B, Hkv, cap, D, scale=5.0), rn(g, B, Hkv, cap, D, scale=2.0 ** 60)
+    check_attn(ctx, q, q, pk, pv, ok, ov, lens_for(g, B, T, cap))
