@@ -7,8 +7,13 @@
 // tcgen05.mma, so a thread owns a cached row, reads its scores for all queries from tensor memory and sums their
 // exponentials without exchanging anything; N is a multiple of 16, so no query slot of a group of 12 heads times three
 // tokens is wasted on a tile of 128.  With 16 queries a tile of 64 KiB takes 128 tensor cycles, with 256 it takes 2048;
-// HBM needs about 2800 to deliver it: HBM-bound throughout.  (The first form ran the same products on mma.sync
-// m16n8k16 with the rows loaded straight into fragments: as fast for 16 queries, twice as long for 64.)
+// HBM needs about 2800 to deliver it.  Up to 64 queries a unit the call is HBM-bound, beyond it is not, because the queries
+// take the place of the ring: one query buffer in place of two, and with 256 a ring of two granules, one tile, so that no
+// rows are on their way while the products of the tile at hand run.  Caches of up to 32768 rows, 32 sequences x 2 kv heads,
+// 16, 64, 80, 128, 192, 256 queries a unit: 6.3, 6.1, 5.4, 4.6, 3.5, 2.5 TB/s (87, 90, 101, 119, 165, 216 us); 512 sequences of
+// up to 256 rows, where the queries weigh more than the rows: 2.3, 1.6, 1.1, 1.0 and, with 256, 0.8 TB/s.  (The first form ran the
+// same products on mma.sync m16n8k16 with the rows loaded straight into fragments: as fast for 16 queries, twice as long
+// for 64.)
 //
 // Work split: the 128-row tiles of all (sequence, kv head) units form one sequence, cut into equal runs, one persistent
 // CTA per run and SM; lengths are read on the device.  Every row belongs to exactly one thread: no atomics, the same bits

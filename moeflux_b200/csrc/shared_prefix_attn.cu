@@ -19,7 +19,8 @@
 // S 128, P twice 64 (bf16, the A operand of P V straight from tensor memory).  S is free again as soon as the softmax
 // has read it, so Q K^T of tile j+1 runs under the softmax of tile j, and P V of tile j under that of tile j+1.  The
 // reference that a row's exponents are taken against is the maximum of its first tile and moves, with a rescaling of O,
-// only when some score exceeds it by more than 2^32 (fp32 and bf16 have the exponents to spare, and no digits are lost):
+// only when some exponential would exceed 2^32 (bf16 has the exponents to spare, so has fp32 for 2^30 rows with V below 2^64,
+// and no digits are lost):
 // so no maximum stands before the exponentials of a tile; its rows' maxima are taken along with them, and the two halves
 // of a row ask one another with one barrier reduction whether either must move, which redoes the tile.  P is rounded to
 // bf16 (the type of V: both operands of one instruction have the same type); the row sums l are taken before that rounding.
@@ -104,8 +105,9 @@ __device__ __forceinline__ int own_tiles(const SharedAttnParams &p, int b) { ret
 // 44 us).  The choice minimises the longest CTA, counted in prefix tiles (2.3 thousand cycles): an own tile, whose rows come
 // from HBM and not from L2, is a quarter more; a further prefix segment 3 (writing the partial of 128 rows takes 4.3
 // thousand cycles), a further own segment 1 and its share of the same.  A split has to win by a fifteenth (64 x 4 tokens
-// over 32768 rows, where the estimates meet: 275 us dealt to all, 282 us split).  Every warp computes the plan by itself from
-// the lengths, 31 splits, one a lane.
+// over 32768 rows, where the estimates meet: 239 us dealt to all, 243 us split).  Elsewhere the two lie further apart (dealt to
+// all, split: 16 x 8192 rows 28.2, 22.7 us; 37 x 3 tokens x 10007 46.5, 40.9; 96 x 4 tokens x 4000 99, 82; 8 x 4 tokens x 4096
+// 23.5, 18.7).  Every warp computes the plan by itself from the lengths, 31 splits, one a lane.
 struct Plan {
     int run, unit_place, own_run;
     int total_own;
@@ -846,11 +848,15 @@ cudaError_t launch_shared_prefix_attn(const CUtensorMap &pk, const CUtensorMap &
     // partials a row has at most, about: the CTAs a unit is spread over, of the prefix and of the own rows
     const int64_t units_p = (int64_t)p.Hkv * p.prefix_mtiles, units_o = (int64_t)p.B * p.Hkv * p.own_mtiles;
     const int64_t own_t = (p.own_cap + SP_N - 1) / SP_N, np = p.grid / units_p + 2, no = p.grid / units_o + 2;
-    // (with few rows the other form spreads them over more SMs: 64 rows of five partials take 6 us less)
+    // One group a row where the partials are few and the rows fill the GPU (32 x 4 tokens, 300 + 2048 rows: 33.5 us against 35.0
+    // in groups; 96 x 4 tokens, 4000 + 1000: 82.5 against 85.0).  With few rows the groups spread them over more SMs, with many
+    // partials they shorten the chain of each (8 x 4 tokens x 4096 rows: 18.7 us in groups, 25.6 with one; 4 x 20000: 21.0, 44.9;
+    // 48 x 2 tokens of 16 heads x 16000: 37.2, 40.8).
     const int64_t blocks = (int64_t)p.Hkv * ((p.B * p.T * p.group + 31) / 32);
     const bool few = (np < p.prefix_tiles ? np : p.prefix_tiles) + (no < own_t ? no : own_t) <= MG_FEW && blocks >= MG_FEW_BLOCKS;
     // otherwise as few groups as give a CTA to every SM: fewer waves of CTAs, each with a chain of latencies of its own (1332
-    // rows of a head, eight partials: 42.5, 43.2, 43.9 us for the call with 2, 4, 8 groups)
+    // rows of a head, eight partials: 42.5, 43.2, 43.9 us for the call with 2, 4, 8 groups).  MG_CTAS: somewhat more than the 148
+    // SMs of a B200.
     int groups = few ? 1 : 8;
     while (groups > 2 && blocks * (groups / 2) >= MG_CTAS) groups /= 2;
     const dim3 grid((unsigned)blocks, (unsigned)groups);

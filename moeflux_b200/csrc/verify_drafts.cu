@@ -10,6 +10,9 @@
 // sequence, each a run of segments of 128 to 1024 entries; a warp sums a segment and keeps the sum in shared memory; the CTAs
 // exchange their totals through distributed shared memory, every CTA finds out whether the border lies in its run, and
 // the one that owns it re-reads the 1024 entries of that segment (from L2).  Order of all sums fixed by the sizes.
+// 128 sequences, 131072 entries, eight drafts: 26.5 us, 24.6 without draft probabilities; 64 x 262144, four drafts: 25.4 and
+// 23.8.  (A sequence without a refusal, or without draft probabilities, reads p alone and its cluster is done sooner; nothing
+// takes its place, the launch is one wave.)
 #include <cooperative_groups.h>
 
 #include <utility>
