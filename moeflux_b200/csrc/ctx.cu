@@ -1463,13 +1463,14 @@ int mfc_mla_sdpa_folded(mfc_ctx *c, int32_t num_heads, int32_t cache_len, float 
 // ---------------------------------------------------------------- serving a batch from cached rows
 
 namespace {
-// The context's device for the duration of a call; the caller's current device comes back afterwards.
+// The context's device for the duration of a call; the caller's current device comes back afterwards.  The device is set even
+// where it is the current one: only then has a host thread that has not used the GPU yet a driver context, which the
+// encoder of tensor maps asks for.
 struct DeviceScope {
     int before = -1;
     explicit DeviceScope(int dev) {
-        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
-        if (before != dev) cudaSetDevice(dev);
-        else before = -1;
+        if (cudaGetDevice(&before) != cudaSuccess || before == dev) before = -1;
+        cudaSetDevice(dev);
     }
     ~DeviceScope() {
         if (before >= 0) cudaSetDevice(before);
@@ -1633,12 +1634,12 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *c, const mfc_shared_prefix_attn *a) try 
         }
         per_launch = (per_launch + 1) / 2;
     }
+    DeviceScope dev(c->cfg.device);
     CUtensorMap m[4];
     memset(m, 0, sizeof(m));
     if (has_prefix && (!make_rows_map(c, &m[0], a->prefix_k, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 2, 128) ||
                        !make_rows_map(c, &m[1], a->prefix_v, a->prefix_len, a->prefix_row_stride, p.Hkv, a->prefix_head_stride, 1, 0, 4, 64)))
         return -1;
-    DeviceScope dev(c->cfg.device);
     const int64_t rows = (int64_t)p.T * p.H;
     for (int b0 = 0; b0 < a->n_seqs; b0 += per_launch) {
         const int n = a->n_seqs - b0 < per_launch ? a->n_seqs - b0 : per_launch;
@@ -1716,9 +1717,9 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *c, const mfc_attn_weights *a) try {
         fail(c, "too many rows in one call");
         return -1;
     }
+    DeviceScope dev(c->cfg.device);
     CUtensorMap k_map;
     if (!make_rows_map(c, &k_map, a->k, a->cap, a->k_row_stride, p.Hkv, a->k_head_stride, p.B, a->k_seq_stride, 2, 128)) return -1;
-    DeviceScope dev(c->cfg.device);
     CK(launch_attn_weights(k_map, p, c->n_sms, c->stream));
     c->launches += 1;
     return 0;

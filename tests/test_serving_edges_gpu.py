@@ -213,3 +213,34 @@ def test_large_values_under_a_growing_maximum(ctx):
     pk *= torch.linspace(0.2, 4.0, P, device="cuda").view(1, P, 1).to(torch.bfloat16)
     ok, ov = rn(g, B, Hkv, cap, D, scale=5.0), rn(g, B, Hkv, cap, D, scale=2.0 ** 60)
     check_attn(ctx, q, q, pk, pv, ok, ov, lens_for(g, B, T, cap))
+
+
+def test_calls_from_a_thread_that_has_not_used_the_gpu(ctx):
+    """The first thing a host thread does on the GPU is the call itself."""
+    import threading
+
+    g = gen(66)
+    B, T, H, Hkv, P, cap = 3, 2, 32, 2, 300, 100
+    q, pk, pv, ok, ov = rn(g, B, T, H, D), rn(g, Hkv, P, D), rn(g, Hkv, P, D), rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    lens = lens_for(g, B, T, cap)
+    out, lse, w = torch.zeros_like(q), torch.zeros(B, T, H, device="cuda"), torch.zeros(B, Hkv, cap, device="cuda")
+    torch.cuda.synchronize()
+    raised = []
+
+    def work(call):
+        try:
+            call()
+        except Exception as e:  # noqa: BLE001 - handed to the test's thread
+            raised.append(e)
+
+    for call in (lambda: ctx.shared_prefix_attn_dev(**attn_args(q, None, pk, pv, ok, ov, lens, out, lse)),
+                 lambda: ctx.attn_weights_accumulate_dev(**weights_args(q, ok, lens, lse, w))):
+        t = threading.Thread(target=work, args=(call,))
+        t.start()
+        t.join()
+    assert not raised, raised
+    ctx.synchronize()
+    ro, rl, bo, bl = attn_ref(q, None, pk, pv, ok, ov, lens)
+    assert ((out.double() - ro).abs() <= bo).all() and ((lse.double() - rl).abs() <= bl).all()
+    ref, tol = weights_ref(q, ok, lens, lse, torch.zeros_like(w), 1.0)
+    assert ((w.double() - ref).abs() <= tol).all()
