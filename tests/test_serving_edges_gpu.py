@@ -244,3 +244,40 @@ def test_calls_from_a_thread_that_has_not_used_the_gpu(ctx):
     assert ((out.double() - ro).abs() <= bo).all() and ((lse.double() - rl).abs() <= bl).all()
     ref, tol = weights_ref(q, ok, lens, lse, torch.zeros_like(w), 1.0)
     assert ((w.double() - ref).abs() <= tol).all()
+
+
+def test_a_capture_joined_from_two_streams(ctx):
+    """Inputs written on another stream of the same capture, just before the call and just after a call of the context: each call
+    follows both."""
+    g = gen(67)
+    B, T, H, Hkv, P, cap = 20, 2, 32, 2, 900, 200
+    src, pk, pv, ok, ov = rn(g, B, T, H, D), rn(g, Hkv, P, D), rn(g, Hkv, P, D), rn(g, B, Hkv, cap, D), rn(g, B, Hkv, cap, D)
+    q, other = torch.zeros_like(src), torch.zeros(1 << 27, device="cuda")
+    lens, lens2 = lens_for(g, B, T, cap), torch.zeros(B, device="cuda", dtype=torch.int32)
+    out, lse, w = torch.zeros_like(q), torch.zeros(B, T, H, device="cuda"), torch.zeros(B, Hkv, cap, device="cuda")
+    main, side, home = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    ctx.set_stream(side.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        other.add_(1)  # (some 0.2 ms, so that a call that does not wait for what follows is seen)
+        q.copy_(src)
+        side.wait_stream(main)
+        ctx.shared_prefix_attn_dev(**attn_args(q, None, pk, pv, ok, ov, lens, out, lse))
+        other.add_(1)
+        lens2.copy_(lens)
+        side.wait_stream(main)
+        ctx.attn_weights_accumulate_dev(**weights_args(q, ok, lens2, lse, w))
+        main.wait_stream(side)
+    ctx.set_stream(home)
+    for _ in range(2):
+        src.copy_(rn(g, B, T, H, D))
+        w.zero_()
+        lens2.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ro, rl, bo, bl = attn_ref(src, None, pk, pv, ok, ov, lens)
+        assert ((out.double() - ro).abs() <= bo).all() and ((lse.double() - rl).abs() <= bl).all()
+        ref, tol = weights_ref(src, ok, lens, lse, torch.zeros_like(w), 1.0)
+        assert ((w.double() - ref).abs() <= tol).all() and bool((w > 0).any())
