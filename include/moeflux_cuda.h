@@ -480,7 +480,8 @@ int mfc_shared_prefix_attn_dev(mfc_ctx *ctx, const mfc_shared_prefix_attn *args)
  * shared prefix are shares of the whole softmax.  q, k bf16, lse and weights
  * fp32.  decay = 0 starts the sums afresh: what `weights` holds is then not read.
  * Strides of q and k are multiples of 8, their pointers 16-byte aligned, the strides
- * of k positive and below 2^39, rows at least 256 elements apart.  The limits on
+ * of k positive and below 2^39, rows at least 256 elements apart; the places of
+ * `weights` that different sequences and kv heads use are different.  The limits on
  * n_seqs, n_tokens and heads are those of the attention call; cap is at most 2^30,
  * and n_seqs * num_kv_heads * ceil(cap / 128) below 2^30.  Up to 64 queries per kv
  * head of a sequence (n_tokens * heads per kv head) the call runs at the speed of
@@ -516,7 +517,7 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *ctx, const mfc_attn_weights *args);
  *   lens, next_pos: int32 [n_seqs]; lens_out[b] = min(lens[b], budget), not lens.
  * cap <= MFC_EVICT_MAX_ROWS, n_seqs <= 4096, num_kv_heads <= 1024; pointers of K and V
  * 16-byte aligned, their strides multiples of 16 bytes, rows at least 256 elements
- * apart.  The moves of one sequence have to fit the scratch reserved at open
+ * apart; no two sequences or kv heads share rows, weights or positions.  The moves of one sequence have to fit the scratch reserved at open
  * (num_kv_heads * min(budget, cap - budget) up to 2^24 always do); more sequences
  * than fit take several launches.  Rows of a context's own sequences can be evicted,
  * but the context's lengths do not follow. */

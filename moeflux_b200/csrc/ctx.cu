@@ -1502,6 +1502,10 @@ bool check_bf16_rows(mfc_ctx *c, const void *k, const void *v) {
         return fail(c, "these are rows of the context's fp32 cache and the call reads bf16: open the context with MFC_KV_BF16");
     return true;
 }
+// arrays that a call writes: two sequences or kv heads in one place would be written by two CTAs at once
+bool share_a_place(int seqs, int64_t seq_stride, int heads, int64_t head_stride) {
+    return (seqs > 1 && seq_stride == 0) || (heads > 1 && head_stride == 0);
+}
 bool strides8(int64_t a, int64_t b, int64_t d) { return a % 8 == 0 && b % 8 == 0 && d % 8 == 0; }
 
 // Map over cached bf16 rows, (64 dims, row, fourth of the 256 dims, kv head, sequence), boxes of `fourths` x box_rows rows:
@@ -1717,6 +1721,10 @@ int mfc_attn_weights_accumulate_dev(mfc_ctx *c, const mfc_attn_weights *a) try {
         fail(c, "too many rows in one call");
         return -1;
     }
+    if (share_a_place(a->n_seqs, a->weights_seq_stride, a->num_kv_heads, a->weights_head_stride)) {
+        fail(c, "weights of different sequences and kv heads must lie in different places: a stride of 0");
+        return -1;
+    }
     DeviceScope dev(c->cfg.device);
     CUtensorMap k_map;
     if (!make_rows_map(c, &k_map, a->k, a->cap, a->k_row_stride, p.Hkv, a->k_head_stride, p.B, a->k_seq_stride, 2, 128)) return -1;
@@ -1763,6 +1771,11 @@ int mfc_kv_evict_dev(mfc_ctx *c, const mfc_kv_evict *a) try {
     }
     if (a->row_stride < HEAD_DIM) {
         fail(c, "rows must be at least 256 elements apart");
+        return -1;
+    }
+    if (share_a_place(a->n_seqs, a->seq_stride, a->num_kv_heads, a->head_stride) ||
+        share_a_place(a->n_seqs, a->map_seq_stride, a->num_kv_heads, a->map_head_stride)) {
+        fail(c, "rows and weights of different sequences and kv heads must lie in different places: a stride of 0");
         return -1;
     }
     if (a->kv_dtype != c->cfg.kv_dtype && (in_own_cache(c, a->k) || in_own_cache(c, a->v))) {

@@ -281,3 +281,25 @@ def test_a_capture_joined_from_two_streams(ctx):
         assert ((out.double() - ro).abs() <= bo).all() and ((lse.double() - rl).abs() <= bl).all()
         ref, tol = weights_ref(src, ok, lens, lse, torch.zeros_like(w), 1.0)
         assert ((w.double() - ref).abs() <= tol).all() and bool((w > 0).any())
+
+
+def test_written_arrays_that_sequences_or_heads_would_share_are_refused(ctx, M):
+    """A stride of 0 along an axis of more than one place, in what a call writes; along an axis of one it means nothing."""
+    k, v = (torch.zeros(2, 2, 8, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    w, pos = torch.zeros(2, 2, 8, device="cuda"), torch.zeros(2, 2, 8, device="cuda", dtype=torch.int32)
+    lens, new = torch.zeros(2, device="cuda", dtype=torch.int32), torch.zeros(2, device="cuda", dtype=torch.int32)
+    q, lse = torch.zeros(2, 1, 2, D, device="cuda", dtype=torch.bfloat16), torch.zeros(2, 1, 2, device="cuda")
+    ev = dict(n_seqs=2, num_kv_heads=2, kv_dtype=M.KV_BF16, cap=8, k=k.data_ptr(), v=v.data_ptr(), seq_stride=k.stride(0), head_stride=k.stride(1),
+              row_stride=D, budget=2, lens=lens.data_ptr(), next_pos=lens.data_ptr(), weights=w.data_ptr(), positions=pos.data_ptr(),
+              map_seq_stride=16, map_head_stride=8, weights_out=w.data_ptr(), positions_out=pos.data_ptr(), lens_out=new.data_ptr())
+    wts = weights_args(q, k, lens, lse, w)
+    before = ctx.launch_count
+    for fn, base, bad in [(ctx.kv_evict_dev, ev, ["seq_stride", "head_stride", "map_seq_stride", "map_head_stride"]),
+                          (ctx.attn_weights_accumulate_dev, wts, ["weights_seq_stride", "weights_head_stride"])]:
+        for field in bad:
+            with pytest.raises(M.MfcError, match="different places"):
+                fn(**{**base, field: 0})
+    assert ctx.launch_count == before
+    ctx.kv_evict_dev(**{**ev, "n_seqs": 1, "seq_stride": 0, "map_seq_stride": 0})
+    ctx.attn_weights_accumulate_dev(**{**wts, "n_seqs": 1, "weights_seq_stride": 0})
+    ctx.synchronize()
